@@ -141,7 +141,8 @@ def work(c):
     if c["op"] == "norm":
         cells = c["rows"] * c["cols"]
         # x, residual, their sum, the codes' values, weights and scales.
-        return {"bytes": cells * (b * (3 if c["residual"] else 1) + b) + c["cols"] * b + 4 * c["rows"], "flops": 6 * cells}
+        values = 2 if c["x"] == "f16" else 4
+        return {"bytes": cells * (b * (3 if c["residual"] else 1) + values) + c["cols"] * b + 4 * c["rows"], "flops": 6 * cells}
     row = c["heads"] * c["dim"]
     fresh = sum(new for length, new in _sequences(c) if length)
     if c["op"] == "write":
@@ -173,7 +174,8 @@ def prepare(case, seed):
         # A few channels carry much larger values than the rest, as a residual stream's do.
         loud = 1 + 30 * (torch.rand((n,), generator=g, device="cuda") < 0.002).float() * torch.rand((n,), generator=g, device="cuda")
         return {"op": "norm", "x": (normal(m, n) * 0.3).to(x), "residual": (normal(m, n) * loud).to(x) if case["residual"] else None,
-                "weight": (1 + 0.2 * normal(n)).to(x), "zero": torch.zeros(m, dtype=torch.int8, device="cuda"), "type": x}
+                "weight": (1 + 0.2 * normal(n)).to(x), "zero": torch.zeros(m, dtype=torch.int8, device="cuda"), "type": x,
+                "values": x if x is torch.float16 else torch.float32}    # what dequantize_linear has
 
     rng = random.Random(seed)
     heads, dim, page, group = case["heads"], case["dim"], case["page"], case.get("group", 4)
@@ -221,7 +223,7 @@ def _own(s):
     from nnops_b200 import ops
     if s["op"] == "norm":
         made = ops.rms_norm_i8(s["x"], s["weight"], residual=s["residual"], eps=_EPS)
-        return (ops.dequantize_linear(made[0], made[1], s["zero"], axis=-1, out_dtype=s["type"]), *made[1:])
+        return (ops.dequantize_linear(made[0], made[1], s["zero"], axis=-1, out_dtype=s["values"]), *made[1:])
     cache = s.get("cache")
     if cache is None:
         cache = s["cache"] = ops.CacheI8(s["k"], s["v"], s["k_scale"], s["v_scale"])
@@ -241,7 +243,7 @@ def _plain_norm(s):
     top = t.abs().amax(dim=1, keepdim=True)
     codes = torch.round(t * (torch.full_like(top, 127.0) / top))
     scale = (top.double() * torch.rsqrt(h.double().square().mean(dim=1, keepdim=True) + _EPS) / 127).float()
-    out = ((codes * scale).to(s["type"]), scale[:, 0])
+    out = ((codes * scale).to(s["values"]), scale[:, 0])
     return out if s["residual"] is None else (*out, h.to(s["type"]))
 
 
