@@ -464,6 +464,122 @@ NNB200_API int nnb200_quantize_linear(const nnb200_quant_linear_args* args, void
 NNB200_API int nnb200_dequantize_linear(const nnb200_quant_linear_args* args, void* stream);
 
 /*
+ * What stands between two int8 products of a transformer block.  No counterpart in the reference's CUDA backend.
+ * Floating operands are f32, f16 or bf16.
+ */
+#define NNB200_FLOAT_F32 0
+#define NNB200_FLOAT_F16 1
+#define NNB200_FLOAT_BF16 2
+
+/*
+ * RMS norm into 8 bits, with the residual's addition: per row
+ *   h = x + residual                       (f32; the statistics are of h before it is rounded)
+ *   residual_out = h                       (rounded to the rows' type)
+ *   t = h * weight,  top = max(max_i |t_i|, 2^-100)
+ *   out = round_half_even(t * (127 / top)) (f32, each step rounded once; the codes need no sum)
+ *   scale = top / (127 * sqrt(mean_i h_i^2 + eps))
+ * so out * scale is the normalised row, and (out, scale) are A and scale_a of nnb200_gemm_i8.  A row with a
+ * NaN or an infinity in t gets scale NaN and codes 0.  residual_out may be x or residual itself (same
+ * strides); no other output may overlap an input.  Strides are row strides in elements.
+ */
+typedef struct nnb200_rms_norm_i8_args {
+    const void* x;        /* [rows][cols] */
+    const void* residual; /* may be NULL */
+    const void* weight;   /* [cols] */
+    void* out;            /* s8 [rows][cols] */
+    float* scale;         /* [rows] */
+    void* residual_out;   /* may be NULL */
+    int64_t rows, cols;
+    int64_t x_stride, residual_stride, out_stride, residual_out_stride;
+    float eps;
+    int32_t float_type;   /* of x, residual and residual_out */
+    int32_t weight_type;  /* float_type, or NNB200_FLOAT_F32 */
+} nnb200_rms_norm_i8_args;
+
+NNB200_API int nnb200_rms_norm_i8(const nnb200_rms_norm_i8_args* args, void* stream);
+
+/*
+ * A key/value cache in 8 bits: s8 codes in pages of page_tokens tokens (16, 32, 64 or 128), one f32 scale for
+ * each page and head; a value is code * scale.  Token t of sequence b lies in page page_table[b][t / page_tokens].
+ * lens[b] counts the sequence's tokens with the call's new ones; the call's rows cu[b] .. cu[b + 1] are the last
+ * ones of sequence b, in order; cu NULL: rows / seqs rows for every sequence.  A sequence may have no row; more
+ * rows than tokens: the first of them stand before the sequence and have no token.  Rows from cu[seqs] on belong to
+ * nobody and are left as they are.  A length beyond the table counts as the table's reach, a negative one as 0.
+ *
+ * page_table, lens and cu are device arrays, so that a captured call follows them.  They are checked where they
+ * are used: a page outside 0 .. pages - 1 is never touched, what a call wanted of it is left out (a write drops the
+ * token, a read gives zeros, attention does not see its keys), and NNB200_DEVICE_ERROR_BAD_PAGE (9) is recorded for
+ * nnb200_take_device_error; rows outside 0 .. rows - 1 are ignored.
+ */
+#define NNB200_DEVICE_ERROR_BAD_PAGE 9
+typedef struct nnb200_cache_i8 {
+    void* k;                    /* s8 [pages][heads][page_tokens][dim], 16-byte aligned */
+    void* v;
+    float* k_scale;             /* [pages][heads] */
+    float* v_scale;
+    int64_t pages;
+    int64_t page_stride;        /* codes from page to page; a multiple of 16, at least heads * page_tokens * dim */
+    int64_t scale_page_stride;  /* scales from page to page */
+    int64_t heads, page_tokens;
+    int64_t dim;                /* a multiple of 16, up to 256 */
+    const int32_t* page_table;  /* [seqs][table_pages], rows table_stride entries apart */
+    int64_t table_stride, table_pages;
+    const int32_t* lens;        /* [seqs] */
+    const int32_t* cu;          /* [seqs + 1], or NULL */
+    int64_t seqs, rows;
+} nnb200_cache_i8;
+
+/*
+ * Write quantises the rows into the cache; read gives the rows' values back.
+ *
+ * Write: a page whose first token is among the call's begins anew, with scale = need, where
+ * need = max(max |x| / 127, 2^-60) over the page's new tokens of that head.  Any other page keeps
+ * what it holds: scale = max(scale, need), and if that has grown every code of the page and head that is
+ * not overwritten becomes round_half_even(code * (old / new)).  New codes: round_half_even(x * (1 / scale)).  A NaN or
+ * an infinity among the new values makes the page's scale NaN until it begins anew: every value of it then reads as NaN.
+ * A page that a call writes belongs to one sequence, and stands once in its row of the table: otherwise what
+ * it holds afterwards is not defined.
+ */
+typedef struct nnb200_cache_rows_args {
+    nnb200_cache_i8 cache;
+    void* k;                  /* [rows][heads][dim], dense along dim; write: const */
+    void* v;
+    int64_t k_stride_row, k_stride_head, v_stride_row, v_stride_head; /* elements */
+    int32_t float_type;
+} nnb200_cache_rows_args;
+
+NNB200_API int nnb200_cache_write_i8(const nnb200_cache_rows_args* args, void* stream);
+NNB200_API int nnb200_cache_read_i8(const nnb200_cache_rows_args* args, void* stream);
+
+/*
+ * Attention over the cache: row r of sequence b, at position p = lens[b] - (its rows) + (its place among them),
+ * and query head a over the keys and values of head a / (q_heads / heads):
+ *   out = sum_j softmax_j(scale * q . k_j) v_j   over the visible tokens j < lens[b]:
+ *   causal: j <= p, and with window > 0 also j > p - window or j < sinks; else all of them.
+ * A row that sees no token gives zeros.  dim 64, 96, 128 or 256.  The products take q and the softmax weights as f16,
+ * each row's q scaled by a power of two (f32 q: as the sum of two f16 values, 2^-22 of the row's largest), codes exactly, and
+ * sum in f32; the softmax is f32.  A block whose v scale is under 2^-60 counts as having that scale.
+ * The workspace (16-byte aligned device memory) is dead when the call's work has completed on the stream.
+ */
+typedef struct nnb200_attention_i8_args {
+    nnb200_cache_i8 cache;
+    const void* q;            /* [rows][q_heads][dim], dense along dim */
+    void* out;
+    int64_t q_stride_row, q_stride_head, out_stride_row, out_stride_head; /* elements */
+    int64_t q_heads;
+    int64_t window, sinks;    /* 0 = no window */
+    float scale;
+    int32_t causal;
+    int32_t float_type;       /* of q and out */
+    int32_t force_engine;     /* 0 auto, 1 rows on warp MMAs */
+    void* workspace;
+    size_t workspace_bytes;
+} nnb200_attention_i8_args;
+
+NNB200_API size_t nnb200_attention_i8_workspace_bytes(const nnb200_attention_i8_args* args);
+NNB200_API int nnb200_attention_i8(const nnb200_attention_i8_args* args, void* stream);
+
+/*
  * Column-sharded Linear, reassembly step: `gathered` holds `shards` dense slabs
  * [shards][m][row_bytes_per_shard] (what an all-gather of per-rank [m, n/shards] outputs
  * produces); writes the row-major [m][shards*row_bytes_per_shard] matrix with row pitch

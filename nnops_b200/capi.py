@@ -121,6 +121,45 @@ class Conv2dI8Args(C.Structure):
     ]
 
 
+class RmsNormI8Args(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("out", C.c_void_p), ("scale", C.c_void_p),
+        ("residual_out", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64),
+        ("x_stride", C.c_int64), ("residual_stride", C.c_int64), ("out_stride", C.c_int64), ("residual_out_stride", C.c_int64),
+        ("eps", C.c_float), ("float_type", C.c_int32), ("weight_type", C.c_int32),
+    ]
+
+
+# nnb200_cache_i8, which stands first in the blocks of the calls over a cache.
+_CACHE_FIELDS = [
+    ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+    ("pages", C.c_int64), ("page_stride", C.c_int64), ("scale_page_stride", C.c_int64),
+    ("heads", C.c_int64), ("page_tokens", C.c_int64), ("dim", C.c_int64),
+    ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int64),
+    ("lens", C.c_void_p), ("cu", C.c_void_p), ("seqs", C.c_int64), ("rows", C.c_int64),
+]
+
+
+class CacheRowsArgs(C.Structure):
+    _fields_ = _CACHE_FIELDS + [
+        ("rows_k", C.c_void_p), ("rows_v", C.c_void_p),
+        ("k_stride_row", C.c_int64), ("k_stride_head", C.c_int64), ("v_stride_row", C.c_int64), ("v_stride_head", C.c_int64),
+        ("float_type", C.c_int32),
+    ]
+
+
+class AttentionI8Args(C.Structure):
+    _fields_ = _CACHE_FIELDS + [
+        ("q", C.c_void_p), ("out", C.c_void_p),
+        ("q_stride_row", C.c_int64), ("q_stride_head", C.c_int64), ("out_stride_row", C.c_int64), ("out_stride_head", C.c_int64),
+        ("q_heads", C.c_int64), ("window", C.c_int64), ("sinks", C.c_int64),
+        ("scale", C.c_float), ("causal", C.c_int32), ("float_type", C.c_int32), ("force_engine", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+FLOAT_F32, FLOAT_F16, FLOAT_BF16 = 0, 1, 2
+
 _FORMATS = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f", C.c_size_t: "N"}
 _packers: dict = {}
 
@@ -166,6 +205,11 @@ SYMBOLS = [
                                         C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
     ("nnb200_quantize_linear", C.c_int, [C.POINTER(QuantLinearArgs), C.c_void_p]),
     ("nnb200_dequantize_linear", C.c_int, [C.POINTER(QuantLinearArgs), C.c_void_p]),
+    ("nnb200_rms_norm_i8", C.c_int, [C.POINTER(RmsNormI8Args), C.c_void_p]),
+    ("nnb200_cache_write_i8", C.c_int, [C.POINTER(CacheRowsArgs), C.c_void_p]),
+    ("nnb200_cache_read_i8", C.c_int, [C.POINTER(CacheRowsArgs), C.c_void_p]),
+    ("nnb200_attention_i8_workspace_bytes", C.c_size_t, [C.POINTER(AttentionI8Args)]),
+    ("nnb200_attention_i8", C.c_int, [C.POINTER(AttentionI8Args), C.c_void_p]),
     ("nnb200_interleave_shards", C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int32, C.c_int64,
                                            C.c_void_p]),
     ("nnb200_rank_barrier", C.c_int, [C.POINTER(C.c_void_p), C.c_int32, C.c_int32, C.c_int64, C.c_void_p]),
@@ -251,6 +295,7 @@ def take_device_error() -> int:
 
 DEVICE_ERROR_SELFTEST = 7
 DEVICE_ERROR_PEER_WAIT = 8
+DEVICE_ERROR_BAD_PAGE = 9
 RANK_FLAG_BYTES = 64
 
 

@@ -1,0 +1,692 @@
+// Attention over a key/value cache in 8 bits, for few rows a sequence: the mathematics, the split and the kernel.
+//
+// For a row q of head a, tokens j, K-codes k_j with scale ks_j, V-codes v_j with scale vs_j (one of each for a page):
+//
+//     t_j = (q . k_j) ks_j c + log2 vs_j       c = scale * log2 e
+//     m = max_j t_j,  w_j = 2^(t_j - m) <= 1,  l = sum_j w_j / vs_j,  out = (sum_j w_j v_j) / l
+//
+// which is the softmax with each block's V scale moved into the exponent: the weights that meet the codes are then at
+// most 1 and the largest is 1 whatever the scales are, so that f16 holds them, and one exponential serves both sums.
+// One pass over the tokens, with the running maximum.
+//
+// A warp takes 16 tokens at a time and is on its own: it copies their codes into its part of shared memory
+// (cp.async.bulk; 16 tokens never leave a page, and one head's share of a page is contiguous), turns bytes into f16
+// integers, which is exact, and feeds mma.m16n8k16 with the TOKENS as the 16-row operand: eight query rows (the heads
+// of a group, a few proposed tokens) fill the narrow side, nothing is padded to 16 or 128.  The transposition between the
+// two products is one movmatrix for 8 x 8 weights.  The order along dim and along the tokens inside an MMA is
+// free, and chosen so that every thread's bytes are contiguous.
+//
+// Bound by the reading of the codes: D bytes of K and of V for a token and head, against some 300 instructions of a warp for
+// 16 tokens.
+//
+// The work of all sequences, row tiles and heads is one line of 16-token groups, cut into equal pieces, one for each block, so
+// that lengths of any mix keep every SM busy to the end.  A row tile of a head that is cut leaves (m, l, sums) in the
+// workspace, in a fixed order of blocks; a second kernel joins them, in that order: results do not depend on timing.
+#pragma once
+
+#include "cache_i8.cuh"
+
+namespace nnb200 {
+
+constexpr int kRowsWarps = 8;
+constexpr int kRowsThreads = 32 * kRowsWarps;
+
+// What a block leaves in the workspace: [0] the end or the middle of a row tile that began in an earlier
+// block, [1] the beginning of one that ends in a later block.
+struct RowsPiece {
+    int32_t kind;      // 0: nothing, 1: begins here, 2: neither begins nor ends, 3: ends
+    int32_t seq, head, tile;
+};
+
+struct RowsPlan {
+    int blocks;    // of the first kernel
+    int columns;   // query rows of a tile / 8
+    size_t bytes;  // of the workspace: the pieces, then their sums ([tile rows][dim], m and l of each row)
+};
+
+struct RowsCall {
+    nnb200_attention_i8_args a;
+    int32_t* error_word;
+    int group;           // query heads of a key head
+    float factor;        // scale * log2 e
+    RowsPiece* pieces;   // [blocks][2]
+    float* sums;         // [blocks][2][piece]
+};
+
+// One sequence's part of the line.
+struct SequenceWork {
+    SequenceRows s;
+    int sink_groups, first_group, groups;   // groups of a row tile: the sinks', then those from first_group on; 1 at least
+    int tiles;
+    int64_t total;
+};
+
+__device__ __forceinline__ SequenceWork sequence_work(const RowsCall& call, int b, int tile_rows)
+{
+    const nnb200_attention_i8_args& a = call.a;
+    SequenceWork w;
+    w.s = sequence_rows(a.cache, b);
+    int64_t low = a.window > 0 ? static_cast<int64_t>(w.s.len) - w.s.n - a.window + 1 : 0;
+    low = low < 0 ? 0 : low;
+    w.first_group = static_cast<int>(low < w.s.len ? low : w.s.len) / 16;
+    const int sinks = static_cast<int>(a.sinks < w.s.len ? a.sinks : w.s.len);
+    w.sink_groups = a.window > 0 ? min((sinks + 15) / 16, w.first_group) : 0;
+    w.groups = max(w.sink_groups + (w.s.len + 15) / 16 - w.first_group, 1);
+    w.tiles = (w.s.n * call.group + tile_rows - 1) / tile_rows;
+    w.total = static_cast<int64_t>(a.cache.heads) * w.tiles * w.groups;
+    return w;
+}
+
+// ---- pieces of the MMAs ---------------------------------------------------------------------
+
+// Bytes of a word (signed) as f16 pairs: (0, 1) and (2, 3).  0x6400 | u is 1024 + u; u = byte + 128.
+__device__ __forceinline__ uint32_t half2_minus(uint32_t v)
+{
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void codes_to_half(uint32_t word, uint32_t& low, uint32_t& high)
+{
+    const uint32_t u = word ^ 0x80808080u;
+    low = half2_minus(__byte_perm(u, 0x64646464u, 0x4140));
+    high = half2_minus(__byte_perm(u, 0x64646464u, 0x4342));
+}
+// Bytes i of x and of y as the pair (x_i, y_i).
+__device__ __forceinline__ void codes_to_half_pairs(uint32_t x, uint32_t y, uint32_t (&p)[4])
+{
+    x ^= 0x80808080u;
+    y ^= 0x80808080u;
+    const uint32_t a = __byte_perm(x, y, 0x5140), b = __byte_perm(x, y, 0x7362);
+    p[0] = half2_minus(__byte_perm(a, 0x64646464u, 0x4140));
+    p[1] = half2_minus(__byte_perm(a, 0x64646464u, 0x4342));
+    p[2] = half2_minus(__byte_perm(b, 0x64646464u, 0x4140));
+    p[3] = half2_minus(__byte_perm(b, 0x64646464u, 0x4342));
+}
+
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// WORDS 32-bit words from shared memory, p aligned to the largest power of two that divides their bytes (up to 16).
+template <int WORDS>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS])
+{
+    if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (WORDS % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < WORDS / 2; ++i) {
+            const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+            w[2 * i] = v.x, w[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        }
+    }
+}
+
+__device__ __forceinline__ float load_float(const void* p, int64_t i, int type)
+{
+    return type == NNB200_FLOAT_F32   ? static_cast<const float*>(p)[i]
+           : type == NNB200_FLOAT_F16 ? __half2float(static_cast<const __half*>(p)[i])
+                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_float(void* p, int64_t i, int type, float v)
+{
+    if (type == NNB200_FLOAT_F32) {
+        static_cast<float*>(p)[i] = v;
+    } else if (type == NNB200_FLOAT_F16) {
+        static_cast<__half*>(p)[i] = __float2half_rn(v);
+    } else {
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    }
+}
+
+// Bytes of shared memory: the warps' rings, which hold the warps' sums when a piece is joined; barriers; per-stage scales.
+template <int D, int NT>
+struct RowsShared {
+    static constexpr int kStageBytes = 2 * 16 * D;
+    static constexpr int kJoinBytes = kRowsWarps * 8 * NT * D * 4;
+    static constexpr int kWanted = NT == 1 && D <= 128 ? 96 * 1024 : 192 * 1024;
+    static constexpr int kStages = kWanted / (kRowsWarps * kStageBytes) > 8 ? 8 : kWanted / (kRowsWarps * kStageBytes);
+    static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
+    static constexpr int kBytes = kRing > kJoinBytes ? kRing : kJoinBytes;
+    static_assert(kStages >= 2 && kBytes <= 200 * 1024, "ring");
+};
+
+struct StageScales {
+    float k, v_log2, v_inv;
+    int there;
+};
+
+template <int D, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kRowsThreads, (NT == 1 && D <= 128) ? 2 : 1)
+attention_i8_rows_kernel(const RowsCall call)
+{
+    using Shared = RowsShared<D, NT>;
+    constexpr int kStages = Shared::kStages;
+    constexpr int kTile = 8 * NT;
+    constexpr int kParts = SPLIT ? 2 : 1;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ __align__(8) uint64_t full[kRowsWarps][kStages];
+    __shared__ StageScales scales[kRowsWarps][kStages];
+    __shared__ float join_m[kRowsWarps][kTile], join_l[kRowsWarps][kTile];
+    __shared__ int64_t scan[kRowsWarps + 1];
+    __shared__ int64_t found_base;
+    __shared__ int found_seq;
+    __shared__ int abort_flag;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int g = lane / 4, c = lane & 3;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < kRowsWarps * kStages; ++i) {
+            mbar_init(&full[0][0] + i, 1);
+        }
+        mbar_init_fence();
+    }
+    __syncthreads();
+    previous_kernel_done();
+    const nnb200_attention_i8_args& a = call.a;
+    const int seqs = static_cast<int>(a.cache.seqs);
+
+    // The line's length, and the sequence in which this block's piece begins.
+    const auto block_sum_before = [&](int64_t v, int64_t& total) {   // of the threads before this one
+        int64_t up = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t other = __shfl_up_sync(0xFFFFFFFFu, up, o);
+            up += lane >= o ? other : 0;
+        }
+        __syncthreads();
+        if (lane == 31) {
+            scan[warp] = up;
+        }
+        __syncthreads();
+        int64_t before = up - v;
+        total = 0;
+        for (int i = 0; i < kRowsWarps; ++i) {
+            before += i < warp ? scan[i] : 0;
+            total += scan[i];
+        }
+        return before;
+    };
+    int64_t line = 0;
+    for (int b0 = 0; b0 < seqs; b0 += kRowsThreads) {
+        const int b = b0 + static_cast<int>(threadIdx.x);
+        int64_t total;
+        (void)block_sum_before(b < seqs ? sequence_work(call, b, kTile).total : 0, total);
+        line += total;
+    }
+    // No fewer than a group a warp for a block.
+    const int64_t share_at_least = kRowsWarps;
+    const int64_t most = (line + share_at_least - 1) / share_at_least;
+    const int64_t blocks = most < gridDim.x ? most : gridDim.x;
+    RowsPiece* pieces = call.pieces + 2 * blockIdx.x;
+    if (static_cast<int64_t>(blockIdx.x) >= blocks) {
+        if (threadIdx.x < 2) {
+            pieces[threadIdx.x].kind = 0;
+        }
+        return;
+    }
+    int64_t at = line / blocks * blockIdx.x + line % blocks * blockIdx.x / blocks;
+    const int64_t end = line / blocks * (blockIdx.x + 1) + line % blocks * (blockIdx.x + 1) / blocks;
+    {
+        int64_t base = 0;
+        for (int b0 = 0; b0 < seqs; b0 += kRowsThreads) {
+            const int b = b0 + static_cast<int>(threadIdx.x);
+            const int64_t own = b < seqs ? sequence_work(call, b, kTile).total : 0;
+            int64_t total;
+            const int64_t first = base + block_sum_before(own, total);
+            if (first <= at && at < first + own) {
+                found_seq = b;
+                found_base = first;
+            }
+            base += total;
+        }
+        __syncthreads();
+    }
+    int seq = found_seq;
+    int64_t base = found_base;
+    int kinds[2] = {0, 0};
+
+    uint32_t issued = 0, taken = 0;   // 16-token groups of this warp
+    uint8_t* const my_ring = ring + warp * kStages * Shared::kStageBytes;
+    bool failed = false;
+
+    while (at < end) {
+        const SequenceWork work = sequence_work(call, seq, kTile);
+        if (at >= base + work.total) {
+            base += work.total;
+            ++seq;
+            continue;
+        }
+        const int64_t item = (at - base) / work.groups;
+        const int off = static_cast<int>((at - base) % work.groups);
+        const int head = static_cast<int>(item / work.tiles), tile = static_cast<int>(item % work.tiles);
+        const int64_t room = end - at;
+        const int count = static_cast<int>(work.groups - off < room ? work.groups - off : room);
+        at += count;
+
+        const int rows = min(kTile, work.s.n * call.group - tile * kTile);
+        const int first_pos = work.s.len - work.s.n;
+
+        // This thread's part of the query rows: row 8 nt + g, dims [c D / 4, + D / 4), in f16 scaled by a power of two.
+        uint32_t q[NT][kParts][D / 16][2];
+        float factor[NT][2];    // of the columns 2 c and 2 c + 1
+        int pos[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g;
+            const int global = tile * kTile + r;
+            const int64_t src = (work.s.row0 + global / call.group) * a.q_stride_row + (head * call.group + global % call.group) * a.q_stride_head + c * (D / 4);
+            float v[D / 4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+                v[i] = r < rows ? load_float(a.q, src + i, a.float_type) : 0.0f;
+                top = max(top, magnitude_bits(v[i]));
+            }
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            int e = a.float_type == NNB200_FLOAT_F16 ? 0 : static_cast<int>(top >> 23) - 127;
+            e = min(max(e, -100), 126);
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * call.factor;
+#pragma unroll
+            for (int w = 0; w < D / 16; ++w) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const float x = v[4 * w + 2 * p] * down, y = v[4 * w + 2 * p + 1] * down;
+                    const __half2 h = __floats2half2_rn(x, y);
+                    q[nt][0][w][p] = *reinterpret_cast<const uint32_t*>(&h);
+                    if constexpr (SPLIT) {
+                        const float2 f = __half22float2(h);
+                        q[nt][kParts - 1][w][p] = pack2<__half>(x - f.x, y - f.y);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                factor[nt][j] = __shfl_sync(0xFFFFFFFFu, up, (2 * c + j) * 4);
+                const int row = tile * kTile + nt * 8 + 2 * c + j;
+                pos[nt][j] = a.causal != 0 ? first_pos + min(row, tile * kTile + rows - 1) / call.group : 0x7FFFFFFF;
+            }
+        }
+        const int least_pos = a.causal != 0 ? first_pos + tile * kTile / call.group : 0x7FFFFFFF;
+        const int most_pos = a.causal != 0 ? first_pos + (tile * kTile + rows - 1) / call.group : 0x7FFFFFFF;
+
+        float m[NT][2], l[NT][2], o[NT][D / 16][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+            }
+        }
+
+        // This warp's groups of the piece: off + warp, off + warp + 8, ...
+        const int mine = count > warp ? (count - warp + kRowsWarps - 1) / kRowsWarps : 0;
+        const auto group_of = [&](int i) {
+            const int idx = off + warp + i * kRowsWarps;
+            return idx < work.sink_groups ? idx : idx - work.sink_groups + work.first_group;
+        };
+        int ahead_page = -1;           // lane i: of group (32-block of the next one to issue) + i
+        float ahead_k = 0.0f, ahead_v = 0.0f;
+        const auto issue = [&](int i) {
+            if ((i & 31) == 0) {
+                ahead_page = -1;
+                if (i + lane < mine && group_of(i + lane) * 16 < work.s.len) {
+                    ahead_page = page_at(a.cache, seq, group_of(i + lane) * 16 / static_cast<int>(a.cache.page_tokens), call.error_word);
+                    if (ahead_page >= 0) {
+                        const int64_t s = ahead_page * a.cache.scale_page_stride + head;
+                        ahead_k = a.cache.k_scale[s];
+                        ahead_v = a.cache.v_scale[s];
+                    }
+                }
+            }
+            const int page = __shfl_sync(0xFFFFFFFFu, ahead_page, i & 31);
+            const float ks = __shfl_sync(0xFFFFFFFFu, ahead_k, i & 31), vs = __shfl_sync(0xFFFFFFFFu, ahead_v, i & 31);
+            if (lane == 0) {
+                const uint32_t slot = issued % kStages;
+                const float sure = vs < kLeastCacheScale ? kLeastCacheScale : vs;
+                scales[warp][slot] = StageScales{ks, log2f(sure), __fdiv_rn(1.0f, sure), page >= 0 ? 1 : 0};
+                if (page >= 0) {
+                    uint8_t* dst = my_ring + slot * Shared::kStageBytes;
+                    const int64_t src = page * a.cache.page_stride +
+                                        (static_cast<int64_t>(head) * a.cache.page_tokens + group_of(i) * 16 % static_cast<int>(a.cache.page_tokens)) * D;
+                    mbar_expect_tx(&full[warp][slot], Shared::kStageBytes);
+                    bulk_load_1d(dst, static_cast<const uint8_t*>(a.cache.k) + src, 16 * D, &full[warp][slot]);
+                    bulk_load_1d(dst + 16 * D, static_cast<const uint8_t*>(a.cache.v) + src, 16 * D, &full[warp][slot]);
+                } else {
+                    mbar_arrive(&full[warp][slot]);
+                }
+            }
+            ++issued;
+        };
+        for (int i = 0; i < min(mine, kStages); ++i) {
+            issue(i);
+        }
+        for (int i = 0; i < mine; ++i) {
+            const uint32_t slot = taken % kStages;
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[warp][slot], taken / kStages & 1u, &abort_flag))) {
+                failed = true;
+                break;
+            }
+            ++taken;
+            __syncwarp();
+            const StageScales sc = scales[warp][slot];
+            if (sc.there != 0) {
+                const uint8_t* kp = my_ring + slot * Shared::kStageBytes;
+                const uint8_t* vp = kp + 16 * D;
+                float s[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                }
+                {
+                    uint32_t x[D / 16], y[D / 16];
+                    load_words(kp + g * D + c * (D / 4), x);
+                    load_words(kp + (g + 8) * D + c * (D / 4), y);
+#pragma unroll
+                    for (int w = 0; w < D / 16; ++w) {
+                        uint32_t f[4];
+                        codes_to_half(x[w], f[0], f[2]);
+                        codes_to_half(y[w], f[1], f[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                            for (int p = 0; p < kParts; ++p) {
+                                mma_16x8x16(s[nt], f[0], f[1], f[2], f[3], q[nt][p][w][0], q[nt][p][w][1]);
+                            }
+                        }
+                    }
+                }
+                const int key0 = group_of(i) * 16;
+                const bool all_seen = key0 + 15 < work.s.len && key0 + 15 <= least_pos &&
+                                      (a.window == 0 || key0 > most_pos - a.window || key0 + 15 < a.sinks);
+                uint32_t pb[NT][kParts][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    // Element e: token g (e < 2) or g + 8, column 2 c + (e & 1).
+                    float inv[4] = {sc.v_inv, sc.v_inv, sc.v_inv, sc.v_inv};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[nt][e] = __fmaf_rn(s[nt][e], sc.k * factor[nt][e & 1], sc.v_log2);
+                    }
+                    if (!all_seen) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + g + (e < 2 ? 0 : 8), at_pos = pos[nt][e & 1];
+                            const bool seen = key < work.s.len && key <= at_pos && (a.window == 0 || key > at_pos - a.window || key < a.sinks);
+                            s[nt][e] = seen ? s[nt][e] : -INFINITY;
+                            inv[e] = seen ? inv[e] : 0.0f;
+                        }
+                    }
+                    float alpha[2];
+                    bool grown = false;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float top = fmaxf(s[nt][j], s[nt][j + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                        const float next = fmaxf(m[nt][j], top);
+                        const float safe = next == -INFINITY ? 0.0f : next;
+                        grown = grown || next > m[nt][j];
+                        alpha[j] = exp2_fast(m[nt][j] - safe);
+                        m[nt][j] = next;
+                        s[nt][j] = exp2_fast(s[nt][j] - safe);
+                        s[nt][j + 2] = exp2_fast(s[nt][j + 2] - safe);
+                        l[nt][j] = __fmaf_rn(s[nt][j + 2], inv[j + 2], __fmaf_rn(s[nt][j], inv[j], l[nt][j] * alpha[j]));
+                    }
+                    if (__any_sync(0xFFFFFFFFu, grown)) {
+#pragma unroll
+                        for (int i2 = 0; i2 < D / 16; ++i2) {
+                            o[nt][i2][0] *= alpha[0];
+                            o[nt][i2][1] *= alpha[1];
+                            o[nt][i2][2] *= alpha[0];
+                            o[nt][i2][3] *= alpha[1];
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const __half2 h = __floats2half2_rn(s[nt][2 * j], s[nt][2 * j + 1]);
+                        pb[nt][0][j] = transposed_8x8(*reinterpret_cast<const uint32_t*>(&h));
+                        if constexpr (SPLIT) {
+                            const float2 f = __half22float2(h);
+                            pb[nt][kParts - 1][j] = transposed_8x8(pack2<__half>(s[nt][2 * j] - f.x, s[nt][2 * j + 1] - f.y));
+                        }
+                    }
+                }
+                uint32_t v0[D / 32], v1[D / 32], v2[D / 32], v3[D / 32];
+                load_words(vp + 2 * c * D + g * (D / 8), v0);
+                load_words(vp + (2 * c + 1) * D + g * (D / 8), v1);
+                load_words(vp + (2 * c + 8) * D + g * (D / 8), v2);
+                load_words(vp + (2 * c + 9) * D + g * (D / 8), v3);
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w) {
+                    uint32_t e0[4], e1[4];
+                    codes_to_half_pairs(v0[w], v1[w], e0);
+                    codes_to_half_pairs(v2[w], v3[w], e1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p) {
+                            mma_16x8x16(o[nt][2 * w], e0[0], e0[1], e1[0], e1[1], pb[nt][p][0], pb[nt][p][1]);
+                            mma_16x8x16(o[nt][2 * w + 1], e0[2], e0[3], e1[2], e1[3], pb[nt][p][0], pb[nt][p][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (i + kStages < mine) {
+                issue(i + kStages);
+            }
+        }
+        if (failed) {
+            if (lane == 0) {
+                atomicCAS(call.error_word, 0, kErrProducerWait);
+                if (!drain_ring(full[warp], kStages, issued)) {
+                    atomicCAS(call.error_word, 0, kErrDrainWait);
+                }
+            }
+            taken = issued;
+            __syncwarp();
+        }
+
+        // The warps' sums, joined through the ring: every copy into it has been taken.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], 4);
+                l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], 8);
+                l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], 16);
+                if (g == 0) {
+                    join_m[warp][nt * 8 + 2 * c + j] = m[nt][j];
+                    join_l[warp][nt * 8 + 2 * c + j] = l[nt][j];
+                }
+            }
+        }
+        __syncthreads();
+        float* join_o = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                float* dst = join_o + (warp * kTile + nt * 8 + 2 * c) * D + g * (D / 8) + 2 * i;
+                *reinterpret_cast<float2*>(dst) = make_float2(o[nt][i][0], o[nt][i][2]);
+                *reinterpret_cast<float2*>(dst + D) = make_float2(o[nt][i][1], o[nt][i][3]);
+            }
+        }
+        __syncthreads();
+        const bool begins = off == 0, ends = off + count == work.groups;
+        const int which = begins ? 1 : 0;
+        float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kTile * (D + 2));
+        for (int i = threadIdx.x; i < rows * (D / 4); i += kRowsThreads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float top = join_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kRowsWarps; ++w) {
+                top = fmaxf(top, join_m[w][r]);
+            }
+            const float safe = top == -INFINITY ? 0.0f : top;
+            float total = 0.0f;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kRowsWarps; ++w) {
+                const float share = exp2_fast(join_m[w][r] - safe);
+                const float4 v = *reinterpret_cast<const float4*>(join_o + (w * kTile + r) * D + d);
+                total = __fmaf_rn(join_l[w][r], share, total);
+                sum.x = __fmaf_rn(v.x, share, sum.x);
+                sum.y = __fmaf_rn(v.y, share, sum.y);
+                sum.z = __fmaf_rn(v.z, share, sum.z);
+                sum.w = __fmaf_rn(v.w, share, sum.w);
+            }
+            if (begins && ends) {
+                const int global = tile * kTile + r;
+                const int64_t dst = (work.s.row0 + global / call.group) * a.out_stride_row + (head * call.group + global % call.group) * a.out_stride_head + d;
+                const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+                store_float(a.out, dst, a.float_type, sum.x * inv);
+                store_float(a.out, dst + 1, a.float_type, sum.y * inv);
+                store_float(a.out, dst + 2, a.float_type, sum.z * inv);
+                store_float(a.out, dst + 3, a.float_type, sum.w * inv);
+            } else {
+                *reinterpret_cast<float4*>(piece + r * D + d) = sum;
+                if (d == 0) {
+                    piece[kTile * D + r] = top;
+                    piece[kTile * D + kTile + r] = total;
+                }
+            }
+        }
+        if (!(begins && ends)) {
+            kinds[which] = begins ? 1 : ends ? 3 : 2;
+            if (threadIdx.x == 0) {
+                pieces[which] = RowsPiece{kinds[which], seq, head, tile};
+            }
+        }
+        fence_proxy_async_smem();
+        __syncthreads();
+    }
+    if (threadIdx.x < 2 && kinds[threadIdx.x] == 0) {
+        pieces[threadIdx.x].kind = 0;
+    }
+}
+
+// Joins the pieces of the row tiles that were cut, one block for each block of the first kernel in which one begins.
+template <int D, int TILE>
+__global__ void __launch_bounds__(kRowsThreads) attention_i8_join_kernel(const RowsCall call)
+{
+    previous_kernel_done();
+    const RowsPiece mine = call.pieces[2 * blockIdx.x + 1];
+    if (mine.kind != 1) {
+        return;
+    }
+    const nnb200_attention_i8_args& a = call.a;
+    const SequenceRows s = sequence_rows(a.cache, mine.seq);
+    const int rows = min(TILE, s.n * call.group - mine.tile * TILE);
+    int last = blockIdx.x + 1;
+    while (last < static_cast<int>(gridDim.x) - 1 && call.pieces[2 * last].kind == 2) {
+        ++last;
+    }
+    constexpr int64_t kPiece = TILE * (D + 2);
+    const float* first = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kPiece;
+    const float* rest = call.sums + 2 * static_cast<int64_t>(blockIdx.x + 1) * kPiece;   // and every second piece from there
+    const int more = last - static_cast<int>(blockIdx.x);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kRowsThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float top = first[TILE * D + r];
+        for (int p = 0; p < more; ++p) {
+            top = fmaxf(top, rest[p * 2 * kPiece + TILE * D + r]);
+        }
+        const float safe = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = -1; p < more; ++p) {
+            const float* piece = p < 0 ? first : rest + p * 2 * kPiece;
+            const float share = exp2_fast(piece[TILE * D + r] - safe);
+            const float4 v = *reinterpret_cast<const float4*>(piece + r * D + d);
+            total = __fmaf_rn(piece[TILE * D + TILE + r], share, total);
+            sum.x = __fmaf_rn(v.x, share, sum.x);
+            sum.y = __fmaf_rn(v.y, share, sum.y);
+            sum.z = __fmaf_rn(v.z, share, sum.z);
+            sum.w = __fmaf_rn(v.w, share, sum.w);
+        }
+        const int global = mine.tile * TILE + r;
+        const int64_t dst = (s.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d;
+        const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+        store_float(a.out, dst, a.float_type, sum.x * inv);
+        store_float(a.out, dst + 1, a.float_type, sum.y * inv);
+        store_float(a.out, dst + 2, a.float_type, sum.z * inv);
+        store_float(a.out, dst + 3, a.float_type, sum.w * inv);
+    }
+}
+
+template <int D, int NT, bool SPLIT>
+cudaError_t launch_rows(const RowsCall& call, int blocks, cudaStream_t stream)
+{
+    using Shared = RowsShared<D, NT>;
+    const auto kernel = attention_i8_rows_kernel<D, NT, SPLIT>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared::kBytes);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return e;
+    }
+    e = launch_overlapping(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowsThreads), Shared::kBytes, stream, 1, call);
+    note_launch();
+    if (e != cudaSuccess) {
+        return e;
+    }
+    e = launch_overlapping(attention_i8_join_kernel<D, 8 * NT>, dim3(static_cast<unsigned>(blocks)), dim3(kRowsThreads), 0, stream, 1, call);
+    note_launch();
+    return e;
+}
+
+template <int D>
+cudaError_t launch_rows_dim(const RowsCall& call, int columns, int blocks, cudaStream_t stream)
+{
+    if (call.a.float_type == NNB200_FLOAT_F32) {
+        return columns == 1 ? launch_rows<D, 1, true>(call, blocks, stream) : launch_rows<D, 2, true>(call, blocks, stream);
+    }
+    if constexpr (D <= 128) {
+        if (columns == 4) {
+            return launch_rows<D, 4, false>(call, blocks, stream);
+        }
+    }
+    return columns == 1 ? launch_rows<D, 1, false>(call, blocks, stream) : launch_rows<D, 2, false>(call, blocks, stream);
+}
+
+// One translation unit for each head size.
+cudaError_t launch_attention_rows_64(const RowsCall& call, int columns, int blocks, cudaStream_t stream);
+cudaError_t launch_attention_rows_96(const RowsCall& call, int columns, int blocks, cudaStream_t stream);
+cudaError_t launch_attention_rows_128(const RowsCall& call, int columns, int blocks, cudaStream_t stream);
+cudaError_t launch_attention_rows_256(const RowsCall& call, int columns, int blocks, cudaStream_t stream);
+
+}  // namespace nnb200

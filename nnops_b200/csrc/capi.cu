@@ -9,6 +9,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "cache_i8.cuh"
 #include "gemm_i8_umma_batched.cuh"
 #include "i8_realign.cuh"
 #include "internal.cuh"
@@ -1165,6 +1166,181 @@ int nnb200_interleave_shards(const void* gathered, void* out, int64_t m, int64_t
     }
     return launch_interleave_shards(gathered, out, m, row_bytes_per_shard, shards, out_pitch_bytes, *dev,
                                     static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+bool float_type_ok(int32_t t) { return t >= NNB200_FLOAT_F32 && t <= NNB200_FLOAT_BF16; }
+uintptr_t float_bytes(int32_t t) { return t == NNB200_FLOAT_F32 ? 4 : 2; }
+
+// The sizes first: a call without rows has nothing else to be right.
+int check_cache(const nnb200_cache_i8& c, bool* empty)
+{
+    constexpr int64_t kMost = 0x7FFFFFFF;
+    *empty = false;
+    if (c.rows < 0 || c.seqs < 0 || c.heads < 1 || c.dim < 1 || c.pages < 0 || c.table_pages < 0 || c.rows > kMost || c.seqs > kMost / 4 ||
+        c.heads > 65536 || c.pages > kMost) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128) {
+        return NNB200_UNSUPPORTED;
+    }
+    if (c.dim % 16 != 0 || c.dim > 256) {
+        return NNB200_UNSUPPORTED;
+    }
+    if (c.rows == 0) {
+        *empty = true;
+        return NNB200_OK;
+    }
+    if (c.seqs == 0 || (c.cu == nullptr && c.rows % c.seqs != 0) || c.table_pages > kMost / c.page_tokens - 1 || c.table_stride < 0 ||
+        (c.seqs > 1 && c.table_stride < c.table_pages)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    if (c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr || c.lens == nullptr ||
+        (c.page_table == nullptr && c.table_pages > 0)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 4) || !aligned(c.v_scale, 4) || !aligned(c.lens, 4) || !aligned(c.cu, 4) ||
+        !aligned(c.page_table, 4)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    if (c.pages > 1 && (c.page_stride % 16 != 0 || c.page_stride < c.heads * c.page_tokens * c.dim || c.scale_page_stride < c.heads)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    return NNB200_OK;
+}
+
+int check_cache_rows(const nnb200_cache_rows_args* a, bool* empty)
+{
+    if (a == nullptr || !float_type_ok(a->float_type)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    const int status = check_cache(a->cache, empty);
+    if (status != NNB200_OK || *empty) {
+        return status;
+    }
+    const uintptr_t bytes = float_bytes(a->float_type);
+    if (a->k == nullptr || a->v == nullptr || !aligned(a->k, bytes) || !aligned(a->v, bytes)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    return NNB200_OK;
+}
+
+int check_attention(const nnb200_attention_i8_args* a, bool* empty)
+{
+    if (a == nullptr || !float_type_ok(a->float_type) || a->q_heads < 1 || a->window < 0 || a->sinks < 0 || a->force_engine < 0 || a->force_engine > 1) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    const int status = check_cache(a->cache, empty);
+    if (status != NNB200_OK) {
+        return status;
+    }
+    const nnb200_cache_i8& c = a->cache;
+    if (a->q_heads % c.heads != 0 || (a->window > 0 && a->causal == 0)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    if (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) {
+        return NNB200_UNSUPPORTED;
+    }
+    if (c.rows > 0x7FFFFFFF / (a->q_heads / c.heads)) {
+        return NNB200_UNSUPPORTED;
+    }
+    if (*empty) {
+        return NNB200_OK;
+    }
+    const uintptr_t bytes = float_bytes(a->float_type);
+    if (a->q == nullptr || a->out == nullptr || !aligned(a->q, bytes) || !aligned(a->out, bytes)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    return NNB200_OK;
+}
+
+}  // namespace
+
+int nnb200_rms_norm_i8(const nnb200_rms_norm_i8_args* args, void* stream)
+{
+    if (args == nullptr || args->rows < 0 || args->cols < 0 || args->rows > 0x7FFFFFFF || !float_type_ok(args->float_type) ||
+        (args->weight_type != args->float_type && args->weight_type != NNB200_FLOAT_F32)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    if (args->rows == 0 || args->cols == 0) {
+        return NNB200_OK;
+    }
+    const uintptr_t bytes = float_bytes(args->float_type);
+    if (args->x == nullptr || args->weight == nullptr || args->out == nullptr || args->scale == nullptr || !aligned(args->x, bytes) ||
+        !aligned(args->residual, bytes) || !aligned(args->residual_out, bytes) || !aligned(args->weight, float_bytes(args->weight_type)) ||
+        !aligned(args->scale, 4)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    const int64_t last = args->rows > 1 ? args->cols : 0;
+    if (args->out_stride < last || (args->residual_out != nullptr && args->residual_out_stride < last)) {
+        return NNB200_INVALID_ARGUMENT;   // rows of an output that overlap
+    }
+    const DeviceInfo* dev = current_device_info();
+    if (dev == nullptr) {
+        return NNB200_INTERNAL;
+    }
+    return launch_rms_norm_i8(*args, *dev, static_cast<cudaStream_t>(stream));
+}
+
+int nnb200_cache_write_i8(const nnb200_cache_rows_args* args, void* stream)
+{
+    bool empty;
+    const int status = check_cache_rows(args, &empty);
+    if (status != NNB200_OK || empty) {
+        return status;
+    }
+    const DeviceInfo* dev = current_device_info();
+    if (dev == nullptr) {
+        return NNB200_INTERNAL;
+    }
+    return launch_cache_write_i8(*args, *dev, static_cast<cudaStream_t>(stream));
+}
+
+int nnb200_cache_read_i8(const nnb200_cache_rows_args* args, void* stream)
+{
+    bool empty;
+    const int status = check_cache_rows(args, &empty);
+    if (status != NNB200_OK || empty) {
+        return status;
+    }
+    const DeviceInfo* dev = current_device_info();
+    if (dev == nullptr) {
+        return NNB200_INTERNAL;
+    }
+    return launch_cache_read_i8(*args, *dev, static_cast<cudaStream_t>(stream));
+}
+
+size_t nnb200_attention_i8_workspace_bytes(const nnb200_attention_i8_args* args)
+{
+    bool empty;
+    if (check_attention(args, &empty) != NNB200_OK || empty) {
+        return 0;
+    }
+    const DeviceInfo* dev = current_device_info();
+    return dev == nullptr ? 0 : attention_i8_workspace_bytes(*args, *dev);
+}
+
+int nnb200_attention_i8(const nnb200_attention_i8_args* args, void* stream)
+{
+    bool empty;
+    const int status = check_attention(args, &empty);
+    if (status != NNB200_OK || empty) {
+        return status;
+    }
+    if (args->workspace == nullptr || !aligned(args->workspace, 16)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    const DeviceInfo* dev = current_device_info();
+    if (dev == nullptr) {
+        return NNB200_INTERNAL;
+    }
+    if (args->workspace_bytes < attention_i8_workspace_bytes(*args, *dev)) {
+        return NNB200_INVALID_ARGUMENT;
+    }
+    return launch_attention_i8(*args, *dev, static_cast<cudaStream_t>(stream));
 }
 
 int nnb200_rank_barrier(int32_t* const* flags_by_rank, int32_t world, int32_t rank, int64_t limit_cycles, void* stream)

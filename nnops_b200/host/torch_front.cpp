@@ -37,6 +37,11 @@ struct Library {
     Run dequantize = nullptr;
     Size conv_bytes = nullptr;
     Run conv = nullptr;
+    Run rms_norm = nullptr;
+    Run cache_write = nullptr;
+    Run cache_read = nullptr;
+    Size attention_bytes = nullptr;
+    Run attention = nullptr;
 } g_lib;
 
 PyObject* g_error = nullptr;   // capi.check: raises for a status that is not ok
@@ -683,11 +688,231 @@ PyObject* conv2d_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     });
 }
 
+int float_type_of(at::ScalarType t)
+{
+    return t == at::kFloat ? NNB200_FLOAT_F32 : t == at::kHalf ? NNB200_FLOAT_F16 : t == at::kBFloat16 ? NNB200_FLOAT_BF16 : (elsewhere(), 0);
+}
+
+// A matrix [m, n] of that type with dense rows.
+const at::Tensor& rows_of(PyObject* o, at::ScalarType type, int64_t m, int64_t n, const c10::Device& dev)
+{
+    const at::Tensor& t = plain(o, dev);
+    if (t.scalar_type() != type || t.dim() != 2 || t.size(0) != m || t.size(1) != n || (n > 1 && t.stride(1) != 1)) {
+        elsewhere();
+    }
+    return t;
+}
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> tensors)
+{
+    PyObject* made = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+    if (made == nullptr) {
+        throw python_error();
+    }
+    Py_ssize_t i = 0;
+    for (const at::Tensor& t : tensors) {
+        PyTuple_SET_ITEM(made, i++, THPVariable_Wrap(t));
+    }
+    return made;
+}
+
+// rms_norm_i8(x, weight, residual, eps, out, scale, residual_out)
+PyObject* rms_norm_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject* {
+        expect(nargs, 7);
+        const c10::Device dev = current_device(args[0]);
+        const at::Tensor& x = plain(args[0], dev);
+        if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1)) {
+            elsewhere();
+        }
+        const at::ScalarType type = x.scalar_type();
+        const int64_t m = x.size(0), n = x.size(1);
+        nnb200_rms_norm_i8_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.float_type = float_type_of(type);
+        const at::Tensor& weight = plain(args[1], dev);
+        if ((weight.scalar_type() != type && weight.scalar_type() != at::kFloat) || weight.dim() != 1 || weight.size(0) != n || !weight.is_contiguous()) {
+            elsewhere();
+        }
+        a.weight_type = float_type_of(weight.scalar_type());
+        a.eps = static_cast<float>(number(args[3]));
+        at::Tensor out, scale, residual_out;
+        const bool more = args[2] != Py_None;
+        if (more) {
+            const at::Tensor& residual = rows_of(args[2], type, m, n, dev);
+            a.residual = residual.data_ptr();
+            a.residual_stride = residual.stride(0);
+            residual_out = args[6] != Py_None ? rows_of(args[6], type, m, n, dev) : empty({m, n}, type, dev);
+            a.residual_out = residual_out.data_ptr();
+            a.residual_out_stride = residual_out.stride(0);
+        } else if (args[6] != Py_None) {
+            elsewhere();
+        }
+        out = args[4] != Py_None ? rows_of(args[4], at::kChar, m, n, dev) : empty({m, n}, at::kChar, dev);
+        if (args[5] != Py_None) {
+            scale = plain(args[5], dev);
+            if (scale.scalar_type() != at::kFloat || scale.dim() != 1 || scale.size(0) != m || !scale.is_contiguous()) {
+                elsewhere();
+            }
+        } else {
+            scale = empty({m}, at::kFloat, dev);
+        }
+        a.x = x.data_ptr();
+        a.weight = weight.data_ptr();
+        a.out = out.data_ptr();
+        a.scale = static_cast<float*>(scale.data_ptr());
+        a.rows = m;
+        a.cols = n;
+        a.x_stride = x.stride(0);
+        a.out_stride = out.stride(0);
+        enqueue(g_lib.rms_norm, &a, dev, "nnb200_rms_norm_i8");
+        return more ? tuple_of({out, scale, residual_out}) : tuple_of({out, scale});
+    });
+}
+
+const int32_t* words(PyObject* o, int64_t dim, const c10::Device& dev)
+{
+    const at::Tensor& t = plain(o, dev);
+    if (t.scalar_type() != at::kInt || t.dim() != dim || (t.size(-1) > 1 && t.stride(-1) != 1)) {
+        elsewhere();
+    }
+    return static_cast<const int32_t*>(t.data_ptr());
+}
+
+// `handle`: CacheI8's device index, addresses, distances and sizes.
+void cache_of(nnb200_cache_i8& c, PyObject* handle, PyObject* table, PyObject* lens, PyObject* cu, int64_t rows, const c10::Device& dev)
+{
+    if (!PyTuple_CheckExact(handle) || PyTuple_GET_SIZE(handle) != 11 || whole(PyTuple_GET_ITEM(handle, 0)) != dev.index()) {
+        elsewhere();
+    }
+    const auto field = [&](int i) { return whole(PyTuple_GET_ITEM(handle, i)); };
+    c.k = reinterpret_cast<void*>(field(1));
+    c.v = reinterpret_cast<void*>(field(2));
+    c.k_scale = reinterpret_cast<float*>(field(3));
+    c.v_scale = reinterpret_cast<float*>(field(4));
+    c.pages = field(5);
+    c.page_stride = field(6);
+    c.scale_page_stride = field(7);
+    c.heads = field(8);
+    c.page_tokens = field(9);
+    c.dim = field(10);
+    c.page_table = words(table, 2, dev);
+    c.lens = words(lens, 1, dev);
+    const at::Tensor& t = THPVariable_Unpack(table);
+    c.table_stride = t.stride(0);
+    c.table_pages = t.size(1);
+    c.seqs = THPVariable_Unpack(lens).size(0);
+    c.rows = rows;
+    if (t.size(0) != c.seqs) {
+        elsewhere();
+    }
+    if (cu != Py_None) {
+        c.cu = words(cu, 1, dev);
+        if (THPVariable_Unpack(cu).size(0) != c.seqs + 1) {
+            elsewhere();
+        }
+    } else if (c.seqs == 0 || rows % c.seqs != 0) {
+        elsewhere();
+    }
+}
+
+// [rows, heads, dim], dense along dim.
+bool head_rows(const at::Tensor& t, int64_t rows, int64_t heads, int64_t dim)
+{
+    return t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == dim && t.stride(2) == 1;
+}
+
+// cache_rows_i8(handle, k, v, page_table, lens, cu, write)
+PyObject* cache_rows_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject* {
+        expect(nargs, 7);
+        const c10::Device dev = current_device(args[1]);
+        const at::Tensor& k = plain(args[1], dev);
+        const at::Tensor& v = plain(args[2], dev);
+        if (k.dim() != 3) {
+            elsewhere();
+        }
+        nnb200_cache_rows_args a;
+        std::memset(&a, 0, sizeof(a));
+        cache_of(a.cache, args[0], args[3], args[4], args[5], k.size(0), dev);
+        if (!head_rows(k, a.cache.rows, a.cache.heads, a.cache.dim) || !head_rows(v, a.cache.rows, a.cache.heads, a.cache.dim) ||
+            v.scalar_type() != k.scalar_type()) {
+            elsewhere();
+        }
+        a.float_type = float_type_of(k.scalar_type());
+        a.k = k.data_ptr();
+        a.v = v.data_ptr();
+        a.k_stride_row = k.stride(0);
+        a.k_stride_head = k.stride(1);
+        a.v_stride_row = v.stride(0);
+        a.v_stride_head = v.stride(1);
+        const bool write = flag(args[6], true);
+        enqueue(write ? g_lib.cache_write : g_lib.cache_read, &a, dev, write ? "nnb200_cache_write_i8" : "nnb200_cache_read_i8");
+        Py_RETURN_TRUE;
+    });
+}
+
+// attention_i8_cache(q, handle, page_table, lens, cu, causal, window, sinks, scale, out, engine)
+PyObject* attention_i8_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject* {
+        expect(nargs, 11);
+        const c10::Device dev = current_device(args[0]);
+        const at::Tensor& q = plain(args[0], dev);
+        if (q.dim() != 3) {
+            elsewhere();
+        }
+        nnb200_attention_i8_args a;
+        std::memset(&a, 0, sizeof(a));
+        cache_of(a.cache, args[1], args[2], args[3], args[4], q.size(0), dev);
+        const int64_t rows = a.cache.rows, heads = q.size(1), dim = a.cache.dim;
+        if (!head_rows(q, rows, heads, dim) || heads < 1 || a.cache.heads < 1 || heads % a.cache.heads != 0) {
+            elsewhere();
+        }
+        a.float_type = float_type_of(q.scalar_type());
+        a.causal = flag(args[5], true) ? 1 : 0;
+        a.window = whole(args[6]);
+        a.sinks = whole(args[7]);
+        if (a.window < 0 || a.sinks < 0 || (a.window > 0 && a.causal == 0)) {
+            elsewhere();
+        }
+        a.scale = args[8] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : static_cast<float>(number(args[8]));
+        static const char* const automatic[] = {"auto"};
+        one_of(args[10], automatic, 0);
+        at::Tensor out;
+        if (args[9] != Py_None) {
+            out = plain(args[9], dev);
+            if (!head_rows(out, rows, heads, dim) || out.scalar_type() != q.scalar_type()) {
+                elsewhere();
+            }
+        } else {
+            out = empty({rows, heads, dim}, q.scalar_type(), dev);
+        }
+        a.q = q.data_ptr();
+        a.out = out.data_ptr();
+        a.q_stride_row = q.stride(0);
+        a.q_stride_head = q.stride(1);
+        a.out_stride_row = out.stride(0);
+        a.out_stride_head = out.stride(1);
+        a.q_heads = heads;
+        at::Tensor workspace;   // stream-ordered: may go when this returns
+        if (const size_t need = g_lib.attention_bytes(&a); need != 0) {
+            workspace = scratch(need, dev);
+            a.workspace = workspace.data_ptr();
+            a.workspace_bytes = need;
+        }
+        enqueue(g_lib.attention, &a, dev, "nnb200_attention_i8");
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 // bind(addresses in the order of Library, check)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     return guarded([&]() -> PyObject* {
-        expect(nargs, 9);
+        expect(nargs, 14);
         const auto address = [&](int i) { return reinterpret_cast<void*>(whole(args[i])); };
         g_lib.gemm_bytes = reinterpret_cast<Size>(address(0));
         g_lib.gemm = reinterpret_cast<Run>(address(1));
@@ -697,9 +922,14 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         g_lib.dequantize = reinterpret_cast<Run>(address(5));
         g_lib.conv_bytes = reinterpret_cast<Size>(address(6));
         g_lib.conv = reinterpret_cast<Run>(address(7));
-        Py_INCREF(args[8]);
+        g_lib.rms_norm = reinterpret_cast<Run>(address(8));
+        g_lib.cache_write = reinterpret_cast<Run>(address(9));
+        g_lib.cache_read = reinterpret_cast<Run>(address(10));
+        g_lib.attention_bytes = reinterpret_cast<Size>(address(11));
+        g_lib.attention = reinterpret_cast<Run>(address(12));
+        Py_INCREF(args[13]);
         Py_XDECREF(g_error);
-        g_error = args[8];
+        g_error = args[13];
         Py_RETURN_TRUE;
     });
 }
@@ -712,6 +942,9 @@ PyMethodDef g_methods[] = {
     {"dequantize_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequantize_linear)), METH_FASTCALL, nullptr},
     {"linear_fp_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_fp_act)), METH_FASTCALL, nullptr},
     {"conv2d_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(conv2d_i8)), METH_FASTCALL, nullptr},
+    {"rms_norm_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm_i8)), METH_FASTCALL, nullptr},
+    {"cache_rows_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_rows_i8)), METH_FASTCALL, nullptr},
+    {"attention_i8_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention_i8_cache)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

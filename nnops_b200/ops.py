@@ -38,7 +38,9 @@ def _front():
             return _native
         bound = front.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
             "nnb200_gemm_i8_workspace_bytes", "nnb200_gemm_i8", "nnb200_q4_1_workspace_bytes", "nnb200_linear_q4_1",
-            "nnb200_quantize_linear", "nnb200_dequantize_linear", "nnb200_conv2d_i8_workspace_bytes", "nnb200_conv2d_i8")), capi.check)
+            "nnb200_quantize_linear", "nnb200_dequantize_linear", "nnb200_conv2d_i8_workspace_bytes", "nnb200_conv2d_i8",
+            "nnb200_rms_norm_i8", "nnb200_cache_write_i8", "nnb200_cache_read_i8", "nnb200_attention_i8_workspace_bytes",
+            "nnb200_attention_i8")), capi.check)
         if bound is not True:
             raise RuntimeError("torch_front is of another version than ops.py: rebuild it with `python -m nnops_b200.build --force`")
         _native = front
@@ -514,3 +516,184 @@ def _conv2d_i8(x: torch.Tensor, w, *, stride=(1, 1), dilation=(1, 1), padding=(0
 
 
 conv2d_i8.__signature__ = inspect.signature(_conv2d_i8)
+
+
+_FLOAT_TYPES = {torch.float32: capi.FLOAT_F32, torch.float16: capi.FLOAT_F16, torch.bfloat16: capi.FLOAT_BF16}
+
+
+def _float_type(t: torch.Tensor, name: str) -> int:
+    kind = _FLOAT_TYPES.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{name} must be f32, f16 or bf16")
+    return kind
+
+
+def _like(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device: torch.device) -> torch.Tensor:
+    if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {device}")
+    return t
+
+
+def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                out: torch.Tensor | None = None, scale: torch.Tensor | None = None, residual_out: torch.Tensor | None = None):
+    """RMS norm of the rows of ``x`` [M, N] (+ ``residual``) into 8 bits on the current CUDA stream, f32 / f16 / bf16:
+    (codes s8 [M, N], scale f32 [M]), the operand and ``scale_a`` of gemm_i8; with a residual also x + residual, the
+    next one.  ``weight`` [N] is of x's type or f32.  ``residual_out`` may be ``x`` or ``residual`` itself."""
+    made = (_native or _front()).rms_norm_i8(x, weight, residual, eps, out, scale, residual_out)
+    if made is not None:
+        return made
+    if not x.is_cuda:
+        raise RuntimeError("nnops_b200.rms_norm_i8 needs CUDA tensors; there is no CPU path")
+    kind = _float_type(x, "x")
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x must be a matrix whose rows are dense")
+    m, n = x.shape
+    dev = x.device
+    if weight.dtype not in (x.dtype, torch.float32) or tuple(weight.shape) != (n,) or weight.device != dev or not weight.is_contiguous():
+        raise ValueError("weight must be a dense vector of x's columns, of x's type or f32")
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    if residual is not None:
+        _like(residual, "residual", x.dtype, (m, n), dev)
+        residual_out = torch.empty((m, n), dtype=x.dtype, device=dev) if residual_out is None else _like(residual_out, "residual_out", x.dtype, (m, n), dev)
+    out = torch.empty((m, n), dtype=torch.int8, device=dev) if out is None else _like(out, "out", torch.int8, (m, n), dev)
+    scale = torch.empty((m,), dtype=torch.float32, device=dev) if scale is None else _like(scale, "scale", torch.float32, (m,), dev)
+    for t in (residual, residual_out, out):
+        if t is not None and n > 1 and t.stride(1) != 1:
+            raise ValueError("rows must be dense")
+    if m > 1 and scale.stride(0) != 1:
+        raise ValueError("scale must be dense")
+    args = capi.block(capi.RmsNormI8Args, x.data_ptr(), residual.data_ptr() if residual is not None else 0, weight.data_ptr(), out.data_ptr(),
+                      scale.data_ptr(), residual_out.data_ptr() if residual_out is not None else 0, m, n, x.stride(0),
+                      residual.stride(0) if residual is not None else 0, out.stride(0), residual_out.stride(0) if residual_out is not None else 0,
+                      float(eps), kind, _FLOAT_TYPES[weight.dtype])
+    _call(capi.lib().nnb200_rms_norm_i8, args, dev, "nnb200_rms_norm_i8")
+    return (out, scale) if residual is None else (out, scale, residual_out)
+
+
+class CacheI8:
+    """A key/value cache in 8 bits: codes s8 [pages, heads, page tokens, dim], dense within a page, and one f32 scale for each
+    page and head [pages, heads] (see nnb200_cache_i8 in nnb200.h).  Which pages a sequence has is its caller's
+    business: every call takes ``page_table`` int32 [seqs, n], ``lens`` int32 [seqs], the sequences' tokens with the call's
+    new ones, and, unless each sequence has the same number of rows, ``cu`` int32 [seqs + 1]."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if k.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise ValueError("codes must be int8 [pages, heads, page tokens, dim], scales f32 [pages, heads]")
+        pages, heads, tokens, dim = k.shape
+        if v.shape != k.shape or tuple(k_scale.shape) != (pages, heads) or v_scale.shape != k_scale.shape:
+            raise ValueError("keys, values and scales must agree in pages, heads, page tokens and dim")
+        if k.stride() != v.stride() or k_scale.stride() != v_scale.stride() or k.stride()[1:] != (tokens * dim, dim, 1) or (heads > 1 and k_scale.stride(1) != 1):
+            raise ValueError("pages and their scales must be dense, those of values at the distances of those of keys")
+        if len({k.device, v.device, k_scale.device, v_scale.device}) != 1:
+            raise ValueError("keys, values and scales must be on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.page_tokens, self.dim, self.device = pages, heads, tokens, dim, k.device
+        # What the calls hand on: addresses, pages, distances and sizes.
+        self._fields = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, k.stride(0), k_scale.stride(0), heads, tokens, dim)
+        self._handle = (-1 if k.device.index is None else k.device.index, *self._fields)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, page_tokens: int, dim: int, device) -> "CacheI8":
+        """A cache of zeros."""
+        k, v = (torch.zeros((pages, heads, page_tokens, dim), dtype=torch.int8, device=device) for _ in range(2))
+        return cls(k, v, *(torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _sequences(cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor | None, rows: int):
+    """The leading fields of a call over ``cache``."""
+    dev = cache.device
+    if dev.type != "cuda":
+        raise RuntimeError("the calls over an 8-bit cache need CUDA tensors; there is no CPU path")
+    for name, t, d in (("page_table", page_table, 2), ("lens", lens, 1), ("cu", cu, 1)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != d or t.device != dev or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{name} must be an int32 {'matrix' if d == 2 else 'vector'} on the cache's device, dense along its last axis")
+    seqs = lens.shape[0]
+    if page_table.shape[0] != seqs or (cu is not None and cu.shape[0] != seqs + 1):
+        raise ValueError("page_table, lens and cu must agree in the number of sequences")
+    if cu is None and rows != (rows // seqs * seqs if seqs else 0):
+        raise ValueError("without cu every sequence has the same number of rows")
+    return (*cache._fields, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), cu.data_ptr() if cu is not None else 0,
+            seqs, rows)
+
+
+def _head_rows(t: torch.Tensor, name: str, rows: int, heads: int, cache: CacheI8) -> None:
+    if tuple(t.shape) != (rows, heads, cache.dim) or t.stride(2) != 1 or t.device != cache.device:
+        raise ValueError(f"{name} must be [{rows}, {heads}, {cache.dim}], dense along its last axis, on the cache's device")
+
+
+def cache_write_i8(cache: CacheI8, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, *,
+                   cu: torch.Tensor | None = None) -> CacheI8:
+    """Quantise the rows ``k``, ``v`` [rows, heads, dim] (f32 / f16 / bf16) into ``cache`` on the current CUDA stream, as the last tokens of
+    their sequences."""
+    if (_native or _front()).cache_rows_i8(cache._handle, k, v, page_table, lens, cu, True) is not None:
+        return cache
+    kind = _float_type(k, "k")
+    if v.dtype is not k.dtype:
+        raise ValueError("k and v must be of one type")
+    rows = k.shape[0]
+    for name, t in (("k", k), ("v", v)):
+        _head_rows(t, name, rows, cache.heads, cache)
+    args = capi.block(capi.CacheRowsArgs, *_sequences(cache, page_table, lens, cu, rows), k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], kind)
+    _call(capi.lib().nnb200_cache_write_i8, args, cache.device, "nnb200_cache_write_i8")
+    return cache
+
+
+def cache_read_i8(cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, *, rows: int | None = None, cu: torch.Tensor | None = None,
+                  out_dtype: torch.dtype = torch.float16, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """The values of the sequences' last tokens as (k, v) [rows, heads, dim] on the current CUDA stream.  ``rows``: of the output, all
+    sequences together."""
+    if out is None:
+        if rows is None:
+            raise ValueError("rows or out is needed")
+        out = tuple(torch.empty((rows, cache.heads, cache.dim), dtype=out_dtype, device=cache.device) for _ in range(2))
+    k, v = out
+    if (_native or _front()).cache_rows_i8(cache._handle, k, v, page_table, lens, cu, False) is not None:
+        return k, v
+    kind = _float_type(k, "out")
+    if v.dtype is not k.dtype or (rows is not None and rows != k.shape[0]):
+        raise ValueError("the outputs must be of one type, and have the rows asked for")
+    rows = k.shape[0]
+    for t in out:
+        _head_rows(t, "out", rows, cache.heads, cache)
+    args = capi.block(capi.CacheRowsArgs, *_sequences(cache, page_table, lens, cu, rows), k.data_ptr(), v.data_ptr(), *k.stride()[:2], *v.stride()[:2], kind)
+    _call(capi.lib().nnb200_cache_read_i8, args, cache.device, "nnb200_cache_read_i8")
+    return k, v
+
+
+ATTENTION_ENGINES = {"auto": 0, "rows": 1}
+
+
+def attention_i8_cache(q: torch.Tensor, cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, *, cu: torch.Tensor | None = None,
+                       causal: bool = True, window: int = 0, sinks: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
+                       engine: str = "auto") -> torch.Tensor:
+    """Attention of the rows ``q`` [rows, query heads, dim] (f32 / f16 / bf16), the last tokens of their sequences, over ``cache`` on the
+    current CUDA stream.  Each group of query heads shares a head of the cache.  ``window``: a row sees that many tokens up to
+    its own and the first ``sinks``; 0: all up to its own.  ``causal`` false: all of its sequence.  ``scale``: 1 / sqrt(dim)."""
+    made = (_native or _front()).attention_i8_cache(q, cache._handle, page_table, lens, cu, causal, window, sinks, scale, out, engine)
+    if made is not None:
+        return made
+    kind = _float_type(q, "q")
+    if q.dim() != 3 or q.shape[1] % cache.heads or not q.shape[1]:
+        raise ValueError("q must be [rows, query heads, dim] with a multiple of the cache's heads")
+    rows, heads = q.shape[:2]
+    _head_rows(q, "q", rows, heads, cache)
+    if window < 0 or sinks < 0 or (window and not causal):
+        raise ValueError("window and sinks are counts, a window is a causal one's")
+    if out is None:
+        out = torch.empty((rows, heads, cache.dim), dtype=q.dtype, device=q.device)
+    else:
+        _head_rows(out, "out", rows, heads, cache)
+        if out.dtype is not q.dtype:
+            raise ValueError("out must be of q's type")
+    args = capi.block(capi.AttentionI8Args, *_sequences(cache, page_table, lens, cu, rows), q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2],
+                      heads, int(window), int(sinks), 1.0 / math.sqrt(cache.dim) if scale is None else float(scale), int(bool(causal)), kind,
+                      ATTENTION_ENGINES[engine])
+    lib = capi.lib()
+    with torch.cuda.device(cache.device):
+        need = lib.nnb200_attention_i8_workspace_bytes(C.byref(args))
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=cache.device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    _call(lib.nnb200_attention_i8, args, cache.device, "nnb200_attention_i8")
+    return out

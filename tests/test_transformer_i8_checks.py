@@ -1,0 +1,153 @@
+"""What the norm, the cache's calls and the attention over it refuse, at the C entry and in the Python front end; no GPU, nothing
+is ever run."""
+import ctypes as C
+
+import pytest
+import torch
+
+from nnops_b200 import capi, ops
+
+BASE = 0x7000_0000_1000    # never dereferenced: validation comes first
+
+
+def _norm(**over):
+    a = capi.RmsNormI8Args(x=BASE, weight=BASE + 0x10000, out=BASE + 0x20000, scale=BASE + 0x30000, rows=2, cols=64, x_stride=64, out_stride=64,
+                           eps=1e-6, float_type=1, weight_type=1)
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+def _cache(cls, **over):
+    a = cls(k=BASE, v=BASE + 0x10000, k_scale=BASE + 0x20000, v_scale=BASE + 0x21000, pages=4, page_stride=2 * 16 * 64, scale_page_stride=2, heads=2,
+            page_tokens=16, dim=64, page_table=BASE + 0x30000, table_stride=4, table_pages=4, lens=BASE + 0x31000, cu=BASE + 0x32000, seqs=2, rows=6)
+    if cls is capi.CacheRowsArgs:
+        a.rows_k, a.rows_v = BASE + 0x40000, BASE + 0x50000
+        a.k_stride_row = a.v_stride_row = 128
+        a.k_stride_head = a.v_stride_head = 64
+    else:
+        a.q, a.out, a.q_heads, a.causal, a.scale = BASE + 0x40000, BASE + 0x50000, 4, 1, 0.125
+        a.q_stride_row = a.out_stride_row = 256
+        a.q_stride_head = a.out_stride_head = 64
+    a.float_type = 1
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_norm_arguments(nnb200_lib):
+    before = nnb200_lib.nnb200_launch_count()
+    for over in (dict(rows=-1), dict(cols=-1), dict(rows=1 << 31), dict(float_type=3), dict(float_type=-1), dict(weight_type=2), dict(x=None),
+                 dict(weight=None), dict(out=None), dict(scale=None), dict(x=BASE + 1), dict(weight=BASE + 1), dict(scale=BASE + 2),
+                 dict(residual=BASE + 1), dict(residual_out=BASE + 1), dict(out_stride=63), dict(residual_out=BASE, residual_out_stride=1)):
+        assert nnb200_lib.nnb200_rms_norm_i8(C.byref(_norm(**over)), None) == capi.INVALID_ARGUMENT, over
+    assert nnb200_lib.nnb200_rms_norm_i8(None, None) == capi.INVALID_ARGUMENT
+    assert nnb200_lib.nnb200_rms_norm_i8(C.byref(_norm(rows=0, x=None)), None) == capi.OK
+    assert nnb200_lib.nnb200_launch_count() == before
+
+
+WRONG_CACHE = [dict(rows=-1), dict(rows=1 << 31), dict(seqs=-1), dict(seqs=0), dict(heads=0), dict(dim=0), dict(pages=-1), dict(pages=1 << 31),
+               dict(table_pages=-1), dict(table_pages=1 << 30), dict(table_stride=3), dict(table_stride=-4), dict(k=None), dict(v=None),
+               dict(k_scale=None), dict(v_scale=None), dict(lens=None), dict(page_table=None), dict(k=BASE + 8), dict(v=BASE + 4),
+               dict(k_scale=BASE + 2), dict(v_scale=BASE + 1), dict(lens=BASE + 2), dict(cu=BASE + 1), dict(page_table=BASE + 3), dict(page_stride=2047),
+               dict(page_stride=2032), dict(page_stride=2056), dict(scale_page_stride=1), dict(cu=None, rows=7), dict(float_type=3)]
+UNKNOWN_CACHE = [dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=256), dict(dim=24), dict(dim=272)]
+
+
+@pytest.mark.parametrize("entry", ["nnb200_cache_write_i8", "nnb200_cache_read_i8", "nnb200_attention_i8"])
+def test_cache_arguments(nnb200_lib, entry):
+    cls = capi.AttentionI8Args if "attention" in entry else capi.CacheRowsArgs
+    call = getattr(nnb200_lib, entry)
+    before = nnb200_lib.nnb200_launch_count()
+    for over in WRONG_CACHE:
+        assert call(C.byref(_cache(cls, **over)), None) == capi.INVALID_ARGUMENT, over
+    for over in UNKNOWN_CACHE:
+        assert call(C.byref(_cache(cls, **over)), None) == capi.UNSUPPORTED, over
+    pointers = ("q", "out") if cls is capi.AttentionI8Args else ("rows_k", "rows_v")
+    for name in pointers:
+        for value in (None, BASE + 1):
+            assert call(C.byref(_cache(cls, **{name: value})), None) == capi.INVALID_ARGUMENT, name
+    assert call(None, None) == capi.INVALID_ARGUMENT
+    assert call(C.byref(_cache(cls, rows=0, k=None, lens=None)), None) == capi.OK    # nothing to do
+    assert nnb200_lib.nnb200_launch_count() == before
+
+
+def test_attention_arguments(nnb200_lib):
+    call = nnb200_lib.nnb200_attention_i8
+    for over in (dict(q_heads=0), dict(q_heads=3), dict(window=-1), dict(sinks=-1), dict(window=4, causal=0), dict(force_engine=9), dict(workspace=None),
+                 dict(workspace=BASE + 8, workspace_bytes=1 << 40)):
+        assert call(C.byref(_cache(capi.AttentionI8Args, **over)), None) == capi.INVALID_ARGUMENT, over
+    for dim in (16, 80, 112, 160):
+        assert call(C.byref(_cache(capi.AttentionI8Args, dim=dim, page_stride=1 << 20)), None) == capi.UNSUPPORTED, dim
+    assert call(C.byref(_cache(capi.AttentionI8Args, rows=0x7FFFFFFE, q_heads=64)), None) == capi.UNSUPPORTED
+    assert nnb200_lib.nnb200_attention_i8_workspace_bytes(C.byref(_cache(capi.AttentionI8Args, rows=0))) == 0
+    assert nnb200_lib.nnb200_attention_i8_workspace_bytes(None) == 0
+
+
+def test_blocks_agree_with_the_header():
+    assert C.sizeof(capi.CacheRowsArgs) == 17 * 8 + 6 * 8 + 8
+    assert C.sizeof(capi.AttentionI8Args) == 17 * 8 + 9 * 8 + 16 + 16
+    assert C.sizeof(capi.RmsNormI8Args) == 12 * 8 + 16
+
+
+def test_caches_that_are_none():
+    codes, scale = torch.zeros((4, 2, 16, 64), dtype=torch.int8), torch.zeros((4, 2))
+    for bad in [(codes.short(), codes, scale, scale), (codes, codes[:3], scale, scale), (codes, codes, scale[:3], scale[:3]), (codes, codes, scale.half(), scale),
+                (codes.transpose(1, 2), codes.transpose(1, 2), torch.zeros((4, 16)), torch.zeros((4, 16))), (codes[0], codes[0], scale, scale),
+                (codes[..., ::2], codes[..., ::2], scale, scale), (codes, codes, torch.zeros((2, 4)).t(), torch.zeros((2, 4)).t())]:
+        with pytest.raises(ValueError):
+            ops.CacheI8(*bad)
+    ops.CacheI8(codes, codes, scale, scale)
+
+
+def test_the_front_end_has_no_cpu_path(nnb200_lib):
+    cache = ops.CacheI8.empty(4, 2, 16, 64, "cpu")
+    x, ints = torch.zeros((2, 2, 64)), torch.zeros((2, 2), dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.rms_norm_i8(torch.zeros((2, 64)), torch.zeros(64))
+    for call in (lambda: ops.cache_write_i8(cache, x, x, ints, ints[0]), lambda: ops.cache_read_i8(cache, ints, ints[0], rows=2),
+                 lambda: ops.attention_i8_cache(x, cache, ints, ints[0])):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_what_the_front_end_refuses(nnb200_lib, monkeypatch):
+    """The checks come before anything is looked at on a device: a cache that says it is on one."""
+    cache = ops.CacheI8.empty(4, 2, 16, 64, "cpu")
+    monkeypatch.setattr(ops, "_native", ops._NoFront())
+    x, table, lens = torch.zeros((4, 2, 64)), torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    q = torch.zeros((4, 4, 64))
+    with pytest.raises(ValueError):
+        ops.cache_write_i8(cache, x.int(), x.int(), table, lens)
+    with pytest.raises(ValueError):
+        ops.cache_write_i8(cache, x, x.half(), table, lens)
+    with pytest.raises(ValueError):
+        ops.cache_write_i8(cache, x, x[:3], table, lens)
+    with pytest.raises(ValueError):
+        ops.cache_write_i8(cache, x[..., :32], x[..., :32], table, lens)
+    with pytest.raises(ValueError):
+        ops.cache_read_i8(cache, table, lens)
+    with pytest.raises(ValueError):
+        ops.cache_read_i8(cache, table, lens, rows=4, out_dtype=torch.int8)
+    for kw in (dict(window=-1), dict(sinks=-1), dict(window=3, causal=False), dict(out=q.half()), dict(out=q[:3])):
+        with pytest.raises(ValueError):
+            ops.attention_i8_cache(q, cache, table, lens, **kw)
+    with pytest.raises(ValueError):
+        ops.attention_i8_cache(q[:, :3], cache, table, lens)
+    with pytest.raises(ValueError):
+        ops.attention_i8_cache(q.double(), cache, table, lens)
+
+    class There:
+        type = "cuda"
+
+        def __eq__(self, other):
+            return other == torch.device("cpu")
+
+        __hash__ = None
+
+    cache.device = There()
+    for bad in [(table.long(), lens, None), (table, lens.long(), None), (table[:1], lens, None), (table, lens, lens), (table, lens[None], None),
+                (table.t().contiguous().t(), lens, None), (torch.zeros((3, 3), dtype=torch.int32), torch.zeros(3, dtype=torch.int32), None)]:
+        with pytest.raises(ValueError):
+            ops._sequences(cache, *bad, 4)
+    assert ops._sequences(cache, table, lens, None, 4)[-2:] == (2, 4)
