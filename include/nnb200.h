@@ -571,7 +571,7 @@ typedef struct nnb200_attention_i8_args {
     float scale;
     int32_t causal;
     int32_t float_type;       /* of q and out */
-    int32_t force_engine;     /* 0 auto, 1 rows on warp MMAs */
+    int32_t force_engine;     /* 0 auto, 1 few rows on warp MMAs, 2 tiles of 128 rows on tcgen05 (not f32) */
     void* workspace;
     size_t workspace_bytes;
 } nnb200_attention_i8_args;

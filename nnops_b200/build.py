@@ -27,7 +27,7 @@ FRONT_SRC = PKG / "host" / "torch_front.cpp"
 NVCC = os.environ.get("NNB200_NVCC", "/usr/local/cuda/bin/nvcc")
 CXX = os.environ.get("NNB200_CXX", "g++")
 
-SOURCES = ["capi.cu", "gemm_i8_umma.cu", "gemm_i8_umma_batched.cu", "i8_realign.cu", "gemm_i8_simt.cu", "gemm_i8_decode.cu", "gemm_i8_skinny.cu", "q4_1_gemv.cu", "q4_1_gemv_mma.cu", "q4_1_gemv_dsq.cu", "q4_1_gemm_umma.cu", "q4_1_rows_umma.cu", "gemm_f16_umma.cu", "shard_gather.cu", "quant_linear.cu", "prepack.cu", "static_scratch.cu", "mma_peak.cu", "conv2d_i8.cu", "rms_norm_i8.cu", "cache_i8.cu", "attention_i8.cu", "attention_i8_rows_d64.cu", "attention_i8_rows_d96.cu", "attention_i8_rows_d128.cu", "attention_i8_rows_d256.cu"]
+SOURCES = ["capi.cu", "gemm_i8_umma.cu", "gemm_i8_umma_batched.cu", "i8_realign.cu", "gemm_i8_simt.cu", "gemm_i8_decode.cu", "gemm_i8_skinny.cu", "q4_1_gemv.cu", "q4_1_gemv_mma.cu", "q4_1_gemv_dsq.cu", "q4_1_gemm_umma.cu", "q4_1_rows_umma.cu", "gemm_f16_umma.cu", "shard_gather.cu", "quant_linear.cu", "prepack.cu", "static_scratch.cu", "mma_peak.cu", "conv2d_i8.cu", "rms_norm_i8.cu", "cache_i8.cu", "attention_i8.cu", "attention_i8_rows_d64.cu", "attention_i8_rows_d96.cu", "attention_i8_rows_d128.cu", "attention_i8_rows_d256.cu", "attention_i8_tile_d64.cu", "attention_i8_tile_d96.cu", "attention_i8_tile_d128.cu", "attention_i8_tile_d256.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

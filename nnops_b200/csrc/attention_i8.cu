@@ -1,17 +1,35 @@
 // Attention over a key/value cache in 8 bits: which kernel, and how it is launched.
 
-#include "attention_i8_rows.cuh"
+#include "attention_i8_tile.cuh"
 
 namespace nnb200 {
 
 namespace {
 
-// Tiles of 8, 16 or 32 query rows: as many as a sequence has, on average where lengths are the device's.  A wider tile reads
-// the codes for more rows at once and holds more sums in registers (head size 256 and f32 rows: 16 at most).
+constexpr int kEngineRows = 1;
+constexpr int kEngineTile = 2;
+
+// Query rows that share a sequence's head, on average where their numbers are the device's.
+int64_t rows_each(const nnb200_attention_i8_args& a)
+{
+    const nnb200_cache_i8& c = a.cache;
+    return (c.rows + c.seqs - 1) / c.seqs * (a.q_heads / c.heads);
+}
+
+int engine_of(const nnb200_attention_i8_args& a)
+{
+    if (a.float_type == NNB200_FLOAT_F32) {
+        return kEngineRows;   // the tiles hold queries and weights as one f16
+    }
+    return a.force_engine != 0 ? a.force_engine : rows_each(a) > 64 ? kEngineTile : kEngineRows;
+}
+
+// Tiles of 8, 16 or 32 query rows: as many as a sequence has.  A wider tile reads the codes for more rows at once and holds
+// more sums in registers (head size 256 and f32 rows: 16 at most).
 RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
 {
     const nnb200_cache_i8& c = a.cache;
-    const int64_t rows = (c.rows + c.seqs - 1) / c.seqs * (a.q_heads / c.heads);
+    const int64_t rows = rows_each(a);
     RowsPlan p;
     p.columns = rows <= 8 ? 1 : (rows <= 16 || c.dim > 128 || a.float_type == NNB200_FLOAT_F32) ? 2 : 4;
     p.blocks = dev.sm_count * (p.columns == 1 && c.dim <= 128 ? 2 : 1);
@@ -20,11 +38,28 @@ RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
     return p;
 }
 
-}  // namespace
+// Where the parts of the tile kernels' workspace lie, each at a multiple of 16 bytes.
+struct TilePlan {
+    size_t tiles, first_tile, pieces, sums, bytes;   // the line's lengths are at 0
+};
 
-size_t attention_i8_workspace_bytes(const nnb200_attention_i8_args& a, const DeviceInfo& dev) { return rows_plan(a, dev).bytes; }
+TilePlan tile_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
+{
+    const nnb200_cache_i8& c = a.cache;
+    const int64_t group = a.q_heads / c.heads, rows = tile_rows(c.dim);
+    const int64_t most = c.cu == nullptr ? c.seqs * ((c.rows / c.seqs * group + rows - 1) / rows) : c.rows * group / rows + c.seqs;
+    const auto up = [](size_t v) { return (v + 15) / 16 * 16; };
+    const size_t pieces = 2 * static_cast<size_t>(dev.sm_count);
+    TilePlan p;
+    p.tiles = 16;
+    p.first_tile = p.tiles + up(static_cast<size_t>(most) * sizeof(TileInfo));
+    p.pieces = p.first_tile + up(static_cast<size_t>(c.seqs + 1) * sizeof(int32_t));
+    p.sums = p.pieces + up(pieces * sizeof(RowsPiece));
+    p.bytes = p.sums + pieces * static_cast<size_t>(rows) * static_cast<size_t>(c.dim + 2) * sizeof(float);
+    return p;
+}
 
-int launch_attention_i8(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStream_t stream)
+int run_rows(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStream_t stream)
 {
     const RowsPlan p = rows_plan(a, dev);
     RowsCall call;
@@ -40,6 +75,44 @@ int launch_attention_i8(const nnb200_attention_i8_args& a, const DeviceInfo& dev
     case 128: return cuda_status(launch_attention_rows_128(call, p.columns, p.blocks, stream));
     default: return cuda_status(launch_attention_rows_256(call, p.columns, p.blocks, stream));
     }
+}
+
+int run_tile(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStream_t stream)
+{
+    const TilePlan p = tile_plan(a, dev);
+    const auto wide = [](const void* q, int64_t row, int64_t head) {
+        return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && row % 8 == 0 && head % 8 == 0;
+    };
+    TileCall call;
+    call.a = a;
+    call.error_word = dev.error_word;
+    call.group = static_cast<int>(a.q_heads / a.cache.heads);
+    call.factor = a.scale * 1.4426950408889634f;
+    call.wide = wide(a.q, a.q_stride_row, a.q_stride_head) && wide(a.out, a.out_stride_row, a.out_stride_head) ? 1 : 0;
+    uint8_t* const base = static_cast<uint8_t*>(a.workspace);
+    call.line = reinterpret_cast<int64_t*>(base);
+    call.tiles = reinterpret_cast<TileInfo*>(base + p.tiles);
+    call.first_tile = reinterpret_cast<int32_t*>(base + p.first_tile);
+    call.pieces = reinterpret_cast<RowsPiece*>(base + p.pieces);
+    call.sums = reinterpret_cast<float*>(base + p.sums);
+    switch (a.cache.dim) {
+    case 64: return cuda_status(launch_attention_tile_64(call, dev.sm_count, stream));
+    case 96: return cuda_status(launch_attention_tile_96(call, dev.sm_count, stream));
+    case 128: return cuda_status(launch_attention_tile_128(call, dev.sm_count, stream));
+    default: return cuda_status(launch_attention_tile_256(call, dev.sm_count, stream));
+    }
+}
+
+}  // namespace
+
+size_t attention_i8_workspace_bytes(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
+{
+    return engine_of(a) == kEngineTile ? tile_plan(a, dev).bytes : rows_plan(a, dev).bytes;
+}
+
+int launch_attention_i8(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStream_t stream)
+{
+    return engine_of(a) == kEngineTile ? run_tile(a, dev, stream) : run_rows(a, dev, stream);
 }
 
 }  // namespace nnb200

@@ -1,0 +1,810 @@
+// Attention over a key/value cache in 8 bits, for many rows a sequence (prompts, chunks of prompts): the same mathematics as
+// attention_i8_rows.cuh, on the fifth-generation tensor cores.
+//
+// A block of the grid takes 256 query rows of a key head at a time (token by token, the heads of the group next to each
+// other; 128 with head size 256) as one or two M = 128 operands of tcgen05.mma, and runs along the tokens in blocks of 128:
+//
+//     S = Q K^T           Q and K f16 in shared memory, S f32 in tensor memory
+//     P = 2^(t - m)       a thread has a row: no exchange between threads; P f16 over S in tensor memory
+//     O += P V            P from tensor memory, V f16 in shared memory (its dim contiguous: the MN-major form)
+//
+// The cache stays in 8 bits up to the SM: four warps load codes, turn them into f16 integers (exact) and store them in the
+// 128-byte-swizzled order that the MMAs read.  That work serves 256 rows, and is done while the tensor cores and the two
+// groups of four softmax warps work on the block before.  The two halves of the rows alternate: one half's weights are computed while
+// the other half's products run.  Every block's scales come along in shared memory, one for each 16 tokens.
+//
+// The sums are rescaled only when a row's maximum has grown by more than 2^8 since they were last: until then weights are at
+// most 2^8, which f16 and the f32 sums hold as well as 1.
+//
+// Sequences, tiles and heads are one line of 128-token blocks, cut into equal pieces, as in attention_i8_rows.cuh; a first
+// kernel writes down which tiles there are.
+#pragma once
+
+#include "attention_i8_rows.cuh"
+
+namespace nnb200 {
+
+constexpr int kTileKeys = 128;
+constexpr int kTileGroups = kTileKeys / 16;
+constexpr int kMetaSlots = 4;   // blocks whose scales are kept: the one the softmax is at, and those the converters are ahead by
+
+// One tile of query rows, of every head.
+struct TileInfo {
+    int32_t seq, tile, row0, n, len;   // the sequence's, as in SequenceRows
+    int32_t blocks;                    // of 128 tokens, for each head
+    int64_t before;                    // blocks of all tiles before this one, of one head
+};
+
+struct TileCall {
+    nnb200_attention_i8_args a;
+    int32_t* error_word;
+    int group;
+    float factor;
+    int wide;             // q's and out's rows and heads are 16-byte aligned
+    int64_t* line;        // [0] tiles, [1] blocks of all tiles, of one head
+    TileInfo* tiles;
+    int32_t* first_tile;  // [seqs + 1]: tiles before each sequence's
+    RowsPiece* pieces;    // [blocks of the grid][2]
+    float* sums;          // [blocks of the grid][2][dim / 4][rows][4], then m and l of each row
+};
+
+// What a tile's rows see, as a list of 16-token groups: the sinks' first, then those from first_group on.
+struct TileRange {
+    int sink_groups, first_group, groups;
+    int least_pos[2], most_pos[2];   // of each 128 rows; without causality beyond every token
+};
+
+template <int ROWS>
+__device__ __forceinline__ TileRange tile_range(const TileCall& call, int tile, int n, int len)
+{
+    const nnb200_attention_i8_args& a = call.a;
+    const int all = n * call.group, first_pos = len - n;
+    TileRange r;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int low = min(tile * ROWS + t * 128, all - 1), high = min(tile * ROWS + t * 128 + 127, all - 1);
+        r.least_pos[t] = a.causal != 0 ? first_pos + low / call.group : 0x7FFFFFFF;
+        r.most_pos[t] = a.causal != 0 ? first_pos + high / call.group : 0x7FFFFFFF;
+    }
+    const int last = ROWS == 256 ? 1 : 0;
+    const int high = r.most_pos[last] < len ? max(r.most_pos[last] + 1, 0) : len;
+    int64_t low = a.window > 0 ? static_cast<int64_t>(r.least_pos[0]) - a.window + 1 : 0;
+    low = low < 0 ? 0 : low > high ? high : low;
+    r.first_group = static_cast<int>(low) / 16;
+    const int sinks = static_cast<int>(a.sinks < high ? a.sinks : high);
+    r.sink_groups = a.window > 0 ? min((sinks + 15) / 16, r.first_group) : 0;
+    r.groups = r.sink_groups + (high + 15) / 16 - r.first_group;
+    return r;
+}
+
+// Which tiles there are, and where each begins on the line.  One block.
+template <int ROWS>
+__global__ void __launch_bounds__(1024) attention_i8_plan_kernel(const TileCall call)
+{
+    previous_kernel_done();
+    __shared__ int64_t part[32];
+    __shared__ int64_t carry;
+    const int seqs = static_cast<int>(call.a.cache.seqs), lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    // Of the threads before this one, on top of what earlier rounds left.
+    const auto before = [&](int64_t v) {
+        int64_t up = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t other = __shfl_up_sync(0xFFFFFFFFu, up, o);
+            up += lane >= o ? other : 0;
+        }
+        if (lane == 31) {
+            part[warp] = up;
+        }
+        __syncthreads();
+        int64_t sum = carry;
+        for (int i = 0; i < warp; ++i) {
+            sum += part[i];
+        }
+        __syncthreads();
+        if (threadIdx.x == 1023) {
+            carry = sum + up;
+        }
+        __syncthreads();
+        return sum + up - v;
+    };
+    if (threadIdx.x == 0) {
+        carry = 0;
+    }
+    __syncthreads();
+    for (int b0 = 0; b0 < seqs; b0 += 1024) {
+        const int b = b0 + static_cast<int>(threadIdx.x);
+        const int own = b < seqs ? (sequence_rows(call.a.cache, b).n * call.group + ROWS - 1) / ROWS : 0;
+        const int64_t first = before(own);
+        if (b < seqs) {
+            call.first_tile[b] = static_cast<int32_t>(first);
+        }
+    }
+    const int tiles = static_cast<int>(carry);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        call.first_tile[seqs] = tiles;
+        call.line[0] = tiles;
+        carry = 0;
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < tiles; i0 += 1024) {
+        const int i = i0 + static_cast<int>(threadIdx.x);
+        TileInfo info{};
+        if (i < tiles) {
+            int low = 0, high = seqs;   // first_tile[low] <= i < first_tile[high]
+            while (high - low > 1) {
+                const int mid = (low + high) / 2;
+                (call.first_tile[mid] <= i ? low : high) = mid;
+            }
+            const SequenceRows s = sequence_rows(call.a.cache, low);
+            info.seq = low;
+            info.tile = i - call.first_tile[low];
+            info.row0 = s.row0;
+            info.n = s.n;
+            info.len = s.len;
+            info.blocks = max((tile_range<ROWS>(call, info.tile, s.n, s.len).groups + kTileGroups - 1) / kTileGroups, 1);
+        }
+        info.before = before(info.blocks);
+        if (i < tiles) {
+            call.tiles[i] = info;
+        }
+    }
+    if (threadIdx.x == 0) {
+        call.line[1] = carry;
+    }
+}
+
+// A walk over this block's piece of the line: the same for every warp.
+struct TileWalk {
+    int64_t at, end;
+    int tiles, index;    // index: of the tile that `at` lies in, or an earlier one
+    // The part of a tile and head that comes next.
+    TileInfo info;
+    int head, off, count;
+    bool begins, ends;
+
+    // Warp-collective.
+    __device__ __forceinline__ void begin(const TileCall& call, int block, int blocks)
+    {
+        tiles = static_cast<int>(call.line[0]);
+        const int64_t line = call.line[1] * call.a.cache.heads;
+        const int64_t most = line < blocks ? line : blocks;   // a block at least for each piece
+        at = end = 0;
+        index = 0;
+        if (block >= most) {
+            return;
+        }
+        at = line / most * block + line % most * block / most;
+        end = line / most * (block + 1) + line % most * (block + 1) / most;
+        // The last tile that begins at or before `at`, 32 probes at a time.
+        int count_ = tiles;
+        const int lane = static_cast<int>(threadIdx.x & 31);
+        while (count_ > 1) {
+            const int step = (count_ + 31) / 32;
+            const bool before = lane * step < count_ && call.tiles[index + lane * step].before * call.a.cache.heads <= at;
+            const int last = (__popc(__ballot_sync(0xFFFFFFFFu, before)) - 1) * step;
+            index += last;
+            count_ = min(step, count_ - last);
+        }
+    }
+
+    __device__ __forceinline__ bool next(const TileCall& call)
+    {
+        if (at >= end) {
+            return false;
+        }
+        info = call.tiles[index];
+        const int64_t heads = call.a.cache.heads;
+        while (at >= (info.before + info.blocks) * heads) {
+            info = call.tiles[++index];
+        }
+        const int64_t rel = at - info.before * heads;
+        head = static_cast<int>(rel / info.blocks);
+        off = static_cast<int>(rel % info.blocks);
+        count = static_cast<int>(min(static_cast<int64_t>(info.blocks - off), end - at));
+        begins = off == 0;
+        ends = off + count == info.blocks;
+        at += count;
+        return true;
+    }
+};
+
+struct GroupMeta {
+    float k, v_log2, v_inv;
+    int key0;   // first token; its low bits: 1 (2) if the first (second) 128 rows do not see all of its tokens
+};
+
+template <int D>
+struct TileShared {
+    static constexpr int kHalves = D <= 128 ? 2 : 1;
+    static constexpr int kRows = 128 * kHalves;
+    static constexpr int kBlockBytes = 16384;   // 128 rows of 128 bytes: 64 f16 of each token
+    static constexpr int kTileBytes = (D + 63) / 64 * kBlockBytes;
+    static constexpr int kStages = D <= 128 ? 2 : 1;
+    static constexpr int kBytes = 1024 + (kHalves + 2 * kStages) * kTileBytes;
+    static constexpr int kSoftmaxWarps = 4 * kHalves;
+    static constexpr int kThreads = 32 * (kSoftmaxWarps + 5);
+    static constexpr int kOutColumn = 256;      // of the sums in tensor memory; S and P are below
+    static_assert(kBytes <= 225 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void tile_mma_p(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tile_tmem_st_16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+          "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tile_tmem_ld_16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tile_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Every lane polls: the data behind the barrier is then every lane's.
+__device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
+{
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
+}
+
+// 16 codes as f16 into the swizzled tile: row `key`, dims [16 segment, + 16).
+template <int D>
+__device__ __forceinline__ void store_codes(uint8_t* tile, int key, int segment, const uint4& codes)
+{
+    uint32_t h[8];
+    codes_to_half(codes.x, h[0], h[1]);
+    codes_to_half(codes.y, h[2], h[3]);
+    codes_to_half(codes.z, h[4], h[5]);
+    codes_to_half(codes.w, h[6], h[7]);
+    uint8_t* row = tile + segment / 4 * TileShared<D>::kBlockBytes + key * 128;
+    const int chunk = 2 * segment & 7, turn = segment / 4 & 1;   // lanes of the two 64-dim blocks use different banks
+    const uint4 a = make_uint4(h[0], h[1], h[2], h[3]), b = make_uint4(h[4], h[5], h[6], h[7]);
+    *reinterpret_cast<uint4*>(row + (((chunk + turn) ^ (key & 7)) << 4)) = turn ? b : a;
+    *reinterpret_cast<uint4*>(row + (((chunk + 1 - turn) ^ (key & 7)) << 4)) = turn ? a : b;
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_kernel(const TileCall call)
+{
+    using Shared = TileShared<D>;
+    constexpr int kHalves = Shared::kHalves, kStages = Shared::kStages, kRows = Shared::kRows;
+    constexpr int kPerThread = D / 16;   // 16-code segments of a tile that a converting thread has
+    extern __shared__ uint8_t raw_shared[];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+    __shared__ GroupMeta meta[kMetaSlots][kTileGroups];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+
+    uint8_t* const shared = raw_shared + (1024 - smem_u32(raw_shared) % 1024) % 1024;
+    uint8_t* const q_tile = shared;
+    uint8_t* const k_tile = q_tile + kHalves * Shared::kTileBytes;
+    uint8_t* const v_tile = k_tile + kStages * Shared::kTileBytes;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 128);
+            mbar_init(&k_full[i], 128);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init_fence();
+    }
+    if (warp == Shared::kSoftmaxWarps + 4) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    previous_kernel_done();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    const nnb200_attention_i8_args& a = call.a;
+
+    TileWalk walk;
+    walk.begin(call, blockIdx.x, gridDim.x);
+
+    if (warp < Shared::kSoftmaxWarps) {
+        // ---------------- softmax: a thread has a row ----------------
+        const int half = warp / 4, row = threadIdx.x & 127;
+        const uint32_t s_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(half * 128);
+        const uint32_t o_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(Shared::kOutColumn + half * 128);
+        uint8_t* const q_row = q_tile + half * Shared::kTileBytes + row * 128;
+        uint32_t n = 0;   // blocks
+        int kinds[2] = {0, 0};
+        bool ok = true;
+        while (ok && walk.next(call)) {
+            const int global = walk.info.tile * kRows + half * 128 + row;
+            const bool there = global < walk.info.n * call.group;
+            const int token = global / call.group, head = walk.head * call.group + global % call.group;
+            int pos = a.causal != 0 ? walk.info.len - walk.info.n + token : 0x7FFFFFFF;
+            pos = pos < walk.info.len ? pos : walk.info.len - 1;
+            const int64_t low = a.window > 0 && there ? static_cast<int64_t>(pos) - a.window + 1 : INT64_MIN;
+
+            // The row's queries, scaled by a power of two into f16.
+            const T* src = static_cast<const T*>(a.q) + (there ? (walk.info.row0 + token) * a.q_stride_row + head * a.q_stride_head : 0);
+            float up = call.factor, down = 1.0f;
+            if constexpr (!std::is_same_v<T, __half>) {
+                uint32_t top = 0;
+                for (int c = 0; c < D / 8 && there; ++c) {
+                    float f[8];
+                    load8(src + c * 8, call.wide != 0, f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        top = max(top, magnitude_bits(f[e]));
+                    }
+                }
+                const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+                down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                up *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+                float f[8] = {};
+                if (there) {
+                    load8(src + c * 8, call.wide != 0, f);
+                }
+                if constexpr (!std::is_same_v<T, __half>) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] *= down;
+                    }
+                }
+                *reinterpret_cast<uint4*>(q_row + c / 8 * Shared::kBlockBytes + (((c & 7) ^ (row & 7)) << 4)) =
+                    make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]), pack2<__half>(f[4], f[5]), pack2<__half>(f[6], f[7]));
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&q_full[half]);
+
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < walk.count; ++j, ++n) {
+                if (!tile_wait(&s_full[half], n & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const GroupMeta* groups = meta[n % kMetaSlots];
+                // t of 16 tokens; those that the row does not see are -infinity.
+                const auto exponents = [&](const uint32_t* s, const GroupMeta& g, float add, float (&t)[16]) {
+                    const float k = g.k * up;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        t[i] = __fmaf_rn(__uint_as_float(s[i]), k, add);
+                    }
+                    if (g.key0 >> half & 1) {
+                        const int key0 = g.key0 & ~15;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = key0 + i;
+                            t[i] = key <= pos && (key >= low || key < a.sinks) ? t[i] : -INFINITY;
+                        }
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32];
+                    tmem_ld_32x32(s_addr + static_cast<uint32_t>(c * 32), s);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const GroupMeta g = groups[2 * c + h];
+                        float t[16];
+                        exponents(s + 16 * h, g, g.v_log2, t);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            top = fmaxf(top, t[i]);
+                        }
+                    }
+                }
+                const bool grown = top > m + 8.0f || (m == -INFINITY && top > m);
+                const float next = grown ? top : m;
+                const float alpha = grown ? exp2_fast(m - next) : 1.0f;
+                if (j > 0 && __any_sync(0xFFFFFFFFu, grown)) {
+                    // The sums so far are complete: the next block's products wait for this one's weights.
+                    if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tile_tmem_ld_16(o_addr + static_cast<uint32_t>(c * 16), o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        }
+                        tile_tmem_st_16(o_addr + static_cast<uint32_t>(c * 16), o);
+                    }
+                }
+                m = next;
+                l *= alpha;
+                const float safe = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32];
+                    tmem_ld_32x32(s_addr + static_cast<uint32_t>(c * 32), s);
+                    tmem_ld_wait();
+                    uint32_t p[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const GroupMeta g = groups[2 * c + h];
+                        float t[16], sum = 0.0f;
+                        exponents(s + 16 * h, g, g.v_log2 - safe, t);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            t[i] = exp2_fast(t[i]);
+                            sum += t[i];
+                        }
+                        l += sum == 0.0f ? 0.0f : sum * g.v_inv;   // (0 times what a masked block has for a scale)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            p[8 * h + i] = pack2<__half>(t[2 * i], t[2 * i + 1]);
+                        }
+                    }
+                    tile_tmem_st_16(s_addr + static_cast<uint32_t>(c * 16), p);
+                }
+                tile_tmem_st_wait();
+                tc_fence_before_sync();
+                mbar_arrive(&p_full[half]);
+            }
+            if (!ok || !tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            const bool whole = walk.begins && walk.ends;
+            const int which = walk.begins ? 1 : 0;
+            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+            float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kRows * (D + 2));
+            T* dst = static_cast<T*>(a.out) + (there ? (walk.info.row0 + token) * a.out_stride_row + head * a.out_stride_head : 0);
+#pragma unroll 2
+            for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tile_tmem_ld_16(o_addr + static_cast<uint32_t>(c * 16), o);
+                tmem_ld_wait();
+                if (there && whole) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float f[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            f[i] = __uint_as_float(o[8 * h + i]) * inv;
+                        }
+                        store8(dst + c * 16 + h * 8, call.wide != 0, f);
+                    }
+                } else if (there) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        reinterpret_cast<uint4*>(piece)[(c * 4 + i) * kRows + half * 128 + row] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+            }
+            if (!whole) {
+                if (there) {
+                    piece[kRows * D + half * 128 + row] = m;
+                    piece[kRows * (D + 1) + half * 128 + row] = l;
+                }
+                kinds[which] = walk.begins ? 1 : walk.ends ? 3 : 2;
+                if (threadIdx.x == 0) {
+                    call.pieces[2 * blockIdx.x + which] = RowsPiece{kinds[which], walk.info.seq, walk.head, walk.info.tile};
+                }
+            }
+            tc_fence_before_sync();
+        }
+        if (threadIdx.x < 2 && kinds[threadIdx.x] == 0) {
+            call.pieces[2 * blockIdx.x + threadIdx.x].kind = 0;
+        }
+        if (!ok && lane == 0) {
+            atomicCAS(call.error_word, 0, kErrEpilogueWait);
+        }
+        __syncwarp();
+    } else if (warp < Shared::kSoftmaxWarps + 4) {
+        // ---------------- codes into f16 tiles ----------------
+        const int t = threadIdx.x - 32 * Shared::kSoftmaxWarps;
+        const int page_tokens = static_cast<int>(a.cache.page_tokens);
+        const int64_t head_bytes = static_cast<int64_t>(page_tokens) * D;
+        // The block that is being loaded: where each of its groups lies (lanes 0..7), or -1.
+        TileRange range{};
+        int j = 0;
+        bool more = walk.next(call);
+        int64_t where = -1;
+        GroupMeta mine{};
+        const auto locate = [&] {   // of block j of the walk's part
+            if (j == 0) {
+                range = tile_range<kRows>(call, walk.info.tile, walk.info.n, walk.info.len);
+            }
+            where = -1;
+            mine = GroupMeta{0.0f, -INFINITY, 0.0f, 0};
+            const int idx = (walk.off + j) * kTileGroups + lane;
+            if (lane < kTileGroups && idx < range.groups) {
+                const int key0 = (idx < range.sink_groups ? idx : idx - range.sink_groups + range.first_group) * 16;
+                const int page = page_at(a.cache, walk.info.seq, key0 / page_tokens, call.error_word);
+                if (page >= 0) {
+                    const int64_t at = page * a.cache.scale_page_stride + walk.head;
+                    const float vs = a.cache.v_scale[at];
+                    where = page * a.cache.page_stride + walk.head * head_bytes + key0 % page_tokens * D;
+                    mine.k = a.cache.k_scale[at];
+                    mine.v_log2 = vs < kLeastCacheScale ? kLeastCacheScale : vs;
+                    mine.key0 = key0;
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) {
+                        const bool all_seen = key0 + 15 < walk.info.len && key0 + 15 <= range.least_pos[h] &&
+                                              (a.window == 0 || key0 > range.most_pos[h] - a.window || key0 + 15 < a.sinks);
+                        mine.key0 |= all_seen ? 0 : 1 << h;
+                    }
+                }
+            }
+        };
+        const auto load = [&](const void* codes, uint4 (&raw)[kPerThread]) {
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int idx = t + i * 128, key = idx / kPerThread, segment = idx % kPerThread;
+                const int64_t base = __shfl_sync(0xFFFFFFFFu, where, key / 16);
+                raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (base >= 0) {
+                    raw[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(codes) + base + (key & 15) * D + segment * 16);
+                }
+            }
+        };
+        const auto store = [&](uint8_t* tile, const uint4 (&raw)[kPerThread]) {
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int idx = t + i * 128;
+                store_codes<D>(tile, idx / kPerThread, idx % kPerThread, raw[i]);
+            }
+        };
+        uint4 raw_k[kPerThread], raw_v[kPerThread];
+        if (more) {
+            locate();
+            load(a.cache.k, raw_k);
+        }
+        bool ok = true;
+        for (uint32_t n = 0; more; ++n) {
+            load(a.cache.v, raw_v);
+            const GroupMeta now = mine;
+            const uint32_t slot = n % kStages, round = n / kStages & 1;
+            if (!tile_wait(&k_empty[slot], round ^ 1, &abort_flag)) {
+                ok = false;
+                break;
+            }
+            if (t < kTileGroups) {
+                const float vs = now.v_log2;
+                meta[n % kMetaSlots][t] = now.v_log2 == -INFINITY ? now : GroupMeta{now.k, log2f(vs), __fdiv_rn(1.0f, vs), now.key0};
+            }
+            store(k_tile + slot * Shared::kTileBytes, raw_k);
+            fence_proxy_async_smem();
+            mbar_arrive(&k_full[slot]);
+            if (++j == walk.count) {
+                j = 0;
+                more = walk.next(call);
+            }
+            if (more) {
+                locate();
+                load(a.cache.k, raw_k);
+            }
+            if (!tile_wait(&v_empty[slot], round ^ 1, &abort_flag)) {
+                ok = false;
+                break;
+            }
+            store(v_tile + slot * Shared::kTileBytes, raw_v);
+            fence_proxy_async_smem();
+            mbar_arrive(&v_full[slot]);
+        }
+        if (!ok && lane == 0) {
+            atomicCAS(call.error_word, 0, kErrDequantWait);
+        }
+        __syncwarp();
+    } else {
+        // ---------------- MMA issuer ----------------
+        const uint32_t base = warp_uniform(tmem);
+        constexpr uint32_t kIdescS = umma_idesc(1, 0, 0, 128, kTileKeys);
+        constexpr uint32_t kIdescO = umma_idesc(1, 0, 0, 128, D) | kUmmaBMajorMN;
+        const uint64_t q_desc = umma_desc_sw128_kmajor(smem_u32(q_tile));
+        const uint64_t k_desc = umma_desc_sw128_kmajor(smem_u32(k_tile));
+        const uint64_t v_desc = umma_desc_sw128_mnmajor(smem_u32(v_tile), Shared::kBlockBytes);
+        constexpr uint64_t kTileStep = Shared::kTileBytes / 16, kBlockStep = Shared::kBlockBytes / 16;
+        uint32_t failed = 0;
+        const auto scores = [&](int half, uint32_t slot) {
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t step = static_cast<uint64_t>(k / 4) * kBlockStep + static_cast<uint64_t>(k % 4 * 2);
+                    umma_f16(base + static_cast<uint32_t>(half * 128), q_desc + static_cast<uint64_t>(half) * kTileStep + step,
+                             k_desc + slot * kTileStep + step, kIdescS, k > 0 ? 1u : 0u);
+                }
+                umma_commit_unless(&s_full[half], failed);
+            }
+            __syncwarp();
+        };
+        uint32_t n = 0, units = 0;
+        while (walk.next(call)) {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                mbar_wait_converged<kErrMmaWait>(&q_full[h], units & 1, &abort_flag, failed);
+            }
+            mbar_wait_converged<kErrMmaWait>(&k_full[n % kStages], n / kStages & 1, &abort_flag, failed);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                scores(h, n % kStages);
+            }
+            if (elect_one()) {
+                umma_commit_unless(&k_empty[n % kStages], failed);
+            }
+            __syncwarp();
+            for (int j = 0; j < walk.count; ++j, ++n) {
+                const bool next = j + 1 < walk.count;
+                const uint32_t slot = n % kStages, next_slot = (n + 1) % kStages;
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h) {
+                    mbar_wait_converged<kErrMmaWait>(&p_full[h], n & 1, &abort_flag, failed);
+                    if (h == 0) {
+                        mbar_wait_converged<kErrMmaWait>(&v_full[slot], n / kStages & 1, &abort_flag, failed);
+                    }
+                    tc_fence_after_sync();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < kTileKeys / 16; ++k) {
+                            tile_mma_p(base + static_cast<uint32_t>(Shared::kOutColumn + h * 128), base + static_cast<uint32_t>(h * 128 + k * 8),
+                                       v_desc + slot * kTileStep + static_cast<uint64_t>(k * 2048 / 16), kIdescO, j > 0 || k > 0 ? 1u : 0u);
+                        }
+                        umma_commit_unless(&o_full[h], failed);
+                    }
+                    __syncwarp();
+                    if (next) {
+                        if (h == 0) {
+                            mbar_wait_converged<kErrMmaWait>(&k_full[next_slot], (n + 1) / kStages & 1, &abort_flag, failed);
+                            tc_fence_after_sync();
+                        }
+                        scores(h, next_slot);
+                    }
+                }
+                if (elect_one()) {
+                    umma_commit_unless(&v_empty[slot], failed);
+                    if (next) {
+                        umma_commit_unless(&k_empty[next_slot], failed);
+                    }
+                }
+                __syncwarp();
+            }
+            ++units;
+        }
+        if (const uint32_t code = warp_failure(failed); code != 0) {
+            if (lane == 0) {
+                atomicCAS(call.error_word, 0, static_cast<int32_t>(code));
+            }
+            umma_settle_after_failure();
+        }
+        __syncwarp();
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == Shared::kSoftmaxWarps + 4) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the pieces of the tiles that were cut: blockIdx.x of the grid of the kernel before, in gridDim.y parts.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) attention_i8_tile_join_kernel(const TileCall call)
+{
+    previous_kernel_done();
+    constexpr int kRows = TileShared<D>::kRows;
+    constexpr int64_t kPiece = kRows * (D + 2);
+    const RowsPiece mine = call.pieces[2 * blockIdx.x + 1];
+    if (mine.kind != 1) {
+        return;
+    }
+    const nnb200_attention_i8_args& a = call.a;
+    const SequenceRows s = sequence_rows(a.cache, mine.seq);
+    const int rows = min(kRows, s.n * call.group - mine.tile * kRows);
+    int last = blockIdx.x + 1;
+    while (last < static_cast<int>(gridDim.x) - 1 && call.pieces[2 * last].kind == 2) {
+        ++last;
+    }
+    const float* first = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kPiece;
+    const float* rest = call.sums + 2 * static_cast<int64_t>(blockIdx.x + 1) * kPiece;
+    const int more = last - static_cast<int>(blockIdx.x);
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < kRows * (D / 4); i += 256 * gridDim.y) {
+        const int r = i % kRows, d = i / kRows * 4;
+        if (r >= rows) {
+            continue;
+        }
+        float top = first[kRows * D + r];
+        for (int p = 0; p < more; ++p) {
+            top = fmaxf(top, rest[p * 2 * kPiece + kRows * D + r]);
+        }
+        const float safe = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = -1; p < more; ++p) {
+            const float* piece = p < 0 ? first : rest + p * 2 * kPiece;
+            const float share = exp2_fast(piece[kRows * D + r] - safe);
+            const float4 v = reinterpret_cast<const float4*>(piece)[d / 4 * kRows + r];
+            total = __fmaf_rn(piece[kRows * (D + 1) + r], share, total);
+            sum.x = __fmaf_rn(v.x, share, sum.x);
+            sum.y = __fmaf_rn(v.y, share, sum.y);
+            sum.z = __fmaf_rn(v.z, share, sum.z);
+            sum.w = __fmaf_rn(v.w, share, sum.w);
+        }
+        const int global = mine.tile * kRows + r;
+        T* dst = static_cast<T*>(a.out) + (s.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d;
+        const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+        dst[0] = from_float<T>(sum.x * inv);
+        dst[1] = from_float<T>(sum.y * inv);
+        dst[2] = from_float<T>(sum.z * inv);
+        dst[3] = from_float<T>(sum.w * inv);
+    }
+}
+
+template <int D, typename T>
+cudaError_t launch_tile_typed(const TileCall& call, int blocks, cudaStream_t stream)
+{
+    using Shared = TileShared<D>;
+    const auto kernel = attention_i8_tile_kernel<D, T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared::kBytes);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return e;
+    }
+    const unsigned grid = static_cast<unsigned>(blocks);
+    e = launch_overlapping(attention_i8_plan_kernel<Shared::kRows>, dim3(1), dim3(1024), 0, stream, 1, call);
+    note_launch();
+    if (e != cudaSuccess) {
+        return e;
+    }
+    e = launch_overlapping(kernel, dim3(grid), dim3(Shared::kThreads), Shared::kBytes, stream, 1, call);
+    note_launch();
+    if (e != cudaSuccess) {
+        return e;
+    }
+    e = launch_overlapping(attention_i8_tile_join_kernel<D, T>, dim3(grid, 8), dim3(256), 0, stream, 1, call);
+    note_launch();
+    return e;
+}
+
+template <int D>
+cudaError_t launch_tile_dim(const TileCall& call, int blocks, cudaStream_t stream)
+{
+    return call.a.float_type == NNB200_FLOAT_F16 ? launch_tile_typed<D, __half>(call, blocks, stream)
+                                                 : launch_tile_typed<D, __nv_bfloat16>(call, blocks, stream);
+}
+
+constexpr int tile_rows(int64_t dim) { return dim <= 128 ? 256 : 128; }
+
+cudaError_t launch_attention_tile_64(const TileCall& call, int blocks, cudaStream_t stream);
+cudaError_t launch_attention_tile_96(const TileCall& call, int blocks, cudaStream_t stream);
+cudaError_t launch_attention_tile_128(const TileCall& call, int blocks, cudaStream_t stream);
+cudaError_t launch_attention_tile_256(const TileCall& call, int blocks, cudaStream_t stream);
+
+}  // namespace nnb200

@@ -1230,7 +1230,7 @@ int check_cache_rows(const nnb200_cache_rows_args* a, bool* empty)
 
 int check_attention(const nnb200_attention_i8_args* a, bool* empty)
 {
-    if (a == nullptr || !float_type_ok(a->float_type) || a->q_heads < 1 || a->window < 0 || a->sinks < 0 || a->force_engine < 0 || a->force_engine > 1) {
+    if (a == nullptr || !float_type_ok(a->float_type) || a->q_heads < 1 || a->window < 0 || a->sinks < 0 || a->force_engine < 0 || a->force_engine > 2) {
         return NNB200_INVALID_ARGUMENT;
     }
     const int status = check_cache(a->cache, empty);
@@ -1240,6 +1240,9 @@ int check_attention(const nnb200_attention_i8_args* a, bool* empty)
     const nnb200_cache_i8& c = a->cache;
     if (a->q_heads % c.heads != 0 || (a->window > 0 && a->causal == 0)) {
         return NNB200_INVALID_ARGUMENT;
+    }
+    if (a->force_engine == 2 && a->float_type == NNB200_FLOAT_F32) {
+        return NNB200_UNSUPPORTED;
     }
     if (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) {
         return NNB200_UNSUPPORTED;

@@ -661,7 +661,7 @@ def cache_read_i8(cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, 
     return k, v
 
 
-ATTENTION_ENGINES = {"auto": 0, "rows": 1}
+ATTENTION_ENGINES = {"auto": 0, "rows": 1, "tile": 2}
 
 
 def attention_i8_cache(q: torch.Tensor, cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, *, cu: torch.Tensor | None = None,

@@ -324,10 +324,51 @@ def test_prompts(cuda_device, nnb200_lib, dtype, dim, new):
     _check_attention(_gen(new), dtype, 2, 4, dim, 64, [new, new + 77, 1200, 3], [new, new - 1, 129, 3])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads,group,tokens", [(1, 1, 16), (2, 4, 64), (3, 7, 32), (2, 16, 128)])
+def test_tiles_from_one_row_on(cuda_device, nnb200_lib, dtype, dim, heads, group, tokens):
+    """The kernel for many rows, whatever their number: empty tiles, tiles that end inside a token's heads, lengths around a block's."""
+    lens = [1, 0, 15, 127, 128, 129, 300, 700, 1000]
+    new = [1, 1, 15, 60, 128, 0, 33, 2, 257]
+    _check_attention(_gen(dim + group), dtype, heads, group, dim, tokens, lens, new, engine="tile")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,heads,group,tokens", [(64, 2, 3, 16), (128, 1, 8, 128), (96, 2, 5, 64), (256, 1, 4, 32), (128, 3, 1, 32)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 3), (40, 20), (100, 1), (64, 500)])
+def test_tiles_with_a_window(cuda_device, nnb200_lib, dtype, dim, heads, group, tokens, window, sinks):
+    lens = [5, 333, 0, 64, 200, 31, 90, 700]
+    new = [5, 37, 2, 0, 1, 40, 17, 400]
+    _check_attention(_gen(dim + window), dtype, heads, group, dim, tokens, lens, new, window=window, sinks=sinks, engine="tile")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tiles_without_causality(cuda_device, nnb200_lib, dim):
+    _check_attention(_gen(dim), torch.float16, 2, 4, dim, 32, [3, 400, 0, 65], [7, 130, 1, 2], causal=False, scale=0.03, engine="tile")
+    _check_attention(_gen(dim), torch.float16, 1, 4, dim, 32, [3, 400, 0, 65], [7, 130, 1, 2], scale=-0.1, engine="tile")
+
+
+def test_maxima_that_grow_along_the_tokens(cuda_device, nnb200_lib):
+    """Logits that rise by far more than the sums are rescaled for, block after block, and fall again."""
+    g = _gen(7)
+    for engine in ("rows", "tile"):
+        cache = _filled(g, 40, 1, 32, 64)
+        ramp = torch.cat([torch.linspace(0.01, 4, 20), torch.linspace(4, 0.01, 20)])
+        cache.k_scale.copy_(ramp[:, None] / 127)
+        table, lens, cu = [list(range(40))], [1280], [0, 300]
+        q = (_randn(g, 300, 2, 64) * 8).half()
+        got = ops.attention_i8_cache(q.cuda(), cache, _i32(table), _i32(lens), engine=engine).cpu().double()
+        want, tol = _attention_reference(q, cache, table, lens, cu, 2, True, 0, 0, 1 / 8)
+        assert ((got - want).abs() <= tol).all(), engine
+
+
 def test_long_context_and_many_sequences(cuda_device, nnb200_lib):
     g = _gen(3)
     _check_attention(g, torch.float16, 2, 4, 128, 128, [40001], [3])
     _check_attention(g, torch.float16, 1, 4, 128, 16, [40001, 39000], [2, 1], window=3000, sinks=4)
+    _check_attention(g, torch.float16, 1, 4, 128, 16, [20001, 9000], [70, 64], engine="tile")
+    _check_attention(g, torch.float16, 1, 2, 64, 16, [(37 * i) % 300 for i in range(1100)], [i % 3 for i in range(1100)], engine="tile")
     lens = [(37 * i) % 300 for i in range(700)]
     _check_attention(g, torch.bfloat16, 1, 2, 64, 16, lens, [1] * 700, uniform=True)
     _check_attention(g, torch.float16, 1, 2, 64, 16, lens, [i % 4 for i in range(700)])
@@ -397,27 +438,27 @@ def test_extreme_scales_and_values(cuda_device, nnb200_lib):
     assert ((got - want).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-def test_what_is_masked_may_be_anything(cuda_device, nnb200_lib, dtype):
+@pytest.mark.parametrize("dtype,engine", [*((t, "rows") for t in TYPES), (torch.float16, "tile"), (torch.bfloat16, "tile")])
+def test_what_is_masked_may_be_anything(cuda_device, nnb200_lib, dtype, engine):
     """Scales of NaN and infinity on pages that a row does not see, or sees none of; queries that are NaN stay their own."""
     g = _gen(6)
     cache = _filled(g, 4, 1, 16, 64)
     clean = ops.CacheI8(cache.k, cache.v, cache.k_scale.clone(), cache.v_scale.clone())
     q = _randn(g, 60, 2, 64).to(dtype).cuda()
     table = _i32([[0, 1, 2, 3]])
-    want = ops.attention_i8_cache(q, clean, table, _i32([60]))
+    want = ops.attention_i8_cache(q, clean, table, _i32([60]), engine=engine)
     for bad in (math.nan, math.inf):
         for scale in (cache.k_scale, cache.v_scale):
             cache.k_scale.copy_(clean.k_scale)
             cache.v_scale.copy_(clean.v_scale)
             scale[2] = bad
-            got = ops.attention_i8_cache(q, cache, table, _i32([60]))
+            got = ops.attention_i8_cache(q, cache, table, _i32([60]), engine=engine)
             assert torch.equal(got[:32], want[:32])
             assert not got[32:].isfinite().any() if scale is cache.v_scale or bad != bad else True
-            got = ops.attention_i8_cache(q[50:], cache, table, _i32([60]), window=3, sinks=20)
+            got = ops.attention_i8_cache(q[50:], cache, table, _i32([60]), window=3, sinks=20, engine=engine)
             assert got.isfinite().all()
     q[7, 1, 3] = math.nan
-    got = ops.attention_i8_cache(q, clean, table, _i32([60]))
+    got = ops.attention_i8_cache(q, clean, table, _i32([60]), engine=engine)
     assert got[7, 1].isnan().all()
     rest = torch.ones((60, 2), dtype=torch.bool, device="cuda")
     rest[7, 1] = False
