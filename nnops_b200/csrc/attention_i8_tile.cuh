@@ -26,13 +26,14 @@ namespace nnb200 {
 
 constexpr int kTileKeys = 128;
 constexpr int kTileGroups = kTileKeys / 16;
+constexpr int kTileCost = 4;    // blocks that a part of a tile costs besides its own: queries, first products, sums
 constexpr int kMetaSlots = 4;   // blocks whose scales are kept: the one the softmax is at, and those the converters are ahead by
 
 // One tile of query rows, of every head.
 struct TileInfo {
     int32_t seq, tile, row0, n, len;   // the sequence's, as in SequenceRows
     int32_t blocks;                    // of 128 tokens, for each head
-    int64_t before;                    // blocks of all tiles before this one, of one head
+    int64_t before;                    // length of all tiles before this one, of one head: blocks, and kTileCost for each
 };
 
 struct TileCall {
@@ -41,7 +42,7 @@ struct TileCall {
     int group;
     float factor;
     int wide;             // q's and out's rows and heads are 16-byte aligned
-    int64_t* line;        // [0] tiles, [1] blocks of all tiles, of one head
+    int64_t* line;        // [0] tiles, [1] length of all tiles, of one head
     TileInfo* tiles;
     int32_t* first_tile;  // [seqs + 1]: tiles before each sequence's
     RowsPiece* pieces;    // [blocks of the grid][2]
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(1024) attention_i8_plan_kernel(const TileCall 
             info.len = s.len;
             info.blocks = max((tile_range<ROWS>(call, info.tile, s.n, s.len).groups + kTileGroups - 1) / kTileGroups, 1);
         }
-        info.before = before(info.blocks);
+        info.before = before(i < tiles ? info.blocks + kTileCost : 0);
         if (i < tiles) {
             call.tiles[i] = info;
         }
@@ -168,8 +169,8 @@ struct TileWalk {
     __device__ __forceinline__ void begin(const TileCall& call, int block, int blocks)
     {
         tiles = static_cast<int>(call.line[0]);
-        const int64_t line = call.line[1] * call.a.cache.heads;
-        const int64_t most = line < blocks ? line : blocks;   // a block at least for each piece
+        const int64_t line = call.line[1] * call.a.cache.heads, least = kTileCost;
+        const int64_t most = (line + least - 1) / least < blocks ? (line + least - 1) / least : blocks;
         at = end = 0;
         index = 0;
         if (block >= most) {
@@ -191,22 +192,27 @@ struct TileWalk {
 
     __device__ __forceinline__ bool next(const TileCall& call)
     {
-        if (at >= end) {
-            return false;
+        while (at < end) {
+            info = call.tiles[index];
+            const int64_t heads = call.a.cache.heads;
+            while (at >= (info.before + info.blocks + kTileCost) * heads) {
+                info = call.tiles[++index];
+            }
+            const int length = info.blocks + kTileCost;
+            const int64_t rel = at - info.before * heads;
+            head = static_cast<int>(rel / length);
+            const int from = static_cast<int>(rel % length);
+            const int to = static_cast<int>(min(static_cast<int64_t>(length), from + (end - at)));
+            at += to - from;
+            off = max(from - kTileCost, 0);
+            count = max(to - kTileCost, 0) - off;
+            begins = off == 0;
+            ends = off + count == info.blocks;
+            if (count > 0) {
+                return true;
+            }
         }
-        info = call.tiles[index];
-        const int64_t heads = call.a.cache.heads;
-        while (at >= (info.before + info.blocks) * heads) {
-            info = call.tiles[++index];
-        }
-        const int64_t rel = at - info.before * heads;
-        head = static_cast<int>(rel / info.blocks);
-        off = static_cast<int>(rel % info.blocks);
-        count = static_cast<int>(min(static_cast<int64_t>(info.blocks - off), end - at));
-        begins = off == 0;
-        ends = off + count == info.blocks;
-        at += count;
-        return true;
+        return false;
     }
 };
 
@@ -222,11 +228,20 @@ struct TileShared {
     static constexpr int kBlockBytes = 16384;   // 128 rows of 128 bytes: 64 f16 of each token
     static constexpr int kTileBytes = (D + 63) / 64 * kBlockBytes;
     static constexpr int kStages = D <= 128 ? 2 : 1;
-    static constexpr int kBytes = 1024 + (kHalves + 2 * kStages) * kTileBytes;
+    // Codes on their way: two units, of all 128 tokens of a block, or of 64 with head size 256.
+    static constexpr int kUnits = D <= 128 ? 1 : 2;   // of a block's keys, and of its values
+    static constexpr int kUnitBytes = kTileKeys * D / kUnits;
+    static constexpr int kBytes = 1024 + (kHalves + 2 * kStages) * kTileBytes + 2 * kUnitBytes;
     static constexpr int kSoftmaxWarps = 4 * kHalves;
-    static constexpr int kThreads = 32 * (kSoftmaxWarps + 5);
+    static constexpr int kThreads = 32 * (kSoftmaxWarps + 8);   // and four for codes, and the MMA issuer's group
+    // Registers of a thread: at launch, and of the three kinds of warps afterwards.
+    static constexpr int kRegisters = kHalves == 2 ? 128 : 168;
+    static constexpr int kSoftmaxRegisters = kHalves == 2 ? 184 : 232;
+    static constexpr int kCodesRegisters = kHalves == 2 ? 96 : 160;
+    static constexpr int kIssuerRegisters = kHalves == 2 ? 48 : 96;
+    static_assert(kHalves * kSoftmaxRegisters + kCodesRegisters + kIssuerRegisters <= (kHalves + 2) * kRegisters, "a group would wait for registers");
     static constexpr int kOutColumn = 256;      // of the sums in tensor memory; S and P are below
-    static_assert(kBytes <= 225 * 1024, "shared memory");
+    static_assert(kBytes <= 226 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ void tile_mma_p(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
@@ -262,6 +277,39 @@ __device__ __forceinline__ void tile_tmem_ld_16(uint32_t taddr, uint32_t (&v)[16
 
 __device__ __forceinline__ void tile_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The warpgroup's registers of a thread from here on.
+template <int N>
+__device__ __forceinline__ void more_registers()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pair_of(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // Every lane polls: the data behind the barrier is then every lane's.
 __device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
 {
@@ -289,10 +337,11 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
 {
     using Shared = TileShared<D>;
     constexpr int kHalves = Shared::kHalves, kStages = Shared::kStages, kRows = Shared::kRows;
-    constexpr int kPerThread = D / 16;   // 16-code segments of a tile that a converting thread has
+    constexpr int kPerThread = D / 16 / Shared::kUnits;   // 16-code segments of a unit that a converting thread has
     extern __shared__ uint8_t raw_shared[];
     __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
     __shared__ GroupMeta meta[kMetaSlots][kTileGroups];
+    __shared__ int by_element[kMetaSlots];   // bit h: some group is not just t = s k + v_log2 to half h
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
 
@@ -300,6 +349,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
     uint8_t* const q_tile = shared;
     uint8_t* const k_tile = q_tile + kHalves * Shared::kTileBytes;
     uint8_t* const v_tile = k_tile + kStages * Shared::kTileBytes;
+    uint8_t* const codes_ring = v_tile + kStages * Shared::kTileBytes;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -331,29 +381,38 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
 
     if (warp < Shared::kSoftmaxWarps) {
         // ---------------- softmax: a thread has a row ----------------
+        more_registers<Shared::kSoftmaxRegisters>();
         const int half = warp / 4, row = threadIdx.x & 127;
         const uint32_t s_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(half * 128);
         const uint32_t o_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(Shared::kOutColumn + half * 128);
         uint8_t* const q_row = q_tile + half * Shared::kTileBytes + row * 128;
         uint32_t n = 0;   // blocks
         int kinds[2] = {0, 0};
-        bool ok = true;
-        while (ok && walk.next(call)) {
+        // The row of the part that is next: its place in out, its range of tokens, its factor.
+        bool there = false;
+        int pos = 0;
+        int64_t low = 0, place = 0;
+        float factor = 0.0f;
+        const auto load_queries = [&] {
             const int global = walk.info.tile * kRows + half * 128 + row;
-            const bool there = global < walk.info.n * call.group;
+            there = global < walk.info.n * call.group;
             const int token = global / call.group, head = walk.head * call.group + global % call.group;
-            int pos = a.causal != 0 ? walk.info.len - walk.info.n + token : 0x7FFFFFFF;
+            pos = a.causal != 0 ? walk.info.len - walk.info.n + token : 0x7FFFFFFF;
             pos = pos < walk.info.len ? pos : walk.info.len - 1;
-            const int64_t low = a.window > 0 && there ? static_cast<int64_t>(pos) - a.window + 1 : INT64_MIN;
-
-            // The row's queries, scaled by a power of two into f16.
+            low = a.window > 0 && there ? static_cast<int64_t>(pos) - a.window + 1 : INT64_MIN;
+            place = there ? (walk.info.row0 + token) * a.out_stride_row + head * a.out_stride_head : 0;
+            // Scaled by a power of two into f16.
             const T* src = static_cast<const T*>(a.q) + (there ? (walk.info.row0 + token) * a.q_stride_row + head * a.q_stride_head : 0);
-            float up = call.factor, down = 1.0f;
+            float down = 1.0f;
+            factor = call.factor;
             if constexpr (!std::is_same_v<T, __half>) {
                 uint32_t top = 0;
-                for (int c = 0; c < D / 8 && there; ++c) {
-                    float f[8];
-                    load8(src + c * 8, call.wide != 0, f);
+#pragma unroll 8
+                for (int c = 0; c < D / 8; ++c) {
+                    float f[8] = {};
+                    if (there) {
+                        load8(src + c * 8, call.wide != 0, f);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         top = max(top, magnitude_bits(f[e]));
@@ -361,9 +420,9 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 }
                 const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
                 down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                up *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             }
-#pragma unroll 4
+#pragma unroll 8
             for (int c = 0; c < D / 8; ++c) {
                 float f[8] = {};
                 if (there) {
@@ -380,94 +439,109 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             }
             fence_proxy_async_smem();
             mbar_arrive(&q_full[half]);
-
+        };
+        bool ok = true, more = walk.next(call);
+        if (more) {
+            load_queries();
+        }
+        while (more) {
             float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < walk.count; ++j, ++n) {
+            const int count = walk.count;
+            for (int j = 0; j < count; ++j, ++n) {
                 if (!tile_wait(&s_full[half], n & 1, &abort_flag)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after_sync();
                 const GroupMeta* groups = meta[n % kMetaSlots];
-                // t of 16 tokens; those that the row does not see are -infinity.
-                const auto exponents = [&](const uint32_t* s, const GroupMeta& g, float add, float (&t)[16]) {
-                    const float k = g.k * up;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        t[i] = __fmaf_rn(__uint_as_float(s[i]), k, add);
-                    }
-                    if (g.key0 >> half & 1) {
-                        const int key0 = g.key0 & ~15;
+                const bool plain = (by_element[n % kMetaSlots] >> half & 1) == 0;
+                if (!plain) {
+                    // Scores become exponents in place, those that the row does not see -infinity.
+#pragma unroll 1
+                    for (int g = 0; g < kTileGroups; ++g) {
+                        const GroupMeta of = groups[g];
+                        uint32_t s[16];
+                        tile_tmem_ld_16(s_addr + static_cast<uint32_t>(g * 16), s);
+                        tmem_ld_wait();
+                        const bool masked = (of.key0 >> half & 1) != 0;
+                        const int key0 = of.key0 & ~15;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int key = key0 + i;
-                            t[i] = key <= pos && (key >= low || key < a.sinks) ? t[i] : -INFINITY;
+                            const float t = __fmaf_rn(__uint_as_float(s[i]), of.k * factor, of.v_log2);
+                            s[i] = __float_as_uint(!masked || (key <= pos && (key >= low || key < a.sinks)) ? t : -INFINITY);
                         }
+                        tile_tmem_st_16(s_addr + static_cast<uint32_t>(g * 16), s);
                     }
-                };
+                    tile_tmem_st_wait();
+                }
+                uint32_t s[kTileKeys];
+#pragma unroll
+                for (int c = 0; c < kTileKeys / 32; ++c) {
+                    tmem_ld_32x32(s_addr + static_cast<uint32_t>(c * 32), *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                }
+                tmem_ld_wait();
+                const float scale = plain ? factor : 1.0f;
                 float top = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t s[32];
-                    tmem_ld_32x32(s_addr + static_cast<uint32_t>(c * 32), s);
-                    tmem_ld_wait();
+                for (int g = 0; g < kTileGroups; ++g) {
+                    float high = __uint_as_float(s[16 * g]);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const GroupMeta g = groups[2 * c + h];
-                        float t[16];
-                        exponents(s + 16 * h, g, g.v_log2, t);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            top = fmaxf(top, t[i]);
-                        }
+                    for (int i = 1; i < 16; ++i) {
+                        high = fmaxf(high, __uint_as_float(s[16 * g + i]));
                     }
+                    const float k = plain ? groups[g].k : 1.0f, add = plain ? groups[g].v_log2 : 0.0f;
+                    top = fmaxf(top, __fmaf_rn(high, k * scale, add));
                 }
                 const bool grown = top > m + 8.0f || (m == -INFINITY && top > m);
-                const float next = grown ? top : m;
-                const float alpha = grown ? exp2_fast(m - next) : 1.0f;
-                if (j > 0 && __any_sync(0xFFFFFFFFu, grown)) {
-                    // The sums so far are complete: the next block's products wait for this one's weights.
-                    if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16];
-                        tile_tmem_ld_16(o_addr + static_cast<uint32_t>(c * 16), o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                if (__any_sync(0xFFFFFFFFu, grown)) {
+                    const float next = grown ? top : m;
+                    const float alpha = grown ? exp2_fast(m - next) : 1.0f;
+                    m = next;
+                    l *= alpha;
+                    if (j > 0) {
+                        // The sums so far are complete: the next block's products wait for this one's weights.
+                        if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+                            ok = false;
+                            break;
                         }
-                        tile_tmem_st_16(o_addr + static_cast<uint32_t>(c * 16), o);
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tile_tmem_ld_16(o_addr + static_cast<uint32_t>(c * 16), o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            }
+                            tile_tmem_st_16(o_addr + static_cast<uint32_t>(c * 16), o);
+                        }
                     }
                 }
-                m = next;
-                l *= alpha;
                 const float safe = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t s[32];
-                    tmem_ld_32x32(s_addr + static_cast<uint32_t>(c * 32), s);
-                    tmem_ld_wait();
+                for (int c = 0; c < kTileGroups / 2; ++c) {
                     uint32_t p[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const GroupMeta g = groups[2 * c + h];
-                        float t[16], sum = 0.0f;
-                        exponents(s + 16 * h, g, g.v_log2 - safe, t);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            t[i] = exp2_fast(t[i]);
-                            sum += t[i];
-                        }
-                        l += sum == 0.0f ? 0.0f : sum * g.v_inv;   // (0 times what a masked block has for a scale)
+                        const int g = 2 * c + h;
+                        const float k = (plain ? groups[g].k : 1.0f) * scale, add = (plain ? groups[g].v_log2 : 0.0f) - safe;
+                        const uint64_t kk = pair_of(k, k), aa = pair_of(add, add);
+                        uint64_t sum = 0;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            p[8 * h + i] = pack2<__half>(t[2 * i], t[2 * i + 1]);
+                            float x, y;
+                            unpair(pair_fma(pair_of(__uint_as_float(s[16 * g + 2 * i]), __uint_as_float(s[16 * g + 2 * i + 1])), kk, aa), x, y);
+                            x = exp2_fast(x);
+                            y = exp2_fast(y);
+                            sum = pair_add(sum, pair_of(x, y));
+                            p[8 * h + i] = pack2<__half>(x, y);
                         }
+                        float x, y;
+                        unpair(sum, x, y);
+                        x += y;
+                        l += x == 0.0f ? 0.0f : x * groups[g].v_inv;   // (not 0 times what a block that is masked has for a scale)
                     }
                     tile_tmem_st_16(s_addr + static_cast<uint32_t>(c * 16), p);
                 }
@@ -475,46 +549,55 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 tc_fence_before_sync();
                 mbar_arrive(&p_full[half]);
             }
-            if (!ok || !tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+            if (!ok) {
+                break;
+            }
+            // The scores of this part are all there, so its queries may go: the next one's first products come behind this one's last.
+            const bool whole = walk.begins && walk.ends, had = there;
+            const int which = walk.begins ? 1 : 0, kind = walk.begins ? 1 : walk.ends ? 3 : 2;
+            const RowsPiece about{kind, walk.info.seq, walk.head, walk.info.tile};
+            T* const dst = static_cast<T*>(a.out) + place;
+            more = walk.next(call);
+            if (more) {
+                load_queries();
+            }
+            if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
                 ok = false;
                 break;
             }
             tc_fence_after_sync();
-            const bool whole = walk.begins && walk.ends;
-            const int which = walk.begins ? 1 : 0;
             const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
             float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kRows * (D + 2));
-            T* dst = static_cast<T*>(a.out) + (there ? (walk.info.row0 + token) * a.out_stride_row + head * a.out_stride_head : 0);
 #pragma unroll 2
-            for (int c = 0; c < D / 16; ++c) {
-                uint32_t o[16];
-                tile_tmem_ld_16(o_addr + static_cast<uint32_t>(c * 16), o);
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_addr + static_cast<uint32_t>(c * 32), o);
                 tmem_ld_wait();
-                if (there && whole) {
+                if (had && whole) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < 4; ++h) {
                         float f[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             f[i] = __uint_as_float(o[8 * h + i]) * inv;
                         }
-                        store8(dst + c * 16 + h * 8, call.wide != 0, f);
+                        store8(dst + c * 32 + h * 8, call.wide != 0, f);
                     }
-                } else if (there) {
+                } else if (had) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        reinterpret_cast<uint4*>(piece)[(c * 4 + i) * kRows + half * 128 + row] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    for (int i = 0; i < 8; ++i) {
+                        reinterpret_cast<uint4*>(piece)[(c * 8 + i) * kRows + half * 128 + row] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
             }
             if (!whole) {
-                if (there) {
+                if (had) {
                     piece[kRows * D + half * 128 + row] = m;
                     piece[kRows * (D + 1) + half * 128 + row] = l;
                 }
-                kinds[which] = walk.begins ? 1 : walk.ends ? 3 : 2;
+                kinds[which] = kind;
                 if (threadIdx.x == 0) {
-                    call.pieces[2 * blockIdx.x + which] = RowsPiece{kinds[which], walk.info.seq, walk.head, walk.info.tile};
+                    call.pieces[2 * blockIdx.x + which] = about;
                 }
             }
             tc_fence_before_sync();
@@ -528,101 +611,159 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         __syncwarp();
     } else if (warp < Shared::kSoftmaxWarps + 4) {
         // ---------------- codes into f16 tiles ----------------
+        fewer_registers<Shared::kCodesRegisters>();
         const int t = threadIdx.x - 32 * Shared::kSoftmaxWarps;
         const int page_tokens = static_cast<int>(a.cache.page_tokens);
         const int64_t head_bytes = static_cast<int64_t>(page_tokens) * D;
-        // The block that is being loaded: where each of its groups lies (lanes 0..7), or -1.
+        // Where a block lies is found in steps, each a block after the one before, as each waits for memory: its
+        // groups' pages; then their places and scales; then the codes.  Lanes 0..7 have a group each.
+        struct Pages {
+            int raw, key0, seq, head;   // key0 -1: no such group
+            int flags;                  // as in GroupMeta
+        };
+        struct Block {
+            int64_t where;   // of the group's codes; -1: none
+            GroupMeta meta;  // v_log2: the scale still, unless it is -infinity
+        };
         TileRange range{};
         int j = 0;
         bool more = walk.next(call);
-        int64_t where = -1;
-        GroupMeta mine{};
-        const auto locate = [&] {   // of block j of the walk's part
+        int ahead = 0;   // blocks found whose codes are not stored yet
+        const auto find_pages = [&](Pages& p) {   // of block j of the walk's part
+            p.key0 = -1;
+            if (!more) {
+                return;
+            }
+            ++ahead;
             if (j == 0) {
                 range = tile_range<kRows>(call, walk.info.tile, walk.info.n, walk.info.len);
             }
-            where = -1;
-            mine = GroupMeta{0.0f, -INFINITY, 0.0f, 0};
             const int idx = (walk.off + j) * kTileGroups + lane;
             if (lane < kTileGroups && idx < range.groups) {
-                const int key0 = (idx < range.sink_groups ? idx : idx - range.sink_groups + range.first_group) * 16;
-                const int page = page_at(a.cache, walk.info.seq, key0 / page_tokens, call.error_word);
-                if (page >= 0) {
-                    const int64_t at = page * a.cache.scale_page_stride + walk.head;
-                    const float vs = a.cache.v_scale[at];
-                    where = page * a.cache.page_stride + walk.head * head_bytes + key0 % page_tokens * D;
-                    mine.k = a.cache.k_scale[at];
-                    mine.v_log2 = vs < kLeastCacheScale ? kLeastCacheScale : vs;
-                    mine.key0 = key0;
+                p.key0 = (idx < range.sink_groups ? idx : idx - range.sink_groups + range.first_group) * 16;
+                p.seq = walk.info.seq;
+                p.head = walk.head;
+                p.raw = a.cache.page_table[p.seq * a.cache.table_stride + p.key0 / page_tokens];
+                p.flags = 0;
 #pragma unroll
-                    for (int h = 0; h < kHalves; ++h) {
-                        const bool all_seen = key0 + 15 < walk.info.len && key0 + 15 <= range.least_pos[h] &&
-                                              (a.window == 0 || key0 > range.most_pos[h] - a.window || key0 + 15 < a.sinks);
-                        mine.key0 |= all_seen ? 0 : 1 << h;
-                    }
+                for (int h = 0; h < kHalves; ++h) {
+                    const bool all_seen = p.key0 + 15 < walk.info.len && p.key0 + 15 <= range.least_pos[h] &&
+                                          (a.window == 0 || p.key0 > range.most_pos[h] - a.window || p.key0 + 15 < a.sinks);
+                    p.flags |= all_seen ? 0 : 1 << h;
+                }
+            }
+            if (++j == walk.count) {
+                j = 0;
+                more = walk.next(call);
+            }
+        };
+        const auto find_block = [&](const Pages& p, Block& b) {
+            b.where = -1;
+            b.meta = GroupMeta{0.0f, -INFINITY, 0.0f, 0};
+            if (p.key0 >= 0) {
+                if (p.raw < 0 || p.raw >= a.cache.pages) {
+                    atomicCAS(call.error_word, 0, kErrBadPage);
+                } else {
+                    const int64_t at = p.raw * a.cache.scale_page_stride + p.head;
+                    b.where = p.raw * a.cache.page_stride + p.head * head_bytes + p.key0 % page_tokens * D;
+                    b.meta = GroupMeta{a.cache.k_scale[at], a.cache.v_scale[at], 0.0f, p.key0 | p.flags};
                 }
             }
         };
-        const auto load = [&](const void* codes, uint4 (&raw)[kPerThread]) {
+        // A thread copies the 16-byte segments that it converts itself: what it waits for is its own copies.
+        uint8_t* const my_codes = codes_ring + t * 16;
+        const auto load = [&](const void* codes, int64_t where, int part, int slot) {
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                const int idx = t + i * 128, key = idx / kPerThread, segment = idx % kPerThread;
+                const int idx = t + (part * kPerThread + i) * 128, key = idx / (D / 16), segment = idx % (D / 16);
                 const int64_t base = __shfl_sync(0xFFFFFFFFu, where, key / 16);
-                raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (base >= 0) {
-                    raw[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(codes) + base + (key & 15) * D + segment * 16);
-                }
+                cp_async_16(my_codes + slot * Shared::kUnitBytes + i * 2048,
+                            static_cast<const uint8_t*>(codes) + (base < 0 ? 0 : base + (key & 15) * D + segment * 16), base < 0 ? 0u : 16u);
             }
         };
-        const auto store = [&](uint8_t* tile, const uint4 (&raw)[kPerThread]) {
+        const auto store = [&](uint8_t* tile, int part, int slot) {
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                const int idx = t + i * 128;
-                store_codes<D>(tile, idx / kPerThread, idx % kPerThread, raw[i]);
+                const int idx = t + (part * kPerThread + i) * 128;
+                store_codes<D>(tile, idx / (D / 16), idx % (D / 16), *reinterpret_cast<const uint4*>(my_codes + slot * Shared::kUnitBytes + i * 2048));
             }
         };
-        uint4 raw_k[kPerThread], raw_v[kPerThread];
-        if (more) {
-            locate();
-            load(a.cache.k, raw_k);
+        Pages pages;
+        Block now, next;
+        find_pages(pages);
+        find_block(pages, now);
+        find_pages(pages);
+        find_block(pages, next);
+        find_pages(pages);
+        if (ahead > 0) {
+            load(a.cache.k, now.where, 0, 0);
+            cp_async_commit();
+            load(Shared::kUnits == 1 ? a.cache.v : a.cache.k, now.where, Shared::kUnits - 1, 1);
+            cp_async_commit();
         }
         bool ok = true;
-        for (uint32_t n = 0; more; ++n) {
-            load(a.cache.v, raw_v);
-            const GroupMeta now = mine;
+        for (uint32_t n = 0; ahead > 0; ++n) {
             const uint32_t slot = n % kStages, round = n / kStages & 1;
             if (!tile_wait(&k_empty[slot], round ^ 1, &abort_flag)) {
                 ok = false;
                 break;
             }
-            if (t < kTileGroups) {
-                const float vs = now.v_log2;
-                meta[n % kMetaSlots][t] = now.v_log2 == -INFINITY ? now : GroupMeta{now.k, log2f(vs), __fdiv_rn(1.0f, vs), now.key0};
+            if (t < 32) {
+                GroupMeta of = now.meta;
+                if (of.v_log2 != -INFINITY) {
+                    const float vs = of.v_log2 < kLeastCacheScale ? kLeastCacheScale : of.v_log2;
+                    of.v_log2 = log2f(vs);
+                    of.v_inv = __fdiv_rn(1.0f, vs);
+                }
+                // A scale below zero turns the order of its scores round.
+                const int odd = (of.key0 & 15) | (of.k * call.factor < 0.0f ? 15 : 0);
+                const int any = __reduce_or_sync(0xFFFFFFFFu, lane < kTileGroups ? odd : 0);
+                if (lane < kTileGroups) {
+                    meta[n % kMetaSlots][lane] = of;
+                }
+                if (lane == 0) {
+                    by_element[n % kMetaSlots] = any;
+                }
             }
-            store(k_tile + slot * Shared::kTileBytes, raw_k);
+#pragma unroll
+            for (int part = 0; part < Shared::kUnits; ++part) {
+                cp_async_wait_group<1>();
+                store(k_tile + slot * Shared::kTileBytes, part, part);
+                if (Shared::kUnits == 2) {
+                    load(a.cache.v, now.where, part, part);
+                } else if (ahead > 1) {
+                    load(a.cache.k, next.where, 0, 0);
+                }
+                cp_async_commit();
+            }
             fence_proxy_async_smem();
             mbar_arrive(&k_full[slot]);
-            if (++j == walk.count) {
-                j = 0;
-                more = walk.next(call);
-            }
-            if (more) {
-                locate();
-                load(a.cache.k, raw_k);
-            }
             if (!tile_wait(&v_empty[slot], round ^ 1, &abort_flag)) {
                 ok = false;
                 break;
             }
-            store(v_tile + slot * Shared::kTileBytes, raw_v);
+#pragma unroll
+            for (int part = 0; part < Shared::kUnits; ++part) {
+                cp_async_wait_group<1>();
+                store(v_tile + slot * Shared::kTileBytes, part, Shared::kUnits == 1 ? 1 : part);
+                if (ahead > 1) {
+                    load(Shared::kUnits == 1 ? a.cache.v : a.cache.k, next.where, part, Shared::kUnits == 1 ? 1 : part);
+                }
+                cp_async_commit();
+            }
             fence_proxy_async_smem();
             mbar_arrive(&v_full[slot]);
+            now = next;
+            find_block(pages, next);
+            --ahead;
+            find_pages(pages);
         }
+        cp_async_wait_group<0>();
         if (!ok && lane == 0) {
             atomicCAS(call.error_word, 0, kErrDequantWait);
         }
         __syncwarp();
-    } else {
+    } else if (fewer_registers<Shared::kIssuerRegisters>(); warp == Shared::kSoftmaxWarps + 4) {
         // ---------------- MMA issuer ----------------
         const uint32_t base = warp_uniform(tmem);
         constexpr uint32_t kIdescS = umma_idesc(1, 0, 0, 128, kTileKeys);
@@ -776,6 +917,14 @@ cudaError_t launch_tile_typed(const TileCall& call, int blocks, cudaStream_t str
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return e;
+    }
+    // Groups trade registers within what the block is launched with; with less, one would wait for good.
+    static const int registers = [&] {
+        cudaFuncAttributes attributes;
+        return cudaFuncGetAttributes(&attributes, kernel) == cudaSuccess ? attributes.numRegs : 0;
+    }();
+    if (registers != Shared::kRegisters) {
+        return cudaErrorInvalidDeviceFunction;
     }
     const unsigned grid = static_cast<unsigned>(blocks);
     e = launch_overlapping(attention_i8_plan_kernel<Shared::kRows>, dim3(1), dim3(1024), 0, stream, 1, call);
