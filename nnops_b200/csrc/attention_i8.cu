@@ -89,6 +89,8 @@ int run_tile(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.group = static_cast<int>(a.q_heads / a.cache.heads);
     call.factor = a.scale * 1.4426950408889634f;
     call.wide = wide(a.q, a.q_stride_row, a.q_stride_head) && wide(a.out, a.out_stride_row, a.out_stride_head) ? 1 : 0;
+    call.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.out_stride_row % 16 == 0 && a.out_stride_head % 16 == 0 ? 1 : 0;
+    call.page_shift = a.cache.page_tokens == 16 ? 4 : a.cache.page_tokens == 32 ? 5 : a.cache.page_tokens == 64 ? 6 : 7;
     uint8_t* const base = static_cast<uint8_t*>(a.workspace);
     call.line = reinterpret_cast<int64_t*>(base);
     call.tiles = reinterpret_cast<TileInfo*>(base + p.tiles);

@@ -42,6 +42,8 @@ struct TileCall {
     int group;
     float factor;
     int wide;             // q's and out's rows and heads are 16-byte aligned
+    int wide_out;         // out's 32-byte aligned
+    int page_shift;       // log2 of the tokens of a page
     int64_t* line;        // [0] tiles, [1] length of all tiles, of one head
     TileInfo* tiles;
     int32_t* first_tile;  // [seqs + 1]: tiles before each sequence's
@@ -221,6 +223,10 @@ struct GroupMeta {
     int key0;   // first token; its low bits: 1 (2) if the first (second) 128 rows do not see all of its tokens
 };
 
+// What the scout says of a block besides: bits 0, 1: half h has more to do than t = s k + v_log2.
+constexpr int kBlockLast = 4;   // of this block of the grid
+constexpr int kBlockNone = 8;   // there is no block at all
+
 template <int D>
 struct TileShared {
     static constexpr int kHalves = D <= 128 ? 2 : 1;
@@ -233,12 +239,12 @@ struct TileShared {
     static constexpr int kUnitBytes = kTileKeys * D / kUnits;
     static constexpr int kBytes = 1024 + (kHalves + 2 * kStages) * kTileBytes + 2 * kUnitBytes;
     static constexpr int kSoftmaxWarps = 4 * kHalves;
-    static constexpr int kThreads = 32 * (kSoftmaxWarps + 8);   // and four for codes, and the MMA issuer's group
+    static constexpr int kThreads = 32 * (kSoftmaxWarps + 8);   // and four for codes, the MMA issuer, the scout (and two to fill its group)
     // Registers of a thread: at launch, and of the three kinds of warps afterwards.
     static constexpr int kRegisters = kHalves == 2 ? 128 : 168;
     static constexpr int kSoftmaxRegisters = kHalves == 2 ? 184 : 232;
-    static constexpr int kCodesRegisters = kHalves == 2 ? 96 : 160;
-    static constexpr int kIssuerRegisters = kHalves == 2 ? 48 : 96;
+    static constexpr int kCodesRegisters = kHalves == 2 ? 88 : 160;
+    static constexpr int kIssuerRegisters = kHalves == 2 ? 56 : 96;
     static_assert(kHalves * kSoftmaxRegisters + kCodesRegisters + kIssuerRegisters <= (kHalves + 2) * kRegisters, "a group would wait for registers");
     static constexpr int kOutColumn = 256;      // of the sums in tensor memory; S and P are below
     static_assert(kBytes <= 226 * 1024, "shared memory");
@@ -303,6 +309,12 @@ __device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c)
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
 {
     uint64_t r;
@@ -310,10 +322,26 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
     return r;
 }
 
-// Every lane polls: the data behind the barrier is then every lane's.
+// Every lane polls: the data behind the barrier is then every lane's.  Without a hint how long to sleep, which costs a
+// hundred cycles on a barrier that is all but ready; within the limit that mbar_wait has.
 __device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
 {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag));
+    bool done = mbar_try_wait(bar, parity);
+    if (!__all_sync(0xFFFFFFFFu, done)) {
+        const long long t0 = clock64();
+        bool give_up = false;
+        for (uint32_t spins = 1; !done && !give_up; ++spins) {
+            done = mbar_try_wait(bar, parity);
+            if ((spins & 63u) == 0) {
+                if (*abort_flag == 0 && clock64() - t0 > kWaitLimitCycles) {
+                    *abort_flag = 1;
+                }
+                give_up = *abort_flag != 0;
+            }
+        }
+        return __all_sync(0xFFFFFFFFu, done);
+    }
+    return true;
 }
 
 // 16 codes as f16 into the swizzled tile: row `key`, dims [16 segment, + 16).
@@ -340,8 +368,10 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
     constexpr int kPerThread = D / 16 / Shared::kUnits;   // 16-code segments of a unit that a converting thread has
     extern __shared__ uint8_t raw_shared[];
     __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
-    __shared__ GroupMeta meta[kMetaSlots][kTileGroups];
-    __shared__ int by_element[kMetaSlots];   // bit h: some group is not just t = s k + v_log2 to half h
+    __shared__ __align__(8) uint64_t meta_full[kMetaSlots], meta_empty[kMetaSlots];
+    __shared__ GroupMeta meta[kMetaSlots][kTileGroups], identity[kTileGroups];
+    __shared__ int64_t where[kMetaSlots][kTileGroups];   // of a group's codes; -1: none
+    __shared__ int state[kMetaSlots];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
 
@@ -362,6 +392,13 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < kMetaSlots; ++i) {
+            mbar_init(&meta_full[i], 1);
+            mbar_init(&meta_empty[i], Shared::kSoftmaxWarps);
+        }
+        for (int i = 0; i < kTileGroups; ++i) {
+            identity[i] = GroupMeta{1.0f, 0.0f, 0.0f, 0};
         }
         mbar_init_fence();
     }
@@ -385,7 +422,6 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         const int half = warp / 4, row = threadIdx.x & 127;
         const uint32_t s_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(half * 128);
         const uint32_t o_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(Shared::kOutColumn + half * 128);
-        uint8_t* const q_row = q_tile + half * Shared::kTileBytes + row * 128;
         uint32_t n = 0;   // blocks
         int kinds[2] = {0, 0};
         // The row of the part that is next: its place in out, its range of tokens, its factor.
@@ -394,58 +430,138 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         int64_t low = 0, place = 0;
         float factor = 0.0f;
         const auto load_queries = [&] {
-            const int global = walk.info.tile * kRows + half * 128 + row;
-            there = global < walk.info.n * call.group;
-            const int token = global / call.group, head = walk.head * call.group + global % call.group;
-            pos = a.causal != 0 ? walk.info.len - walk.info.n + token : 0x7FFFFFFF;
+            const int first = walk.info.tile * kRows + half * 128 + (warp & 3) * 32, all = walk.info.n * call.group;
+            const auto source = [&](int r, int64_t stride_row, int64_t stride_head) {   // of this warp's r-th row
+                const int token = (first + r) / call.group;
+                return (walk.info.row0 + token) * stride_row + (walk.head * call.group + (first + r) - token * call.group) * stride_head;
+            };
+            there = first + lane < all;
+            place = there ? source(lane, a.out_stride_row, a.out_stride_head) : 0;
+            pos = a.causal != 0 ? walk.info.len - walk.info.n + (first + lane) / call.group : 0x7FFFFFFF;
             pos = pos < walk.info.len ? pos : walk.info.len - 1;
             low = a.window > 0 && there ? static_cast<int64_t>(pos) - a.window + 1 : INT64_MIN;
-            place = there ? (walk.info.row0 + token) * a.out_stride_row + head * a.out_stride_head : 0;
-            // Scaled by a power of two into f16.
-            const T* src = static_cast<const T*>(a.q) + (there ? (walk.info.row0 + token) * a.q_stride_row + head * a.q_stride_head : 0);
-            float down = 1.0f;
             factor = call.factor;
-            if constexpr (!std::is_same_v<T, __half>) {
-                uint32_t top = 0;
-#pragma unroll 8
-                for (int c = 0; c < D / 8; ++c) {
-                    float f[8] = {};
-                    if (there) {
-                        load8(src + c * 8, call.wide != 0, f);
-                    }
+            // Four lanes to a row, eight rows at a time: 64 bytes of each next to each other.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + lane / 4;
+                const bool row_there = first + r < all;
+                const T* src = static_cast<const T*>(a.q) + (row_there ? source(r, a.q_stride_row, a.q_stride_head) : 0) + lane % 4 * 8;
+                float f[D / 32][8];
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        top = max(top, magnitude_bits(f[e]));
+                        f[c][e] = 0.0f;
+                    }
+                    if (row_there) {
+                        load8(src + c * 32, call.wide != 0, f[c]);
                     }
                 }
-                const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
-                down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                factor *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            }
-#pragma unroll 8
-            for (int c = 0; c < D / 8; ++c) {
-                float f[8] = {};
-                if (there) {
-                    load8(src + c * 8, call.wide != 0, f);
-                }
-                if constexpr (!std::is_same_v<T, __half>) {
+                if constexpr (!std::is_same_v<T, __half>) {   // scaled by a power of two into f16
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[e] *= down;
+                    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            top = max(top, magnitude_bits(f[c][e]));
+                        }
+                    }
+                    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                    const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+                    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    const float up = call.factor * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                    const float mine = __shfl_sync(0xFFFFFFFFu, up, lane % 8 * 4);
+                    factor = lane / 8 == i ? mine : factor;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            f[c][k] *= down;
+                        }
                     }
                 }
-                *reinterpret_cast<uint4*>(q_row + c / 8 * Shared::kBlockBytes + (((c & 7) ^ (row & 7)) << 4)) =
-                    make_uint4(pack2<__half>(f[0], f[1]), pack2<__half>(f[2], f[3]), pack2<__half>(f[4], f[5]), pack2<__half>(f[6], f[7]));
+                uint8_t* const to = q_tile + half * Shared::kTileBytes + ((warp & 3) * 32 + r) * 128;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    const int chunk = c * 4 + lane % 4;
+                    *reinterpret_cast<uint4*>(to + chunk / 8 * Shared::kBlockBytes + (((chunk & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(pack2<__half>(f[c][0], f[c][1]), pack2<__half>(f[c][2], f[c][3]), pack2<__half>(f[c][4], f[c][5]), pack2<__half>(f[c][6], f[c][7]));
+                }
             }
             fence_proxy_async_smem();
             mbar_arrive(&q_full[half]);
         };
+        // The part whose sums are next: where they go.
+        bool had = false, whole = false, pending = false;
+        int which = 0;
+        T* dst = nullptr;
+        RowsPiece about{};
+        float m = 0.0f, l = 0.0f;
         bool ok = true, more = walk.next(call);
-        if (more) {
-            load_queries();
-        }
-        while (more) {
-            float m = -INFINITY, l = 0.0f;
+        while (more || pending) {
+            // The scores of the part before are all there, so its queries may go, and the next one's first products come right
+            // behind its last.
+            if (more) {
+                load_queries();
+            }
+            if (pending) {
+                if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+                float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kRows * (D + 2));
+#pragma unroll 2
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld_32x32(o_addr + static_cast<uint32_t>(c * 32), o);
+                    tmem_ld_wait();
+                    if (had && whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+                        }
+                        const auto two = [&](int i) { return pack2<T>(__uint_as_float(o[i]), __uint_as_float(o[i + 1])); };
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (call.wide_out != 0) {   // whole sectors
+                                st_global_32(dst + c * 32 + h * 16, two(16 * h), two(16 * h + 2), two(16 * h + 4), two(16 * h + 6), two(16 * h + 8), two(16 * h + 10),
+                                             two(16 * h + 12), two(16 * h + 14));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    dst[c * 32 + h * 16 + i] = from_float<T>(__uint_as_float(o[16 * h + i]));
+                                }
+                            }
+                        }
+                    } else if (had) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            reinterpret_cast<uint4*>(piece)[(c * 8 + i) * kRows + half * 128 + row] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                    }
+                }
+                if (!whole) {
+                    if (had) {
+                        piece[kRows * D + half * 128 + row] = m;
+                        piece[kRows * (D + 1) + half * 128 + row] = l;
+                    }
+                    kinds[which] = about.kind;
+                    if (threadIdx.x == 0) {
+                        call.pieces[2 * blockIdx.x + which] = about;
+                    }
+                }
+                tc_fence_before_sync();
+                pending = false;
+            }
+            if (!more) {
+                break;
+            }
+            m = -INFINITY;
+            l = 0.0f;
             const int count = walk.count;
             for (int j = 0; j < count; ++j, ++n) {
                 if (!tile_wait(&s_full[half], n & 1, &abort_flag)) {
@@ -453,8 +569,10 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                     break;
                 }
                 tc_fence_after_sync();
-                const GroupMeta* groups = meta[n % kMetaSlots];
-                const bool plain = (by_element[n % kMetaSlots] >> half & 1) == 0;
+                (void)tile_wait(&meta_full[n % kMetaSlots], n / kMetaSlots & 1, &abort_flag);   // long since: the products waited for it
+                const GroupMeta* const groups = meta[n % kMetaSlots];
+                const bool plain = (state[n % kMetaSlots] >> half & 1) == 0;
+                const GroupMeta* const linear = plain ? groups : identity;
                 if (!plain) {
                     // Scores become exponents in place, those that the row does not see -infinity.
 #pragma unroll 1
@@ -485,13 +603,14 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 float top = -INFINITY;
 #pragma unroll
                 for (int g = 0; g < kTileGroups; ++g) {
-                    float high = __uint_as_float(s[16 * g]);
+                    float high = __uint_as_float(s[16 * g]), other = __uint_as_float(s[16 * g + 1]);
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) {
-                        high = fmaxf(high, __uint_as_float(s[16 * g + i]));
+                    for (int i = 2; i < 14; i += 4) {
+                        high = max3(high, __uint_as_float(s[16 * g + i]), __uint_as_float(s[16 * g + i + 1]));
+                        other = max3(other, __uint_as_float(s[16 * g + i + 2]), __uint_as_float(s[16 * g + i + 3]));
                     }
-                    const float k = plain ? groups[g].k : 1.0f, add = plain ? groups[g].v_log2 : 0.0f;
-                    top = fmaxf(top, __fmaf_rn(high, k * scale, add));
+                    high = max3(high, __uint_as_float(s[16 * g + 14]), __uint_as_float(s[16 * g + 15]));
+                    top = fmaxf(top, __fmaf_rn(fmaxf(high, other), linear[g].k * scale, linear[g].v_log2));
                 }
                 const bool grown = top > m + 8.0f || (m == -INFINITY && top > m);
                 if (__any_sync(0xFFFFFFFFu, grown)) {
@@ -526,7 +645,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int g = 2 * c + h;
-                        const float k = (plain ? groups[g].k : 1.0f) * scale, add = (plain ? groups[g].v_log2 : 0.0f) - safe;
+                        const float k = linear[g].k * scale, add = linear[g].v_log2 - safe;
                         const uint64_t kk = pair_of(k, k), aa = pair_of(add, add);
                         uint64_t sum = 0;
 #pragma unroll
@@ -548,59 +667,21 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 tile_tmem_st_wait();
                 tc_fence_before_sync();
                 mbar_arrive(&p_full[half]);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&meta_empty[n % kMetaSlots]);
+                }
             }
             if (!ok) {
                 break;
             }
-            // The scores of this part are all there, so its queries may go: the next one's first products come behind this one's last.
-            const bool whole = walk.begins && walk.ends, had = there;
-            const int which = walk.begins ? 1 : 0, kind = walk.begins ? 1 : walk.ends ? 3 : 2;
-            const RowsPiece about{kind, walk.info.seq, walk.head, walk.info.tile};
-            T* const dst = static_cast<T*>(a.out) + place;
+            whole = walk.begins && walk.ends;
+            had = there;
+            which = walk.begins ? 1 : 0;
+            about = RowsPiece{walk.begins ? 1 : walk.ends ? 3 : 2, walk.info.seq, walk.head, walk.info.tile};
+            dst = static_cast<T*>(a.out) + place;
+            pending = true;
             more = walk.next(call);
-            if (more) {
-                load_queries();
-            }
-            if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after_sync();
-            const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-            float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kRows * (D + 2));
-#pragma unroll 2
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld_32x32(o_addr + static_cast<uint32_t>(c * 32), o);
-                tmem_ld_wait();
-                if (had && whole) {
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        float f[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            f[i] = __uint_as_float(o[8 * h + i]) * inv;
-                        }
-                        store8(dst + c * 32 + h * 8, call.wide != 0, f);
-                    }
-                } else if (had) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        reinterpret_cast<uint4*>(piece)[(c * 8 + i) * kRows + half * 128 + row] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    }
-                }
-            }
-            if (!whole) {
-                if (had) {
-                    piece[kRows * D + half * 128 + row] = m;
-                    piece[kRows * (D + 1) + half * 128 + row] = l;
-                }
-                kinds[which] = kind;
-                if (threadIdx.x == 0) {
-                    call.pieces[2 * blockIdx.x + which] = about;
-                }
-            }
-            tc_fence_before_sync();
         }
         if (threadIdx.x < 2 && kinds[threadIdx.x] == 0) {
             call.pieces[2 * blockIdx.x + threadIdx.x].kind = 0;
@@ -613,150 +694,69 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         // ---------------- codes into f16 tiles ----------------
         fewer_registers<Shared::kCodesRegisters>();
         const int t = threadIdx.x - 32 * Shared::kSoftmaxWarps;
-        const int page_tokens = static_cast<int>(a.cache.page_tokens);
-        const int64_t head_bytes = static_cast<int64_t>(page_tokens) * D;
-        // Where a block lies is found in steps, each a block after the one before, as each waits for memory: its
-        // groups' pages; then their places and scales; then the codes.  Lanes 0..7 have a group each.
-        struct Pages {
-            int raw, key0, seq, head;   // key0 -1: no such group
-            int flags;                  // as in GroupMeta
-        };
-        struct Block {
-            int64_t where;   // of the group's codes; -1: none
-            GroupMeta meta;  // v_log2: the scale still, unless it is -infinity
-        };
-        TileRange range{};
-        int j = 0;
-        bool more = walk.next(call);
-        int ahead = 0;   // blocks found whose codes are not stored yet
-        const auto find_pages = [&](Pages& p) {   // of block j of the walk's part
-            p.key0 = -1;
-            if (!more) {
-                return;
-            }
-            ++ahead;
-            if (j == 0) {
-                range = tile_range<kRows>(call, walk.info.tile, walk.info.n, walk.info.len);
-            }
-            const int idx = (walk.off + j) * kTileGroups + lane;
-            if (lane < kTileGroups && idx < range.groups) {
-                p.key0 = (idx < range.sink_groups ? idx : idx - range.sink_groups + range.first_group) * 16;
-                p.seq = walk.info.seq;
-                p.head = walk.head;
-                p.raw = a.cache.page_table[p.seq * a.cache.table_stride + p.key0 / page_tokens];
-                p.flags = 0;
-#pragma unroll
-                for (int h = 0; h < kHalves; ++h) {
-                    const bool all_seen = p.key0 + 15 < walk.info.len && p.key0 + 15 <= range.least_pos[h] &&
-                                          (a.window == 0 || p.key0 > range.most_pos[h] - a.window || p.key0 + 15 < a.sinks);
-                    p.flags |= all_seen ? 0 : 1 << h;
-                }
-            }
-            if (++j == walk.count) {
-                j = 0;
-                more = walk.next(call);
-            }
-        };
-        const auto find_block = [&](const Pages& p, Block& b) {
-            b.where = -1;
-            b.meta = GroupMeta{0.0f, -INFINITY, 0.0f, 0};
-            if (p.key0 >= 0) {
-                if (p.raw < 0 || p.raw >= a.cache.pages) {
-                    atomicCAS(call.error_word, 0, kErrBadPage);
-                } else {
-                    const int64_t at = p.raw * a.cache.scale_page_stride + p.head;
-                    b.where = p.raw * a.cache.page_stride + p.head * head_bytes + p.key0 % page_tokens * D;
-                    b.meta = GroupMeta{a.cache.k_scale[at], a.cache.v_scale[at], 0.0f, p.key0 | p.flags};
-                }
-            }
-        };
         // A thread copies the 16-byte segments that it converts itself: what it waits for is its own copies.
         uint8_t* const my_codes = codes_ring + t * 16;
-        const auto load = [&](const void* codes, int64_t where, int part, int slot) {
+        const auto load = [&](const void* codes, uint32_t block, int part, int slot) {
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
                 const int idx = t + (part * kPerThread + i) * 128, key = idx / (D / 16), segment = idx % (D / 16);
-                const int64_t base = __shfl_sync(0xFFFFFFFFu, where, key / 16);
+                const int64_t base = where[block % kMetaSlots][key / 16];
                 cp_async_16(my_codes + slot * Shared::kUnitBytes + i * 2048,
-                            static_cast<const uint8_t*>(codes) + (base < 0 ? 0 : base + (key & 15) * D + segment * 16), base < 0 ? 0u : 16u);
+                            static_cast<const uint8_t*>(codes) + (base < 0 ? 0 : base + ((key & 15) * D + segment * 16)), base < 0 ? 0u : 16u);
             }
+            cp_async_commit();
         };
         const auto store = [&](uint8_t* tile, int part, int slot) {
+            cp_async_wait_group<1>();
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
                 const int idx = t + (part * kPerThread + i) * 128;
                 store_codes<D>(tile, idx / (D / 16), idx % (D / 16), *reinterpret_cast<const uint4*>(my_codes + slot * Shared::kUnitBytes + i * 2048));
             }
         };
-        Pages pages;
-        Block now, next;
-        find_pages(pages);
-        find_block(pages, now);
-        find_pages(pages);
-        find_block(pages, next);
-        find_pages(pages);
-        if (ahead > 0) {
-            load(a.cache.k, now.where, 0, 0);
-            cp_async_commit();
-            load(Shared::kUnits == 1 ? a.cache.v : a.cache.k, now.where, Shared::kUnits - 1, 1);
-            cp_async_commit();
+        bool ok = tile_wait(&meta_full[0], 0, &abort_flag);
+        bool more = ok && (state[0] & kBlockNone) == 0;
+        if (more) {
+            load(a.cache.k, 0, 0, 0);
+            load(Shared::kUnits == 1 ? a.cache.v : a.cache.k, 0, Shared::kUnits - 1, 1);
         }
-        bool ok = true;
-        for (uint32_t n = 0; ahead > 0; ++n) {
+        for (uint32_t n = 0; more; ++n) {
             const uint32_t slot = n % kStages, round = n / kStages & 1;
-            if (!tile_wait(&k_empty[slot], round ^ 1, &abort_flag)) {
-                ok = false;
+            const bool next = (state[n % kMetaSlots] & kBlockLast) == 0;
+            ok = tile_wait(&k_empty[slot], round ^ 1, &abort_flag) &&
+                 (!next || tile_wait(&meta_full[(n + 1) % kMetaSlots], (n + 1) / kMetaSlots & 1, &abort_flag));
+            if (!ok) {
                 break;
-            }
-            if (t < 32) {
-                GroupMeta of = now.meta;
-                if (of.v_log2 != -INFINITY) {
-                    const float vs = of.v_log2 < kLeastCacheScale ? kLeastCacheScale : of.v_log2;
-                    of.v_log2 = log2f(vs);
-                    of.v_inv = __fdiv_rn(1.0f, vs);
-                }
-                // A scale below zero turns the order of its scores round.
-                const int odd = (of.key0 & 15) | (of.k * call.factor < 0.0f ? 15 : 0);
-                const int any = __reduce_or_sync(0xFFFFFFFFu, lane < kTileGroups ? odd : 0);
-                if (lane < kTileGroups) {
-                    meta[n % kMetaSlots][lane] = of;
-                }
-                if (lane == 0) {
-                    by_element[n % kMetaSlots] = any;
-                }
             }
 #pragma unroll
             for (int part = 0; part < Shared::kUnits; ++part) {
-                cp_async_wait_group<1>();
                 store(k_tile + slot * Shared::kTileBytes, part, part);
                 if (Shared::kUnits == 2) {
-                    load(a.cache.v, now.where, part, part);
-                } else if (ahead > 1) {
-                    load(a.cache.k, next.where, 0, 0);
+                    load(a.cache.v, n, part, part);
+                } else if (next) {
+                    load(a.cache.k, n + 1, 0, 0);
+                } else {
+                    cp_async_commit();
                 }
-                cp_async_commit();
             }
             fence_proxy_async_smem();
             mbar_arrive(&k_full[slot]);
-            if (!tile_wait(&v_empty[slot], round ^ 1, &abort_flag)) {
-                ok = false;
+            ok = tile_wait(&v_empty[slot], round ^ 1, &abort_flag);
+            if (!ok) {
                 break;
             }
 #pragma unroll
             for (int part = 0; part < Shared::kUnits; ++part) {
-                cp_async_wait_group<1>();
                 store(v_tile + slot * Shared::kTileBytes, part, Shared::kUnits == 1 ? 1 : part);
-                if (ahead > 1) {
-                    load(Shared::kUnits == 1 ? a.cache.v : a.cache.k, next.where, part, Shared::kUnits == 1 ? 1 : part);
+                if (next) {
+                    load(Shared::kUnits == 1 ? a.cache.v : a.cache.k, n + 1, part, Shared::kUnits == 1 ? 1 : part);
+                } else {
+                    cp_async_commit();
                 }
-                cp_async_commit();
             }
             fence_proxy_async_smem();
             mbar_arrive(&v_full[slot]);
-            now = next;
-            find_block(pages, next);
-            --ahead;
-            find_pages(pages);
+            more = next;
         }
         cp_async_wait_group<0>();
         if (!ok && lane == 0) {
@@ -786,7 +786,9 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             __syncwarp();
         };
         uint32_t n = 0, units = 0;
-        while (walk.next(call)) {
+        // What steers the loops is made uniform in the compiler's eyes: the MMAs' operands then stay in uniform registers.
+        while (warp_uniform(walk.next(call) ? 1 : 0) != 0) {
+            const int count = warp_uniform(walk.count);
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 mbar_wait_converged<kErrMmaWait>(&q_full[h], units & 1, &abort_flag, failed);
@@ -801,8 +803,8 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 umma_commit_unless(&k_empty[n % kStages], failed);
             }
             __syncwarp();
-            for (int j = 0; j < walk.count; ++j, ++n) {
-                const bool next = j + 1 < walk.count;
+            for (int j = 0; j < count; ++j, ++n) {
+                const bool next = j + 1 < count;
                 const uint32_t slot = n % kStages, next_slot = (n + 1) % kStages;
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) {
@@ -843,6 +845,68 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 atomicCAS(call.error_word, 0, static_cast<int32_t>(code));
             }
             umma_settle_after_failure();
+        }
+        __syncwarp();
+    } else if (warp == Shared::kSoftmaxWarps + 5) {
+        // ---------------- scout: where the blocks' codes lie, and their scales ----------------
+        const int tokens = static_cast<int>(a.cache.page_tokens);
+        bool ok = true, more = walk.next(call);
+        if (!more && lane == 0) {
+            state[0] = kBlockNone;
+            mbar_arrive(&meta_full[0]);
+        }
+        uint32_t n = 0;
+        while (ok && more) {
+            const TileRange range = tile_range<kRows>(call, walk.info.tile, walk.info.n, walk.info.len);
+            const TileInfo info = walk.info;
+            const int head = walk.head, off = walk.off, count = walk.count;
+            more = walk.next(call);
+            for (int j = 0; j < count; ++j, ++n) {
+                // Lanes 0..7 have a group each.
+                const int idx = (off + j) * kTileGroups + lane;
+                GroupMeta of{0.0f, -INFINITY, 0.0f, 0};
+                int64_t at = -1;
+                if (lane < kTileGroups && idx < range.groups) {
+                    const int key0 = (idx < range.sink_groups ? idx : idx - range.sink_groups + range.first_group) * 16;
+                    const int page = page_at(a.cache, info.seq, key0 >> call.page_shift, call.error_word);
+                    if (page >= 0) {
+                        const int64_t scale = page * a.cache.scale_page_stride + head;
+                        const float vs = a.cache.v_scale[scale], sure = vs < kLeastCacheScale ? kLeastCacheScale : vs;
+                        of.k = a.cache.k_scale[scale];
+                        of.v_log2 = log2f(sure);
+                        of.v_inv = __fdiv_rn(1.0f, sure);
+                        of.key0 = key0;
+                        at = page * a.cache.page_stride + (static_cast<int64_t>(head) * tokens + (key0 & (tokens - 1))) * D;
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h) {
+                            const bool all_seen = key0 + 15 < info.len && key0 + 15 <= range.least_pos[h] &&
+                                                  (a.window == 0 || key0 > range.most_pos[h] - a.window || key0 + 15 < a.sinks);
+                            of.key0 |= all_seen ? 0 : 1 << h;
+                        }
+                    }
+                }
+                // A scale below zero turns the order of its scores round: those too are looked at one by one.
+                const int odd = __reduce_or_sync(0xFFFFFFFFu, (of.key0 & 3) | (of.k * call.factor < 0.0f ? 3 : 0));
+                const uint32_t slot = n % kMetaSlots;
+                if (!tile_wait(&meta_empty[slot], (n / kMetaSlots & 1) ^ 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                if (lane < kTileGroups) {
+                    meta[slot][lane] = of;
+                    where[slot][lane] = at;
+                }
+                if (lane == 0) {
+                    state[slot] = odd | (!more && j + 1 == count ? kBlockLast : 0);
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&meta_full[slot]);
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicCAS(call.error_word, 0, kErrProducerWait);
         }
         __syncwarp();
     }
@@ -937,7 +1001,7 @@ cudaError_t launch_tile_typed(const TileCall& call, int blocks, cudaStream_t str
     if (e != cudaSuccess) {
         return e;
     }
-    e = launch_overlapping(attention_i8_tile_join_kernel<D, T>, dim3(grid, 8), dim3(256), 0, stream, 1, call);
+    e = launch_overlapping(attention_i8_tile_join_kernel<D, T>, dim3(grid, Shared::kRows * (D / 4) / 256), dim3(256), 0, stream, 1, call);
     note_launch();
     return e;
 }
