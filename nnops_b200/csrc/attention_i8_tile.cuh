@@ -26,6 +26,9 @@ namespace nnb200 {
 
 constexpr int kTileKeys = 128;
 constexpr int kTileGroups = kTileKeys / 16;
+constexpr int kParts = 2;       // of a block: the products of one with V run while the softmax is at the next
+constexpr int kPartKeys = kTileKeys / kParts;
+constexpr int kPartGroups = kPartKeys / 16;
 constexpr int kTileCost = 4;    // blocks that a part of a tile costs besides its own: queries, first products, sums
 constexpr int kMetaSlots = 4;   // blocks whose scales are kept: the one the softmax is at, and those the converters are ahead by
 
@@ -242,9 +245,9 @@ struct TileShared {
     static constexpr int kThreads = 32 * (kSoftmaxWarps + 8);   // and four for codes, the MMA issuer, the scout (and two to fill its group)
     // Registers of a thread: at launch, and of the three kinds of warps afterwards.
     static constexpr int kRegisters = kHalves == 2 ? 128 : 168;
-    static constexpr int kSoftmaxRegisters = kHalves == 2 ? 184 : 232;
-    static constexpr int kCodesRegisters = kHalves == 2 ? 88 : 160;
-    static constexpr int kIssuerRegisters = kHalves == 2 ? 56 : 96;
+    static constexpr int kSoftmaxRegisters = kHalves == 2 ? 152 : 200;
+    static constexpr int kCodesRegisters = kHalves == 2 ? 112 : 168;
+    static constexpr int kIssuerRegisters = kHalves == 2 ? 96 : 136;
     static_assert(kHalves * kSoftmaxRegisters + kCodesRegisters + kIssuerRegisters <= (kHalves + 2) * kRegisters, "a group would wait for registers");
     static constexpr int kOutColumn = 256;      // of the sums in tensor memory; S and P are below
     static_assert(kBytes <= 226 * 1024, "shared memory");
@@ -344,6 +347,9 @@ __device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
+// The same in every lane, and in a uniform register: what a reduction gives is, what a shuffle gives is not.
+__device__ __forceinline__ uint32_t in_uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
+
 // 16 codes as f16 into the swizzled tile: row `key`, dims [16 segment, + 16).
 template <int D>
 __device__ __forceinline__ void store_codes(uint8_t* tile, int key, int segment, const uint4& codes)
@@ -367,7 +373,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
     constexpr int kHalves = Shared::kHalves, kStages = Shared::kStages, kRows = Shared::kRows;
     constexpr int kPerThread = D / 16 / Shared::kUnits;   // 16-code segments of a unit that a converting thread has
     extern __shared__ uint8_t raw_shared[];
-    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][kParts], o_full[2][kParts];
     __shared__ __align__(8) uint64_t meta_full[kMetaSlots], meta_empty[kMetaSlots];
     __shared__ GroupMeta meta[kMetaSlots][kTileGroups], identity[kTileGroups];
     __shared__ int64_t where[kMetaSlots][kTileGroups];   // of a group's codes; -1: none
@@ -387,11 +393,13 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             mbar_init(&q_full[i], 128);
             mbar_init(&k_full[i], 128);
             mbar_init(&v_full[i], 128);
-            mbar_init(&p_full[i], 128);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&o_full[i], 1);
+            for (int part = 0; part < kParts; ++part) {
+                mbar_init(&p_full[i][part], 128);
+                mbar_init(&o_full[i][part], 1);
+            }
         }
         for (int i = 0; i < kMetaSlots; ++i) {
             mbar_init(&meta_full[i], 1);
@@ -507,7 +515,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 load_queries();
             }
             if (pending) {
-                if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+                if (!tile_wait(&o_full[half][kParts - 1], (n - 1) & 1, &abort_flag)) {
                     ok = false;
                     break;
                 }
@@ -563,54 +571,70 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             m = -INFINITY;
             l = 0.0f;
             const int count = walk.count;
-            for (int j = 0; j < count; ++j, ++n) {
-                if (!tile_wait(&s_full[half], n & 1, &abort_flag)) {
-                    ok = false;
-                    break;
+#pragma unroll 1
+            for (int i = 0; i < kParts * count; ++i) {
+                // Part i % kParts of block n.
+                const int part = i % kParts;
+                const uint32_t part_addr = s_addr + static_cast<uint32_t>(part * kPartKeys);
+                if (part == 0) {
+                    ok = tile_wait(&s_full[half], n & 1, &abort_flag) &&
+                         tile_wait(&meta_full[n % kMetaSlots], n / kMetaSlots & 1, &abort_flag);   // long since: the products waited for it
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after_sync();
                 }
-                tc_fence_after_sync();
-                (void)tile_wait(&meta_full[n % kMetaSlots], n / kMetaSlots & 1, &abort_flag);   // long since: the products waited for it
-                const GroupMeta* const groups = meta[n % kMetaSlots];
+                const GroupMeta* const groups = meta[n % kMetaSlots] + part * kPartGroups;
                 const bool plain = (state[n % kMetaSlots] >> half & 1) == 0;
                 const GroupMeta* const linear = plain ? groups : identity;
                 if (!plain) {
                     // Scores become exponents in place, those that the row does not see -infinity.
 #pragma unroll 1
-                    for (int g = 0; g < kTileGroups; ++g) {
+                    for (int g = 0; g < kPartGroups; ++g) {
                         const GroupMeta of = groups[g];
                         uint32_t s[16];
-                        tile_tmem_ld_16(s_addr + static_cast<uint32_t>(g * 16), s);
+                        tile_tmem_ld_16(part_addr + static_cast<uint32_t>(g * 16), s);
                         tmem_ld_wait();
                         const bool masked = (of.key0 >> half & 1) != 0;
                         const int key0 = of.key0 & ~15;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int key = key0 + i;
-                            const float t = __fmaf_rn(__uint_as_float(s[i]), of.k * factor, of.v_log2);
-                            s[i] = __float_as_uint(!masked || (key <= pos && (key >= low || key < a.sinks)) ? t : -INFINITY);
+                        for (int e = 0; e < 16; ++e) {
+                            const int key = key0 + e;
+                            const float t = __fmaf_rn(__uint_as_float(s[e]), of.k * factor, of.v_log2);
+                            s[e] = __float_as_uint(!masked || (key <= pos && (key >= low || key < a.sinks)) ? t : -INFINITY);
                         }
-                        tile_tmem_st_16(s_addr + static_cast<uint32_t>(g * 16), s);
+                        tile_tmem_st_16(part_addr + static_cast<uint32_t>(g * 16), s);
                     }
                     tile_tmem_st_wait();
                 }
-                uint32_t s[kTileKeys];
+                uint32_t s[kPartKeys];
+                float k[kPartGroups], add[kPartGroups], tops[kPartGroups];
+                const float scale = plain ? factor : 1.0f;
 #pragma unroll
-                for (int c = 0; c < kTileKeys / 32; ++c) {
-                    tmem_ld_32x32(s_addr + static_cast<uint32_t>(c * 32), *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                for (int c = 0; c < kPartKeys / 32; ++c) {
+                    tmem_ld_32x32(part_addr + static_cast<uint32_t>(c * 32), *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                }
+#pragma unroll
+                for (int g = 0; g < kPartGroups; ++g) {
+                    k[g] = linear[g].k * scale;
+                    add[g] = linear[g].v_log2;
                 }
                 tmem_ld_wait();
-                const float scale = plain ? factor : 1.0f;
-                float top = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < kTileGroups; ++g) {
+                for (int g = 0; g < kPartGroups; ++g) {
                     float high = __uint_as_float(s[16 * g]), other = __uint_as_float(s[16 * g + 1]);
 #pragma unroll
-                    for (int i = 2; i < 14; i += 4) {
-                        high = max3(high, __uint_as_float(s[16 * g + i]), __uint_as_float(s[16 * g + i + 1]));
-                        other = max3(other, __uint_as_float(s[16 * g + i + 2]), __uint_as_float(s[16 * g + i + 3]));
+                    for (int e = 2; e < 14; e += 4) {
+                        high = max3(high, __uint_as_float(s[16 * g + e]), __uint_as_float(s[16 * g + e + 1]));
+                        other = max3(other, __uint_as_float(s[16 * g + e + 2]), __uint_as_float(s[16 * g + e + 3]));
                     }
                     high = max3(high, __uint_as_float(s[16 * g + 14]), __uint_as_float(s[16 * g + 15]));
-                    top = fmaxf(top, __fmaf_rn(fmaxf(high, other), linear[g].k * scale, linear[g].v_log2));
+                    tops[g] = __fmaf_rn(fmaxf(high, other), k[g], add[g]);
+                }
+                float top = tops[0];
+#pragma unroll
+                for (int g = 1; g < kPartGroups; ++g) {
+                    top = fmaxf(top, tops[g]);
                 }
                 const bool grown = top > m + 8.0f || (m == -INFINITY && top > m);
                 if (__any_sync(0xFFFFFFFFu, grown)) {
@@ -618,9 +642,9 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                     const float alpha = grown ? exp2_fast(m - next) : 1.0f;
                     m = next;
                     l *= alpha;
-                    if (j > 0) {
-                        // The sums so far are complete: the next block's products wait for this one's weights.
-                        if (!tile_wait(&o_full[half], (n - 1) & 1, &abort_flag)) {
+                    if (i > 0) {
+                        // The sums so far are complete: the next part's products wait for this one's weights.
+                        if (!tile_wait(&o_full[half][(part + kParts - 1) % kParts], (part == 0 ? n - 1 : n) & 1, &abort_flag)) {
                             ok = false;
                             break;
                         }
@@ -631,45 +655,53 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                             tile_tmem_ld_16(o_addr + static_cast<uint32_t>(c * 16), o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            for (int e = 0; e < 16; ++e) {
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
                             }
                             tile_tmem_st_16(o_addr + static_cast<uint32_t>(c * 16), o);
                         }
                     }
                 }
                 const float safe = m == -INFINITY ? 0.0f : m;
+                uint64_t sums[kPartGroups];
 #pragma unroll
-                for (int c = 0; c < kTileGroups / 2; ++c) {
+                for (int c = 0; c < kPartGroups / 2; ++c) {
                     uint32_t p[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int g = 2 * c + h;
-                        const float k = linear[g].k * scale, add = linear[g].v_log2 - safe;
-                        const uint64_t kk = pair_of(k, k), aa = pair_of(add, add);
-                        uint64_t sum = 0;
+                        const float less = add[g] - safe;
+                        const uint64_t kk = pair_of(k[g], k[g]), aa = pair_of(less, less);
+                        uint64_t sum[2] = {0, 0};
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
+                        for (int e = 0; e < 8; ++e) {
                             float x, y;
-                            unpair(pair_fma(pair_of(__uint_as_float(s[16 * g + 2 * i]), __uint_as_float(s[16 * g + 2 * i + 1])), kk, aa), x, y);
+                            unpair(pair_fma(pair_of(__uint_as_float(s[16 * g + 2 * e]), __uint_as_float(s[16 * g + 2 * e + 1])), kk, aa), x, y);
                             x = exp2_fast(x);
                             y = exp2_fast(y);
-                            sum = pair_add(sum, pair_of(x, y));
-                            p[8 * h + i] = pack2<__half>(x, y);
+                            sum[e & 1] = e < 2 ? pair_of(x, y) : pair_add(sum[e & 1], pair_of(x, y));
+                            p[8 * h + e] = pack2<__half>(x, y);
                         }
-                        float x, y;
-                        unpair(sum, x, y);
-                        x += y;
-                        l += x == 0.0f ? 0.0f : x * groups[g].v_inv;   // (not 0 times what a block that is masked has for a scale)
+                        sums[g] = pair_add(sum[0], sum[1]);
                     }
-                    tile_tmem_st_16(s_addr + static_cast<uint32_t>(c * 16), p);
+                    tile_tmem_st_16(part_addr + static_cast<uint32_t>(c * 16), p);
                 }
                 tile_tmem_st_wait();
                 tc_fence_before_sync();
-                mbar_arrive(&p_full[half]);
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&meta_empty[n % kMetaSlots]);
+                mbar_arrive(&p_full[half][part]);
+#pragma unroll
+                for (int g = 0; g < kPartGroups; ++g) {
+                    float x, y;
+                    unpair(sums[g], x, y);
+                    x += y;
+                    l += x == 0.0f ? 0.0f : x * groups[g].v_inv;   // (not 0 times what a block that is masked has for a scale)
+                }
+                if (part == kParts - 1) {
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&meta_empty[n % kMetaSlots]);
+                    }
+                    ++n;
                 }
             }
             if (!ok) {
@@ -765,7 +797,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         __syncwarp();
     } else if (fewer_registers<Shared::kIssuerRegisters>(); warp == Shared::kSoftmaxWarps + 4) {
         // ---------------- MMA issuer ----------------
-        const uint32_t base = warp_uniform(tmem);
+        const uint32_t base = in_uniform(tmem);
         constexpr uint32_t kIdescS = umma_idesc(1, 0, 0, 128, kTileKeys);
         constexpr uint32_t kIdescO = umma_idesc(1, 0, 0, 128, D) | kUmmaBMajorMN;
         const uint64_t q_desc = umma_desc_sw128_kmajor(smem_u32(q_tile));
@@ -773,7 +805,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         const uint64_t v_desc = umma_desc_sw128_mnmajor(smem_u32(v_tile), Shared::kBlockBytes);
         constexpr uint64_t kTileStep = Shared::kTileBytes / 16, kBlockStep = Shared::kBlockBytes / 16;
         uint32_t failed = 0;
-        const auto scores = [&](int half, uint32_t slot) {
+        const auto scores = [&](int half, uint32_t slot, bool last) {
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
@@ -782,61 +814,61 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                              k_desc + slot * kTileStep + step, kIdescS, k > 0 ? 1u : 0u);
                 }
                 umma_commit_unless(&s_full[half], failed);
+                if (last) {
+                    umma_commit_unless(&k_empty[slot], failed);
+                }
             }
             __syncwarp();
         };
         uint32_t n = 0, units = 0;
         // What steers the loops is made uniform in the compiler's eyes: the MMAs' operands then stay in uniform registers.
-        while (warp_uniform(walk.next(call) ? 1 : 0) != 0) {
-            const int count = warp_uniform(walk.count);
+        while (in_uniform(walk.next(call) ? 1u : 0u) != 0) {
+            const int count = static_cast<int>(in_uniform(static_cast<uint32_t>(walk.count)));
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 mbar_wait_converged<kErrMmaWait>(&q_full[h], units & 1, &abort_flag, failed);
+                if (h == 0) {
+                    mbar_wait_converged<kErrMmaWait>(&k_full[n % kStages], n / kStages & 1, &abort_flag, failed);
+                }
+                tc_fence_after_sync();
+                scores(h, n % kStages, h == kHalves - 1);
             }
-            mbar_wait_converged<kErrMmaWait>(&k_full[n % kStages], n / kStages & 1, &abort_flag, failed);
-            tc_fence_after_sync();
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                scores(h, n % kStages);
-            }
-            if (elect_one()) {
-                umma_commit_unless(&k_empty[n % kStages], failed);
-            }
-            __syncwarp();
             for (int j = 0; j < count; ++j, ++n) {
                 const bool next = j + 1 < count;
                 const uint32_t slot = n % kStages, next_slot = (n + 1) % kStages;
+                // One half after the other: while the products of one run, the softmax of the other does.
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) {
-                    mbar_wait_converged<kErrMmaWait>(&p_full[h], n & 1, &abort_flag, failed);
                     if (h == 0) {
                         mbar_wait_converged<kErrMmaWait>(&v_full[slot], n / kStages & 1, &abort_flag, failed);
                     }
-                    tc_fence_after_sync();
-                    if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < kTileKeys / 16; ++k) {
-                            tile_mma_p(base + static_cast<uint32_t>(Shared::kOutColumn + h * 128), base + static_cast<uint32_t>(h * 128 + k * 8),
-                                       v_desc + slot * kTileStep + static_cast<uint64_t>(k * 2048 / 16), kIdescO, j > 0 || k > 0 ? 1u : 0u);
+                    for (int part = 0; part < kParts; ++part) {
+                        mbar_wait_converged<kErrMmaWait>(&p_full[h][part], n & 1, &abort_flag, failed);
+                        tc_fence_after_sync();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < kPartKeys / 16; ++k) {
+                                tile_mma_p(base + static_cast<uint32_t>(Shared::kOutColumn + h * 128),
+                                           base + static_cast<uint32_t>(h * 128 + part * kPartKeys + k * 8),
+                                           v_desc + slot * kTileStep + static_cast<uint64_t>((part * kPartKeys + k * 16) * 128 / 16), kIdescO,
+                                           j > 0 || part > 0 || k > 0 ? 1u : 0u);
+                            }
+                            umma_commit_unless(&o_full[h][part], failed);
+                            if (h == kHalves - 1 && part == kParts - 1) {
+                                umma_commit_unless(&v_empty[slot], failed);
+                            }
                         }
-                        umma_commit_unless(&o_full[h], failed);
+                        __syncwarp();
                     }
-                    __syncwarp();
                     if (next) {
                         if (h == 0) {
                             mbar_wait_converged<kErrMmaWait>(&k_full[next_slot], (n + 1) / kStages & 1, &abort_flag, failed);
                             tc_fence_after_sync();
                         }
-                        scores(h, next_slot);
+                        scores(h, next_slot, h == kHalves - 1);   // over the weights that have just been used
                     }
                 }
-                if (elect_one()) {
-                    umma_commit_unless(&v_empty[slot], failed);
-                    if (next) {
-                        umma_commit_unless(&k_empty[next_slot], failed);
-                    }
-                }
-                __syncwarp();
             }
             ++units;
         }
