@@ -54,7 +54,7 @@ TilePlan tile_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
     p.tiles = 16;
     p.first_tile = p.tiles + up(static_cast<size_t>(most) * sizeof(TileInfo));
     p.pieces = p.first_tile + up(static_cast<size_t>(c.seqs + 1) * sizeof(int32_t));
-    p.sums = p.pieces + up(pieces * sizeof(RowsPiece));
+    p.sums = p.pieces + up(pieces * sizeof(TilePiece));
     p.bytes = p.sums + pieces * static_cast<size_t>(rows) * static_cast<size_t>(c.dim + 2) * sizeof(float);
     return p;
 }
@@ -95,7 +95,7 @@ int run_tile(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.line = reinterpret_cast<int64_t*>(base);
     call.tiles = reinterpret_cast<TileInfo*>(base + p.tiles);
     call.first_tile = reinterpret_cast<int32_t*>(base + p.first_tile);
-    call.pieces = reinterpret_cast<RowsPiece*>(base + p.pieces);
+    call.pieces = reinterpret_cast<TilePiece*>(base + p.pieces);
     call.sums = reinterpret_cast<float*>(base + p.sums);
     switch (a.cache.dim) {
     case 64: return cuda_status(launch_attention_tile_64(call, dev.sm_count, stream));

@@ -39,6 +39,15 @@ struct TileInfo {
     int64_t before;                    // length of all tiles before this one, of one head: blocks, and kTileCost for each
 };
 
+// A part of a tile that was cut, as in RowsPiece, and the rows that it is of.
+struct TilePiece {
+    int32_t kind, head;
+    int32_t row0;    // the sequence's first
+    int32_t first;   // of the sequence's rows times heads of the group
+    int32_t rows;
+    int32_t unused[3];
+};
+
 struct TileCall {
     nnb200_attention_i8_args a;
     int32_t* error_word;
@@ -50,7 +59,7 @@ struct TileCall {
     int64_t* line;        // [0] tiles, [1] length of all tiles, of one head
     TileInfo* tiles;
     int32_t* first_tile;  // [seqs + 1]: tiles before each sequence's
-    RowsPiece* pieces;    // [blocks of the grid][2]
+    TilePiece* pieces;    // [blocks of the grid][2]
     float* sums;          // [blocks of the grid][2][dim / 4][rows][4], then m and l of each row
 };
 
@@ -83,16 +92,20 @@ __device__ __forceinline__ TileRange tile_range(const TileCall& call, int tile, 
     return r;
 }
 
-// Which tiles there are, and where each begins on the line.  One block.
+// Which tiles there are, and where each begins on the line.  One block; what it has found out of the first 1024 sequences
+// stays in shared memory.
 template <int ROWS>
 __global__ void __launch_bounds__(1024) attention_i8_plan_kernel(const TileCall call)
 {
+    constexpr int kKept = 1024;
+    __shared__ int64_t part[2][32];
+    __shared__ int kept_first[kKept + 1];
+    __shared__ SequenceRows kept_rows[kKept];
     previous_kernel_done();
-    __shared__ int64_t part[32];
-    __shared__ int64_t carry;
     const int seqs = static_cast<int>(call.a.cache.seqs), lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    // Of the threads before this one, on top of what earlier rounds left.
-    const auto before = [&](int64_t v) {
+    int turn = 0;
+    // Of the threads before this one and of all, over the block.
+    const auto before = [&](int64_t v, int64_t& total) {
         int64_t up = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -100,64 +113,65 @@ __global__ void __launch_bounds__(1024) attention_i8_plan_kernel(const TileCall 
             up += lane >= o ? other : 0;
         }
         if (lane == 31) {
-            part[warp] = up;
+            part[turn][warp] = up;
         }
         __syncthreads();
-        int64_t sum = carry;
-        for (int i = 0; i < warp; ++i) {
-            sum += part[i];
+        int64_t warps = part[turn][lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t other = __shfl_up_sync(0xFFFFFFFFu, warps, o);
+            warps += lane >= o ? other : 0;
         }
-        __syncthreads();
-        if (threadIdx.x == 1023) {
-            carry = sum + up;
-        }
-        __syncthreads();
-        return sum + up - v;
+        total = __shfl_sync(0xFFFFFFFFu, warps, 31);
+        const int64_t earlier = __shfl_sync(0xFFFFFFFFu, warps, warp > 0 ? warp - 1 : 0);
+        turn ^= 1;   // the next round's may be written while this one's are read
+        return (warp > 0 ? earlier : 0) + up - v;
     };
-    if (threadIdx.x == 0) {
-        carry = 0;
-    }
-    __syncthreads();
+    int64_t tiles = 0, total;
     for (int b0 = 0; b0 < seqs; b0 += 1024) {
         const int b = b0 + static_cast<int>(threadIdx.x);
-        const int own = b < seqs ? (sequence_rows(call.a.cache, b).n * call.group + ROWS - 1) / ROWS : 0;
-        const int64_t first = before(own);
+        SequenceRows s{};
+        if (b < seqs) {
+            s = sequence_rows(call.a.cache, b);
+        }
+        const int64_t first = tiles + before((s.n * call.group + ROWS - 1) / ROWS, total);
         if (b < seqs) {
             call.first_tile[b] = static_cast<int32_t>(first);
+            if (b < kKept) {
+                kept_first[b] = static_cast<int>(first);
+                kept_rows[b] = s;
+            }
         }
-    }
-    const int tiles = static_cast<int>(carry);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        call.first_tile[seqs] = tiles;
-        call.line[0] = tiles;
-        carry = 0;
+        tiles += total;
     }
     __syncthreads();
+    int64_t line = 0;
     for (int i0 = 0; i0 < tiles; i0 += 1024) {
         const int i = i0 + static_cast<int>(threadIdx.x);
         TileInfo info{};
         if (i < tiles) {
-            int low = 0, high = seqs;   // first_tile[low] <= i < first_tile[high]
+            int low = 0, high = seqs;   // first_tile[low] <= i, and below first_tile[high]
             while (high - low > 1) {
                 const int mid = (low + high) / 2;
-                (call.first_tile[mid] <= i ? low : high) = mid;
+                ((mid < kKept ? kept_first[mid] : call.first_tile[mid]) <= i ? low : high) = mid;
             }
-            const SequenceRows s = sequence_rows(call.a.cache, low);
+            const SequenceRows s = low < kKept ? kept_rows[low] : sequence_rows(call.a.cache, low);
             info.seq = low;
-            info.tile = i - call.first_tile[low];
+            info.tile = i - (low < kKept ? kept_first[low] : call.first_tile[low]);
             info.row0 = s.row0;
             info.n = s.n;
             info.len = s.len;
             info.blocks = max((tile_range<ROWS>(call, info.tile, s.n, s.len).groups + kTileGroups - 1) / kTileGroups, 1);
         }
-        info.before = before(i < tiles ? info.blocks + kTileCost : 0);
+        info.before = line + before(i < tiles ? info.blocks + kTileCost : 0, total);
         if (i < tiles) {
             call.tiles[i] = info;
         }
+        line += total;
     }
     if (threadIdx.x == 0) {
-        call.line[1] = carry;
+        call.line[0] = tiles;
+        call.line[1] = line;
     }
 }
 
@@ -505,7 +519,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         bool had = false, whole = false, pending = false;
         int which = 0;
         T* dst = nullptr;
-        RowsPiece about{};
+        TilePiece about{};
         float m = 0.0f, l = 0.0f;
         bool ok = true, more = walk.next(call);
         while (more || pending) {
@@ -710,7 +724,8 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             whole = walk.begins && walk.ends;
             had = there;
             which = walk.begins ? 1 : 0;
-            about = RowsPiece{walk.begins ? 1 : walk.ends ? 3 : 2, walk.info.seq, walk.head, walk.info.tile};
+            about = TilePiece{walk.begins ? 1 : walk.ends ? 3 : 2, walk.head, walk.info.row0, walk.info.tile * kRows,
+                              min(kRows, walk.info.n * call.group - walk.info.tile * kRows), {}};
             dst = static_cast<T*>(a.out) + place;
             pending = true;
             more = walk.next(call);
@@ -951,56 +966,59 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
     }
 }
 
-// Joins the pieces of the tiles that were cut: blockIdx.x of the grid of the kernel before, in gridDim.y parts.
+// Joins the pieces of the tiles that were cut: blockIdx.x of the grid of the kernel before, 16 dims each block.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) attention_i8_tile_join_kernel(const TileCall call)
 {
     previous_kernel_done();
     constexpr int kRows = TileShared<D>::kRows;
     constexpr int64_t kPiece = kRows * (D + 2);
-    const RowsPiece mine = call.pieces[2 * blockIdx.x + 1];
+    const TilePiece mine = call.pieces[2 * blockIdx.x + 1];
     if (mine.kind != 1) {
         return;
     }
     const nnb200_attention_i8_args& a = call.a;
-    const SequenceRows s = sequence_rows(a.cache, mine.seq);
-    const int rows = min(kRows, s.n * call.group - mine.tile * kRows);
     int last = blockIdx.x + 1;
     while (last < static_cast<int>(gridDim.x) - 1 && call.pieces[2 * last].kind == 2) {
         ++last;
     }
     const float* first = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kPiece;
     const float* rest = call.sums + 2 * static_cast<int64_t>(blockIdx.x + 1) * kPiece;
-    const int more = last - static_cast<int>(blockIdx.x);
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < kRows * (D / 4); i += 256 * gridDim.y) {
-        const int r = i % kRows, d = i / kRows * 4;
-        if (r >= rows) {
-            continue;
+    const int more = last - static_cast<int>(blockIdx.x), r = threadIdx.x, d = blockIdx.y * 16;
+    if (r >= mine.rows) {
+        return;
+    }
+    // A maximum that later turns out too small is made up for, so that a piece is read once.
+    float top = -INFINITY, total = 0.0f;
+    float4 sum[4] = {};
+    for (int p = -1; p < more; ++p) {
+        const float* piece = p < 0 ? first : rest + p * 2 * kPiece;
+        const float m = piece[kRows * D + r], l = piece[kRows * (D + 1) + r];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = reinterpret_cast<const float4*>(piece)[(d / 4 + i) * kRows + r];
         }
-        float top = first[kRows * D + r];
-        for (int p = 0; p < more; ++p) {
-            top = fmaxf(top, rest[p * 2 * kPiece + kRows * D + r]);
+        const float next = fmaxf(top, m), safe = next == -INFINITY ? 0.0f : next;
+        const float old = exp2_fast(top - safe), share = exp2_fast(m - safe);
+        top = next;
+        total = __fmaf_rn(l, share, total * old);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum[i].x = __fmaf_rn(v[i].x, share, sum[i].x * old);
+            sum[i].y = __fmaf_rn(v[i].y, share, sum[i].y * old);
+            sum[i].z = __fmaf_rn(v[i].z, share, sum[i].z * old);
+            sum[i].w = __fmaf_rn(v[i].w, share, sum[i].w * old);
         }
-        const float safe = top == -INFINITY ? 0.0f : top;
-        float total = 0.0f;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = -1; p < more; ++p) {
-            const float* piece = p < 0 ? first : rest + p * 2 * kPiece;
-            const float share = exp2_fast(piece[kRows * D + r] - safe);
-            const float4 v = reinterpret_cast<const float4*>(piece)[d / 4 * kRows + r];
-            total = __fmaf_rn(piece[kRows * (D + 1) + r], share, total);
-            sum.x = __fmaf_rn(v.x, share, sum.x);
-            sum.y = __fmaf_rn(v.y, share, sum.y);
-            sum.z = __fmaf_rn(v.z, share, sum.z);
-            sum.w = __fmaf_rn(v.w, share, sum.w);
-        }
-        const int global = mine.tile * kRows + r;
-        T* dst = static_cast<T*>(a.out) + (s.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d;
-        const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-        dst[0] = from_float<T>(sum.x * inv);
-        dst[1] = from_float<T>(sum.y * inv);
-        dst[2] = from_float<T>(sum.z * inv);
-        dst[3] = from_float<T>(sum.w * inv);
+    }
+    const int global = mine.first + r;
+    T* dst = static_cast<T*>(a.out) + (mine.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d;
+    const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float f[8] = {sum[2 * i].x * inv, sum[2 * i].y * inv, sum[2 * i].z * inv, sum[2 * i].w * inv,
+                            sum[2 * i + 1].x * inv, sum[2 * i + 1].y * inv, sum[2 * i + 1].z * inv, sum[2 * i + 1].w * inv};
+        store8(dst + 8 * i, call.wide != 0, f);
     }
 }
 
@@ -1033,7 +1051,7 @@ cudaError_t launch_tile_typed(const TileCall& call, int blocks, cudaStream_t str
     if (e != cudaSuccess) {
         return e;
     }
-    e = launch_overlapping(attention_i8_tile_join_kernel<D, T>, dim3(grid, Shared::kRows * (D / 4) / 256), dim3(256), 0, stream, 1, call);
+    e = launch_overlapping(attention_i8_tile_join_kernel<D, T>, dim3(grid, D / 16), dim3(Shared::kRows), 0, stream, 1, call);
     note_launch();
     return e;
 }
