@@ -364,6 +364,18 @@ __device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volati
 // The same in every lane, and in a uniform register: what a reduction gives is, what a shuffle gives is not.
 __device__ __forceinline__ uint32_t in_uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
 
+// Eight 16-bit values as they are; `wide`: the address is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ uint4 eight_of(const T* p, bool wide)
+{
+    if (wide) {
+        return *reinterpret_cast<const uint4*>(p);
+    }
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    const auto two = [&](int i) { return static_cast<uint32_t>(h[i]) | static_cast<uint32_t>(h[i + 1]) << 16; };
+    return make_uint4(two(0), two(2), two(4), two(6));
+}
+
 // 16 codes as f16 into the swizzled tile: row `key`, dims [16 segment, + 16).
 template <int D>
 __device__ __forceinline__ void store_codes(uint8_t* tile, int key, int segment, const uint4& codes)
@@ -463,30 +475,29 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             pos = pos < walk.info.len ? pos : walk.info.len - 1;
             low = a.window > 0 && there ? static_cast<int64_t>(pos) - a.window + 1 : INT64_MIN;
             factor = call.factor;
-            // Four lanes to a row, eight rows at a time: 64 bytes of each next to each other.
+            // Four lanes to a row, eight rows at a time: 64 bytes of each next to each other.  All are asked for before any is looked at.
+            uint4 raw[4][D / 32];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = i * 8 + lane / 4;
                 const bool row_there = first + r < all;
                 const T* src = static_cast<const T*>(a.q) + (row_there ? source(r, a.q_stride_row, a.q_stride_head) : 0) + lane % 4 * 8;
-                float f[D / 32][8];
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[c][e] = 0.0f;
-                    }
-                    if (row_there) {
-                        load8(src + c * 32, call.wide != 0, f[c]);
-                    }
+                    raw[i][c] = row_there ? eight_of(src + c * 32, call.wide != 0) : make_uint4(0u, 0u, 0u, 0u);
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + lane / 4;
                 if constexpr (!std::is_same_v<T, __half>) {   // scaled by a power of two into f16
                     uint32_t top = 0;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
+                        const uint32_t w[4] = {raw[i][c].x, raw[i][c].y, raw[i][c].z, raw[i][c].w};
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            top = max(top, magnitude_bits(f[c][e]));
+                        for (int e = 0; e < 4; ++e) {
+                            top = max(top, max(w[e] << 16 & 0x7FFF0000u, w[e] & 0x7FFF0000u));
                         }
                     }
                     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
@@ -496,20 +507,21 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                     const float up = call.factor * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                     const float mine = __shfl_sync(0xFFFFFFFFu, up, lane % 8 * 4);
                     factor = lane / 8 == i ? mine : factor;
+                    const auto scaled = [&](uint32_t w) {
+                        float x, y;
+                        unpack2<T>(w, x, y);
+                        return pack2<__half>(x * down, y * down);
+                    };
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            f[c][k] *= down;
-                        }
+                        raw[i][c] = make_uint4(scaled(raw[i][c].x), scaled(raw[i][c].y), scaled(raw[i][c].z), scaled(raw[i][c].w));
                     }
                 }
                 uint8_t* const to = q_tile + half * Shared::kTileBytes + ((warp & 3) * 32 + r) * 128;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     const int chunk = c * 4 + lane % 4;
-                    *reinterpret_cast<uint4*>(to + chunk / 8 * Shared::kBlockBytes + (((chunk & 7) ^ (r & 7)) << 4)) =
-                        make_uint4(pack2<__half>(f[c][0], f[c][1]), pack2<__half>(f[c][2], f[c][3]), pack2<__half>(f[c][4], f[c][5]), pack2<__half>(f[c][6], f[c][7]));
+                    *reinterpret_cast<uint4*>(to + chunk / 8 * Shared::kBlockBytes + (((chunk & 7) ^ (r & 7)) << 4)) = raw[i][c];
                 }
             }
             fence_proxy_async_smem();
@@ -908,6 +920,17 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             const TileInfo info = walk.info;
             const int head = walk.head, off = walk.off, count = walk.count;
             more = walk.next(call);
+            if (more) {   // the queries that come after this part's are on their way into L2 by the time they are asked for
+                const int first = walk.info.tile * kRows, rows = min(kRows, walk.info.n * call.group - first);
+                for (int r = lane; r < rows; r += 32) {
+                    const int token = (first + r) / call.group;
+                    const T* src = static_cast<const T*>(a.q) + (walk.info.row0 + token) * a.q_stride_row + (walk.head * call.group + (first + r) - token * call.group) * a.q_stride_head;
+#pragma unroll
+                    for (int byte = 0; byte < 2 * D; byte += 128) {
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const uint8_t*>(src) + byte));
+                    }
+                }
+            }
             for (int j = 0; j < count; ++j, ++n) {
                 // Lanes 0..7 have a group each.
                 const int idx = (off + j) * kTileGroups + lane;
