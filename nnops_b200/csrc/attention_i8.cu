@@ -16,6 +16,11 @@ int64_t rows_each(const nnb200_attention_i8_args& a)
     return (c.rows + c.seqs - 1) / c.seqs * (a.q_heads / c.heads);
 }
 
+int page_shift(const nnb200_attention_i8_args& a)
+{
+    return a.cache.page_tokens == 16 ? 4 : a.cache.page_tokens == 32 ? 5 : a.cache.page_tokens == 64 ? 6 : 7;
+}
+
 int engine_of(const nnb200_attention_i8_args& a)
 {
     if (a.float_type == NNB200_FLOAT_F32) {
@@ -67,6 +72,13 @@ int run_rows(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.error_word = dev.error_word;
     call.group = static_cast<int>(a.q_heads / a.cache.heads);
     call.factor = a.scale * 1.4426950408889634f;
+    const int64_t per = a.float_type == NNB200_FLOAT_F32 ? 4 : 8;
+    const auto multiple = [&](const void* p, uintptr_t bytes, int64_t row, int64_t head, int64_t values) {
+        return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && row % values == 0 && head % values == 0 ? 1 : 0;
+    };
+    call.wide = multiple(a.q, 16, a.q_stride_row, a.q_stride_head, per);
+    call.wide_out = multiple(a.out, 128 / per / 2, a.out_stride_row, a.out_stride_head, 4);
+    call.page_shift = page_shift(a);
     call.pieces = static_cast<RowsPiece*>(a.workspace);
     call.sums = reinterpret_cast<float*>(call.pieces + 2 * static_cast<size_t>(p.blocks));
     switch (a.cache.dim) {
@@ -90,7 +102,7 @@ int run_tile(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.factor = a.scale * 1.4426950408889634f;
     call.wide = wide(a.q, a.q_stride_row, a.q_stride_head) && wide(a.out, a.out_stride_row, a.out_stride_head) ? 1 : 0;
     call.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.out_stride_row % 16 == 0 && a.out_stride_head % 16 == 0 ? 1 : 0;
-    call.page_shift = a.cache.page_tokens == 16 ? 4 : a.cache.page_tokens == 32 ? 5 : a.cache.page_tokens == 64 ? 6 : 7;
+    call.page_shift = page_shift(a);
     uint8_t* const base = static_cast<uint8_t*>(a.workspace);
     call.line = reinterpret_cast<int64_t*>(base);
     call.tiles = reinterpret_cast<TileInfo*>(base + p.tiles);

@@ -7,7 +7,8 @@
 //
 // which is the softmax with each block's V scale moved into the exponent: the weights that meet the codes are then at
 // most 1 and the largest is 1 whatever the scales are, so that f16 holds them, and one exponential serves both sums.
-// One pass over the tokens, with the running maximum.
+// One pass over the tokens, with the running maximum; the sums are rescaled only when that has grown by more than 2^8, so
+// weights are at most 2^8, and the lanes of a row compare their maxima only then.
 //
 // A warp takes 16 tokens at a time and is on its own: it copies their codes into its part of shared memory
 // (cp.async.bulk; 16 tokens never leave a page, and one head's share of a page is contiguous), turns bytes into f16
@@ -30,6 +31,8 @@ namespace nnb200 {
 
 constexpr int kRowsWarps = 8;
 constexpr int kRowsThreads = 32 * kRowsWarps;
+constexpr int kRowsCost = 16;     // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
+constexpr float kGrowth = 8.0f;   // log2 of what a weight may be
 
 // What a block leaves in the workspace: [0] the end or the middle of a row tile that began in an earlier
 // block, [1] the beginning of one that ends in a later block.
@@ -49,6 +52,9 @@ struct RowsCall {
     int32_t* error_word;
     int group;           // query heads of a key head
     float factor;        // scale * log2 e
+    int wide;            // q's rows and heads are 16-byte aligned
+    int wide_out;        // out's are, to four values
+    int page_shift;      // log2 of the tokens of a page
     RowsPiece* pieces;   // [blocks][2]
     float* sums;         // [blocks][2][piece]
 };
@@ -58,7 +64,7 @@ struct SequenceWork {
     SequenceRows s;
     int sink_groups, first_group, groups;   // groups of a row tile: the sinks', then those from first_group on; 1 at least
     int tiles;
-    int64_t total;
+    int64_t total;   // length: of every item its groups and kRowsCost
 };
 
 __device__ __forceinline__ SequenceWork sequence_work(const RowsCall& call, int b, int tile_rows)
@@ -73,7 +79,7 @@ __device__ __forceinline__ SequenceWork sequence_work(const RowsCall& call, int 
     w.sink_groups = a.window > 0 ? min((sinks + 15) / 16, w.first_group) : 0;
     w.groups = max(w.sink_groups + (w.s.len + 15) / 16 - w.first_group, 1);
     w.tiles = (w.s.n * call.group + tile_rows - 1) / tile_rows;
-    w.total = static_cast<int64_t>(a.cache.heads) * w.tiles * w.groups;
+    w.total = static_cast<int64_t>(a.cache.heads) * w.tiles * (w.groups + kRowsCost);
     return w;
 }
 
@@ -148,22 +154,75 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
     }
 }
 
-__device__ __forceinline__ float load_float(const void* p, int64_t i, int type)
+// COUNT consecutive values from element i on; `wide`: their address is 16-byte aligned.
+template <int COUNT, typename T>
+__device__ __forceinline__ void load_values(const T* p, bool wide, float (&v)[COUNT])
 {
-    return type == NNB200_FLOAT_F32   ? static_cast<const float*>(p)[i]
-           : type == NNB200_FLOAT_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                                      : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+#pragma unroll
+    for (int i = 0; i < COUNT; i += 8) {
+        load8(p + i, wide, *reinterpret_cast<float(*)[8]>(v + i));
+    }
 }
-
-__device__ __forceinline__ void store_float(void* p, int64_t i, int type, float v)
+template <int COUNT>
+__device__ __forceinline__ void load_floats(const void* p, int64_t i, int type, bool wide, float (&v)[COUNT])
 {
     if (type == NNB200_FLOAT_F32) {
-        static_cast<float*>(p)[i] = v;
+        load_values(static_cast<const float*>(p) + i, wide, v);
     } else if (type == NNB200_FLOAT_F16) {
-        static_cast<__half*>(p)[i] = __float2half_rn(v);
+        load_values(static_cast<const __half*>(p) + i, wide, v);
     } else {
-        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+        load_values(static_cast<const __nv_bfloat16*>(p) + i, wide, v);
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_four(T* p, bool wide, float4 v)
+{
+    if (!wide) {
+        p[0] = from_float<T>(v.x);
+        p[1] = from_float<T>(v.y);
+        p[2] = from_float<T>(v.z);
+        p[3] = from_float<T>(v.w);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = v;
+    } else {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+    }
+}
+// sum / total, or zeros where nothing was seen.
+__device__ __forceinline__ void store_row(const RowsCall& call, int64_t i, float4 sum, float total)
+{
+    const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+    const float4 v = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    if (call.a.float_type == NNB200_FLOAT_F32) {
+        store_four(static_cast<float*>(call.a.out) + i, call.wide_out != 0, v);
+    } else if (call.a.float_type == NNB200_FLOAT_F16) {
+        store_four(static_cast<__half*>(call.a.out) + i, call.wide_out != 0, v);
+    } else {
+        store_four(static_cast<__nv_bfloat16*>(call.a.out) + i, call.wide_out != 0, v);
+    }
+}
+
+// Every lane polls: the data behind the barrier is then every lane's.  Without a hint how long to sleep, which costs a
+// hundred cycles on a barrier that is all but ready; within the limit that mbar_wait has.
+__device__ __forceinline__ bool wait_every_lane(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
+{
+    bool done = mbar_try_wait(bar, parity);
+    if (!__all_sync(0xFFFFFFFFu, done)) {
+        const long long t0 = clock64();
+        bool give_up = false;
+        for (uint32_t spins = 1; !done && !give_up; ++spins) {
+            done = mbar_try_wait(bar, parity);
+            if ((spins & 63u) == 0) {
+                if (*abort_flag == 0 && clock64() - t0 > kWaitLimitCycles) {
+                    *abort_flag = 1;
+                }
+                give_up = *abort_flag != 0;
+            }
+        }
+        return __all_sync(0xFFFFFFFFu, done);
+    }
+    return true;
 }
 
 // Bytes of shared memory: the warps' rings, which hold the warps' sums when a piece is joined; barriers; per-stage scales.
@@ -242,8 +301,8 @@ attention_i8_rows_kernel(const RowsCall call)
         (void)block_sum_before(b < seqs ? sequence_work(call, b, kTile).total : 0, total);
         line += total;
     }
-    // No fewer than a group a warp for a block.
-    const int64_t share_at_least = kRowsWarps;
+    // No fewer than a group a warp for a block, besides what an item costs.
+    const int64_t share_at_least = kRowsWarps + kRowsCost;
     const int64_t most = (line + share_at_least - 1) / share_at_least;
     const int64_t blocks = most < gridDim.x ? most : gridDim.x;
     RowsPiece* pieces = call.pieces + 2 * blockIdx.x;
@@ -274,7 +333,8 @@ attention_i8_rows_kernel(const RowsCall call)
     int64_t base = found_base;
     int kinds[2] = {0, 0};
 
-    uint32_t issued = 0, taken = 0;   // 16-token groups of this warp
+    uint32_t issued = 0;   // 16-token groups of this warp
+    uint32_t issue_slot = 0, slot = 0, round = 0;   // of the ring: the next to fill, the next to take and its turn
     uint8_t* const my_ring = ring + warp * kStages * Shared::kStageBytes;
     bool failed = false;
 
@@ -285,12 +345,16 @@ attention_i8_rows_kernel(const RowsCall call)
             ++seq;
             continue;
         }
-        const int64_t item = (at - base) / work.groups;
-        const int off = static_cast<int>((at - base) % work.groups);
+        const int length = work.groups + kRowsCost;
+        const int64_t item = (at - base) / length;
+        const int from = static_cast<int>((at - base) % length);
+        const int to = static_cast<int>(from + (end - at) < length ? from + (end - at) : length);
+        at += to - from;
+        const int off = max(from - kRowsCost, 0), count = max(to - kRowsCost, 0) - off;
+        if (count <= 0) {
+            continue;
+        }
         const int head = static_cast<int>(item / work.tiles), tile = static_cast<int>(item % work.tiles);
-        const int64_t room = end - at;
-        const int count = static_cast<int>(work.groups - off < room ? work.groups - off : room);
-        at += count;
 
         const int rows = min(kTile, work.s.n * call.group - tile * kTile);
         const int first_pos = work.s.len - work.s.n;
@@ -305,10 +369,16 @@ attention_i8_rows_kernel(const RowsCall call)
             const int global = tile * kTile + r;
             const int64_t src = (work.s.row0 + global / call.group) * a.q_stride_row + (head * call.group + global % call.group) * a.q_stride_head + c * (D / 4);
             float v[D / 4];
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+                v[i] = 0.0f;
+            }
+            if (r < rows) {
+                load_floats(a.q, src, a.float_type, call.wide != 0, v);
+            }
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < D / 4; ++i) {
-                v[i] = r < rows ? load_float(a.q, src + i, a.float_type) : 0.0f;
                 top = max(top, magnitude_bits(v[i]));
             }
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
@@ -357,50 +427,49 @@ attention_i8_rows_kernel(const RowsCall call)
             const int idx = off + warp + i * kRowsWarps;
             return idx < work.sink_groups ? idx : idx - work.sink_groups + work.first_group;
         };
-        int ahead_page = -1;           // lane i: of group (32-block of the next one to issue) + i
-        float ahead_k = 0.0f, ahead_v = 0.0f;
+        // Lane i has the i-th of 32 groups at a time: where its codes lie (-1: nowhere), its scales; and asks for them when their turn comes.
+        int64_t ahead = -1;
+        float ahead_k = 0.0f, ahead_log2 = 0.0f, ahead_inv = 0.0f;
         const auto issue = [&](int i) {
             if ((i & 31) == 0) {
-                ahead_page = -1;
-                if (i + lane < mine && group_of(i + lane) * 16 < work.s.len) {
-                    ahead_page = page_at(a.cache, seq, group_of(i + lane) * 16 / static_cast<int>(a.cache.page_tokens), call.error_word);
-                    if (ahead_page >= 0) {
-                        const int64_t s = ahead_page * a.cache.scale_page_stride + head;
+                ahead = -1;
+                const int key0 = group_of(i + lane) * 16;
+                if (i + lane < mine && key0 < work.s.len) {
+                    const int page = page_at(a.cache, seq, key0 >> call.page_shift, call.error_word);
+                    if (page >= 0) {
+                        const int64_t s = page * a.cache.scale_page_stride + head;
+                        const float vs = a.cache.v_scale[s], sure = vs < kLeastCacheScale ? kLeastCacheScale : vs;
                         ahead_k = a.cache.k_scale[s];
-                        ahead_v = a.cache.v_scale[s];
+                        ahead_log2 = log2f(sure);
+                        ahead_inv = __fdiv_rn(1.0f, sure);
+                        ahead = page * a.cache.page_stride +
+                                ((static_cast<int64_t>(head) << call.page_shift) + (key0 & ((1 << call.page_shift) - 1))) * D;
                     }
                 }
             }
-            const int page = __shfl_sync(0xFFFFFFFFu, ahead_page, i & 31);
-            const float ks = __shfl_sync(0xFFFFFFFFu, ahead_k, i & 31), vs = __shfl_sync(0xFFFFFFFFu, ahead_v, i & 31);
-            if (lane == 0) {
-                const uint32_t slot = issued % kStages;
-                const float sure = vs < kLeastCacheScale ? kLeastCacheScale : vs;
-                scales[warp][slot] = StageScales{ks, log2f(sure), __fdiv_rn(1.0f, sure), page >= 0 ? 1 : 0};
-                if (page >= 0) {
-                    uint8_t* dst = my_ring + slot * Shared::kStageBytes;
-                    const int64_t src = page * a.cache.page_stride +
-                                        (static_cast<int64_t>(head) * a.cache.page_tokens + group_of(i) * 16 % static_cast<int>(a.cache.page_tokens)) * D;
-                    mbar_expect_tx(&full[warp][slot], Shared::kStageBytes);
-                    bulk_load_1d(dst, static_cast<const uint8_t*>(a.cache.k) + src, 16 * D, &full[warp][slot]);
-                    bulk_load_1d(dst + 16 * D, static_cast<const uint8_t*>(a.cache.v) + src, 16 * D, &full[warp][slot]);
+            if (lane == (i & 31)) {
+                uint64_t* const bar = &full[warp][issue_slot];
+                scales[warp][issue_slot] = StageScales{ahead_k, ahead_log2, ahead_inv, ahead >= 0 ? 1 : 0};
+                if (ahead >= 0) {
+                    uint8_t* const dst = my_ring + issue_slot * Shared::kStageBytes;
+                    mbar_expect_tx(bar, Shared::kStageBytes);
+                    bulk_load_1d(dst, static_cast<const uint8_t*>(a.cache.k) + ahead, 16 * D, bar);
+                    bulk_load_1d(dst + 16 * D, static_cast<const uint8_t*>(a.cache.v) + ahead, 16 * D, bar);
                 } else {
-                    mbar_arrive(&full[warp][slot]);
+                    mbar_arrive(bar);
                 }
             }
             ++issued;
+            issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
         };
         for (int i = 0; i < min(mine, kStages); ++i) {
             issue(i);
         }
         for (int i = 0; i < mine; ++i) {
-            const uint32_t slot = taken % kStages;
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[warp][slot], taken / kStages & 1u, &abort_flag))) {
+            if (!wait_every_lane(&full[warp][slot], round, &abort_flag)) {
                 failed = true;
                 break;
             }
-            ++taken;
-            __syncwarp();
             const StageScales sc = scales[warp][slot];
             if (sc.there != 0) {
                 const uint8_t* kp = my_ring + slot * Shared::kStageBytes;
@@ -435,53 +504,61 @@ attention_i8_rows_kernel(const RowsCall call)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     // Element e: token g (e < 2) or g + 8, column 2 c + (e & 1).
-                    float inv[4] = {sc.v_inv, sc.v_inv, sc.v_inv, sc.v_inv};
+                    const float kf[2] = {sc.k * factor[nt][0], sc.k * factor[nt][1]};
+                    const float less[2] = {sc.v_log2 - m[nt][0], sc.v_log2 - m[nt][1]};   // +infinity until a row has seen something
+                    float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        s[nt][e] = __fmaf_rn(s[nt][e], sc.k * factor[nt][e & 1], sc.v_log2);
+                        x[e] = __fmaf_rn(s[nt][e], kf[e & 1], less[e & 1]);
                     }
+                    bool seen[4] = {true, true, true, true};
                     if (!all_seen) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int key = key0 + g + (e < 2 ? 0 : 8), at_pos = pos[nt][e & 1];
-                            const bool seen = key < work.s.len && key <= at_pos && (a.window == 0 || key > at_pos - a.window || key < a.sinks);
-                            s[nt][e] = seen ? s[nt][e] : -INFINITY;
-                            inv[e] = seen ? inv[e] : 0.0f;
+                            seen[e] = key < work.s.len && key <= at_pos && (a.window == 0 || key > at_pos - a.window || key < a.sinks);
+                            x[e] = seen[e] ? x[e] : -INFINITY;
                         }
                     }
-                    float alpha[2];
-                    bool grown = false;
+                    if (__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kGrowth)) {
+                        float alpha[2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float top = fmaxf(s[nt][j], s[nt][j + 2]);
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                        const float next = fmaxf(m[nt][j], top);
-                        const float safe = next == -INFINITY ? 0.0f : next;
-                        grown = grown || next > m[nt][j];
-                        alpha[j] = exp2_fast(m[nt][j] - safe);
-                        m[nt][j] = next;
-                        s[nt][j] = exp2_fast(s[nt][j] - safe);
-                        s[nt][j + 2] = exp2_fast(s[nt][j + 2] - safe);
-                        l[nt][j] = __fmaf_rn(s[nt][j + 2], inv[j + 2], __fmaf_rn(s[nt][j], inv[j], l[nt][j] * alpha[j]));
-                    }
-                    if (__any_sync(0xFFFFFFFFu, grown)) {
+                        for (int j = 0; j < 2; ++j) {
+                            const float t0 = seen[j] ? __fmaf_rn(s[nt][j], kf[j], sc.v_log2) : -INFINITY;
+                            const float t1 = seen[j + 2] ? __fmaf_rn(s[nt][j + 2], kf[j], sc.v_log2) : -INFINITY;
+                            float top = fmaxf(t0, t1);
+                            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                            const float next = fmaxf(m[nt][j], top), safe = next == -INFINITY ? 0.0f : next;
+                            alpha[j] = exp2_fast(m[nt][j] - safe);
+                            m[nt][j] = next;
+                            l[nt][j] *= alpha[j];
+                            x[j] = t0 - safe;
+                            x[j + 2] = t1 - safe;
+                        }
 #pragma unroll
-                        for (int i2 = 0; i2 < D / 16; ++i2) {
-                            o[nt][i2][0] *= alpha[0];
-                            o[nt][i2][1] *= alpha[1];
-                            o[nt][i2][2] *= alpha[0];
-                            o[nt][i2][3] *= alpha[1];
+                        for (int d = 0; d < D / 16; ++d) {
+                            o[nt][d][0] *= alpha[0];
+                            o[nt][d][1] *= alpha[1];
+                            o[nt][d][2] *= alpha[0];
+                            o[nt][d][3] *= alpha[1];
                         }
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const __half2 h = __floats2half2_rn(s[nt][2 * j], s[nt][2 * j + 1]);
+                        x[j] = exp2_fast(x[j]);
+                        x[j + 2] = exp2_fast(x[j + 2]);
+                        const float both = x[j] + x[j + 2];
+                        l[nt][j] += both == 0.0f ? 0.0f : both * sc.v_inv;   // (not 0 times what a block that is masked has for a scale)
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
                         pb[nt][0][j] = transposed_8x8(*reinterpret_cast<const uint32_t*>(&h));
                         if constexpr (SPLIT) {
                             const float2 f = __half22float2(h);
-                            pb[nt][kParts - 1][j] = transposed_8x8(pack2<__half>(s[nt][2 * j] - f.x, s[nt][2 * j + 1] - f.y));
+                            pb[nt][kParts - 1][j] = transposed_8x8(pack2<__half>(x[2 * j] - f.x, x[2 * j + 1] - f.y));
                         }
                     }
                 }
@@ -509,6 +586,10 @@ attention_i8_rows_kernel(const RowsCall call)
             if (i + kStages < mine) {
                 issue(i + kStages);
             }
+            if (++slot == kStages) {
+                slot = 0;
+                round ^= 1;
+            }
         }
         if (failed) {
             if (lane == 0) {
@@ -517,7 +598,6 @@ attention_i8_rows_kernel(const RowsCall call)
                     atomicCAS(call.error_word, 0, kErrDrainWait);
                 }
             }
-            taken = issued;
             __syncwarp();
         }
 
@@ -572,12 +652,7 @@ attention_i8_rows_kernel(const RowsCall call)
             }
             if (begins && ends) {
                 const int global = tile * kTile + r;
-                const int64_t dst = (work.s.row0 + global / call.group) * a.out_stride_row + (head * call.group + global % call.group) * a.out_stride_head + d;
-                const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-                store_float(a.out, dst, a.float_type, sum.x * inv);
-                store_float(a.out, dst + 1, a.float_type, sum.y * inv);
-                store_float(a.out, dst + 2, a.float_type, sum.z * inv);
-                store_float(a.out, dst + 3, a.float_type, sum.w * inv);
+                store_row(call, (work.s.row0 + global / call.group) * a.out_stride_row + (head * call.group + global % call.group) * a.out_stride_head + d, sum, total);
             } else {
                 *reinterpret_cast<float4*>(piece + r * D + d) = sum;
                 if (d == 0) {
@@ -612,40 +687,61 @@ __global__ void __launch_bounds__(kRowsThreads) attention_i8_join_kernel(const R
     const nnb200_attention_i8_args& a = call.a;
     const SequenceRows s = sequence_rows(a.cache, mine.seq);
     const int rows = min(TILE, s.n * call.group - mine.tile * TILE);
-    int last = blockIdx.x + 1;
-    while (last < static_cast<int>(gridDim.x) - 1 && call.pieces[2 * last].kind == 2) {
-        ++last;
+    // How many blocks on it ends, everybody looking at once.
+    __shared__ int ends;
+    if (threadIdx.x == 0) {
+        ends = 0x7FFFFFFF;
     }
+    __syncthreads();
+    for (int p = blockIdx.x + 1 + threadIdx.x; p < static_cast<int>(gridDim.x); p += kRowsThreads) {
+        if (call.pieces[2 * p].kind == 3) {
+            atomicMin(&ends, p - static_cast<int>(blockIdx.x));
+            break;
+        }
+    }
+    __syncthreads();
+    const int more = min(ends, static_cast<int>(gridDim.x - blockIdx.x) - 1);
     constexpr int64_t kPiece = TILE * (D + 2);
     const float* first = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kPiece;
-    const float* rest = call.sums + 2 * static_cast<int64_t>(blockIdx.x + 1) * kPiece;   // and every second piece from there
-    const int more = last - static_cast<int>(blockIdx.x);
+    const float* rest = first + kPiece;   // and every second piece from there
     for (int i = threadIdx.x; i < rows * (D / 4); i += kRowsThreads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = first[TILE * D + r];
-        for (int p = 0; p < more; ++p) {
-            top = fmaxf(top, rest[p * 2 * kPiece + TILE * D + r]);
-        }
-        const float safe = top == -INFINITY ? 0.0f : top;
-        float total = 0.0f;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = -1; p < more; ++p) {
-            const float* piece = p < 0 ? first : rest + p * 2 * kPiece;
-            const float share = exp2_fast(piece[TILE * D + r] - safe);
-            const float4 v = *reinterpret_cast<const float4*>(piece + r * D + d);
-            total = __fmaf_rn(piece[TILE * D + TILE + r], share, total);
-            sum.x = __fmaf_rn(v.x, share, sum.x);
-            sum.y = __fmaf_rn(v.y, share, sum.y);
-            sum.z = __fmaf_rn(v.z, share, sum.z);
-            sum.w = __fmaf_rn(v.w, share, sum.w);
+        float top = first[TILE * D + r], total = first[TILE * D + TILE + r];
+        float4 sum = *reinterpret_cast<const float4*>(first + r * D + d);
+        constexpr int kAtOnce = 8;
+        for (int p0 = 0; p0 < more; p0 += kAtOnce) {
+            float m[kAtOnce], l[kAtOnce];
+            float4 v[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const float* piece = rest + min(p0 + k, more - 1) * 2 * kPiece;
+                m[k] = p0 + k < more ? piece[TILE * D + r] : -INFINITY;
+                l[k] = piece[TILE * D + TILE + r];
+                v[k] = *reinterpret_cast<const float4*>(piece + r * D + d);
+            }
+            float next = top;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                next = fmaxf(next, m[k]);
+            }
+            const float safe = next == -INFINITY ? 0.0f : next, old = exp2_fast(top - safe);
+            top = next;
+            total *= old;
+            sum = make_float4(sum.x * old, sum.y * old, sum.z * old, sum.w * old);
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (p0 + k < more) {
+                    const float share = exp2_fast(m[k] - safe);
+                    total = __fmaf_rn(l[k], share, total);
+                    sum.x = __fmaf_rn(v[k].x, share, sum.x);
+                    sum.y = __fmaf_rn(v[k].y, share, sum.y);
+                    sum.z = __fmaf_rn(v[k].z, share, sum.z);
+                    sum.w = __fmaf_rn(v[k].w, share, sum.w);
+                }
+            }
         }
         const int global = mine.tile * TILE + r;
-        const int64_t dst = (s.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d;
-        const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-        store_float(a.out, dst, a.float_type, sum.x * inv);
-        store_float(a.out, dst + 1, a.float_type, sum.y * inv);
-        store_float(a.out, dst + 2, a.float_type, sum.z * inv);
-        store_float(a.out, dst + 3, a.float_type, sum.w * inv);
+        store_row(call, (s.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d, sum, total);
     }
 }
 

@@ -339,28 +339,6 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
     return r;
 }
 
-// Every lane polls: the data behind the barrier is then every lane's.  Without a hint how long to sleep, which costs a
-// hundred cycles on a barrier that is all but ready; within the limit that mbar_wait has.
-__device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
-{
-    bool done = mbar_try_wait(bar, parity);
-    if (!__all_sync(0xFFFFFFFFu, done)) {
-        const long long t0 = clock64();
-        bool give_up = false;
-        for (uint32_t spins = 1; !done && !give_up; ++spins) {
-            done = mbar_try_wait(bar, parity);
-            if ((spins & 63u) == 0) {
-                if (*abort_flag == 0 && clock64() - t0 > kWaitLimitCycles) {
-                    *abort_flag = 1;
-                }
-                give_up = *abort_flag != 0;
-            }
-        }
-        return __all_sync(0xFFFFFFFFu, done);
-    }
-    return true;
-}
-
 // The same in every lane, and in a uniform register: what a reduction gives is, what a shuffle gives is not.
 __device__ __forceinline__ uint32_t in_uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
 
@@ -541,7 +519,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 load_queries();
             }
             if (pending) {
-                if (!tile_wait(&o_full[half][kParts - 1], (n - 1) & 1, &abort_flag)) {
+                if (!wait_every_lane(&o_full[half][kParts - 1], (n - 1) & 1, &abort_flag)) {
                     ok = false;
                     break;
                 }
@@ -603,8 +581,8 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 const int part = i % kParts;
                 const uint32_t part_addr = s_addr + static_cast<uint32_t>(part * kPartKeys);
                 if (part == 0) {
-                    ok = tile_wait(&s_full[half], n & 1, &abort_flag) &&
-                         tile_wait(&meta_full[n % kMetaSlots], n / kMetaSlots & 1, &abort_flag);   // long since: the products waited for it
+                    ok = wait_every_lane(&s_full[half], n & 1, &abort_flag) &&
+                         wait_every_lane(&meta_full[n % kMetaSlots], n / kMetaSlots & 1, &abort_flag);   // long since: the products waited for it
                     if (!ok) {
                         break;
                     }
@@ -670,7 +648,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                     l *= alpha;
                     if (i > 0) {
                         // The sums so far are complete: the next part's products wait for this one's weights.
-                        if (!tile_wait(&o_full[half][(part + kParts - 1) % kParts], (part == 0 ? n - 1 : n) & 1, &abort_flag)) {
+                        if (!wait_every_lane(&o_full[half][(part + kParts - 1) % kParts], (part == 0 ? n - 1 : n) & 1, &abort_flag)) {
                             ok = false;
                             break;
                         }
@@ -773,7 +751,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 store_codes<D>(tile, idx / (D / 16), idx % (D / 16), *reinterpret_cast<const uint4*>(my_codes + slot * Shared::kUnitBytes + i * 2048));
             }
         };
-        bool ok = tile_wait(&meta_full[0], 0, &abort_flag);
+        bool ok = wait_every_lane(&meta_full[0], 0, &abort_flag);
         bool more = ok && (state[0] & kBlockNone) == 0;
         if (more) {
             load(a.cache.k, 0, 0, 0);
@@ -782,8 +760,8 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         for (uint32_t n = 0; more; ++n) {
             const uint32_t slot = n % kStages, round = n / kStages & 1;
             const bool next = (state[n % kMetaSlots] & kBlockLast) == 0;
-            ok = tile_wait(&k_empty[slot], round ^ 1, &abort_flag) &&
-                 (!next || tile_wait(&meta_full[(n + 1) % kMetaSlots], (n + 1) / kMetaSlots & 1, &abort_flag));
+            ok = wait_every_lane(&k_empty[slot], round ^ 1, &abort_flag) &&
+                 (!next || wait_every_lane(&meta_full[(n + 1) % kMetaSlots], (n + 1) / kMetaSlots & 1, &abort_flag));
             if (!ok) {
                 break;
             }
@@ -800,7 +778,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             }
             fence_proxy_async_smem();
             mbar_arrive(&k_full[slot]);
-            ok = tile_wait(&v_empty[slot], round ^ 1, &abort_flag);
+            ok = wait_every_lane(&v_empty[slot], round ^ 1, &abort_flag);
             if (!ok) {
                 break;
             }
@@ -958,7 +936,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 // A scale below zero turns the order of its scores round: those too are looked at one by one.
                 const int odd = __reduce_or_sync(0xFFFFFFFFu, (of.key0 & 3) | (of.k * call.factor < 0.0f ? 3 : 0));
                 const uint32_t slot = n % kMetaSlots;
-                if (!tile_wait(&meta_empty[slot], (n / kMetaSlots & 1) ^ 1, &abort_flag)) {
+                if (!wait_every_lane(&meta_empty[slot], (n / kMetaSlots & 1) ^ 1, &abort_flag)) {
                     ok = false;
                     break;
                 }
