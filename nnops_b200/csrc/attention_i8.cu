@@ -29,17 +29,19 @@ int engine_of(const nnb200_attention_i8_args& a)
     return a.force_engine != 0 ? a.force_engine : rows_each(a) > 64 ? kEngineTile : kEngineRows;
 }
 
-// Tiles of 8, 16 or 32 query rows: as many as a sequence has.  A wider tile reads the codes for more rows at once and holds
-// more sums in registers (head size 256 and f32 rows: 16 at most).
+// Tiles of 8 to 32 query rows: as many as a sequence has, or the widest.  A wider tile reads the codes for more rows at once
+// and holds more sums in registers (head size 256 and f32 rows: 16 at most).
 RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
 {
     const nnb200_cache_i8& c = a.cache;
     const int64_t rows = rows_each(a);
     RowsPlan p;
-    p.columns = rows <= 8 ? 1 : (rows <= 16 || c.dim > 128 || a.float_type == NNB200_FLOAT_F32) ? 2 : 4;
-    p.blocks = dev.sm_count * (p.columns == 1 && c.dim <= 128 ? 2 : 1);
-    const size_t pieces = 2 * static_cast<size_t>(p.blocks);
-    p.bytes = pieces * (sizeof(RowsPiece) + static_cast<size_t>(8 * p.columns) * static_cast<size_t>(c.dim + 2) * sizeof(float));
+    const int most = c.dim > 128 || a.float_type == NNB200_FLOAT_F32 ? 2 : 4;
+    const int64_t tiles = (rows + 8 * most - 1) / (8 * most);
+    p.columns = static_cast<int>((rows + 8 * tiles - 1) / (8 * tiles));
+    p.blocks = dev.sm_count * rows_blocks(c.dim, p.columns);
+    const size_t blocks = static_cast<size_t>(p.blocks);
+    p.bytes = blocks * (sizeof(RowsPiece) + 2 * static_cast<size_t>(8 * p.columns) * static_cast<size_t>(c.dim + 2) * sizeof(float));
     return p;
 }
 
@@ -80,7 +82,7 @@ int run_rows(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.wide_out = multiple(a.out, 128 / per / 2, a.out_stride_row, a.out_stride_head, 4);
     call.page_shift = page_shift(a);
     call.pieces = static_cast<RowsPiece*>(a.workspace);
-    call.sums = reinterpret_cast<float*>(call.pieces + 2 * static_cast<size_t>(p.blocks));
+    call.sums = reinterpret_cast<float*>(call.pieces + p.blocks);
     switch (a.cache.dim) {
     case 64: return cuda_status(launch_attention_rows_64(call, p.columns, p.blocks, stream));
     case 96: return cuda_status(launch_attention_rows_96(call, p.columns, p.blocks, stream));

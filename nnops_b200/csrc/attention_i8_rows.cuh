@@ -34,11 +34,15 @@ constexpr int kRowsThreads = 32 * kRowsWarps;
 constexpr int kRowsCost = 16;     // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
 constexpr float kGrowth = 8.0f;   // log2 of what a weight may be
 
-// What a block leaves in the workspace: [0] the end or the middle of a row tile that began in an earlier
-// block, [1] the beginning of one that ends in a later block.
+// A row tile of a head that begins in a block and ends in a later one.  What a block leaves of its sums: [0] the end or the middle of
+// one that began in an earlier block, [1] the beginning of one that ends in a later block.
 struct RowsPiece {
-    int32_t kind;      // 0: nothing, 1: begins here, 2: neither begins nor ends, 3: ends
-    int32_t seq, head, tile;
+    int32_t more;    // blocks behind this one that have a part of it; 0: nothing begins here that does not end here
+    int32_t head;
+    int32_t row0;    // the sequence's first row
+    int32_t first;   // of the sequence's rows times heads of the group
+    int32_t rows;
+    int32_t unused[3];
 };
 
 struct RowsPlan {
@@ -55,7 +59,7 @@ struct RowsCall {
     int wide;            // q's rows and heads are 16-byte aligned
     int wide_out;        // out's are, to four values
     int page_shift;      // log2 of the tokens of a page
-    RowsPiece* pieces;   // [blocks][2]
+    RowsPiece* pieces;   // [blocks]
     float* sums;         // [blocks][2][piece]
 };
 
@@ -226,15 +230,18 @@ __device__ __forceinline__ bool wait_every_lane(uint64_t* bar, uint32_t parity, 
 }
 
 // Bytes of shared memory: the warps' rings, which hold the warps' sums when a piece is joined; barriers; per-stage scales.
+// Blocks on an SM: two where their registers and rings have room.
+constexpr int rows_blocks(int64_t dim, int columns) { return dim == 64 ? (columns <= 3 ? 2 : 1) : dim <= 128 && columns == 1 ? 2 : 1; }
+
 template <int D, int NT>
 struct RowsShared {
     static constexpr int kStageBytes = 2 * 16 * D;
     static constexpr int kJoinBytes = kRowsWarps * 8 * NT * D * 4;
-    static constexpr int kWanted = NT == 1 && D <= 128 ? 96 * 1024 : 192 * 1024;
+    static constexpr int kWanted = (rows_blocks(D, NT) == 2 ? 96 : 192) * 1024;
     static constexpr int kStages = kWanted / (kRowsWarps * kStageBytes) > 8 ? 8 : kWanted / (kRowsWarps * kStageBytes);
     static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
     static constexpr int kBytes = kRing > kJoinBytes ? kRing : kJoinBytes;
-    static_assert(kStages >= 2 && kBytes <= 200 * 1024, "ring");
+    static_assert(kStages >= 2 && rows_blocks(D, NT) * kBytes <= 200 * 1024, "ring");
 };
 
 struct StageScales {
@@ -243,7 +250,7 @@ struct StageScales {
 };
 
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kRowsThreads, (NT == 1 && D <= 128) ? 2 : 1)
+__global__ void __launch_bounds__(kRowsThreads, rows_blocks(D, NT))
 attention_i8_rows_kernel(const RowsCall call)
 {
     using Shared = RowsShared<D, NT>;
@@ -294,44 +301,51 @@ attention_i8_rows_kernel(const RowsCall call)
         }
         return before;
     };
-    int64_t line = 0;
+    // Up to so many threads: everyone has its own sequence's place at once.
+    int64_t line = 0, own = 0, own_before = 0;
     for (int b0 = 0; b0 < seqs; b0 += kRowsThreads) {
         const int b = b0 + static_cast<int>(threadIdx.x);
         int64_t total;
-        (void)block_sum_before(b < seqs ? sequence_work(call, b, kTile).total : 0, total);
+        own = b < seqs ? sequence_work(call, b, kTile).total : 0;
+        own_before = line + block_sum_before(own, total);
         line += total;
     }
-    // No fewer than a group a warp for a block, besides what an item costs.
-    const int64_t share_at_least = kRowsWarps + kRowsCost;
+    // No fewer than a group a warp for a block, besides half of what an item costs.
+    const int64_t share_at_least = kRowsWarps + kRowsCost / 2;
     const int64_t most = (line + share_at_least - 1) / share_at_least;
     const int64_t blocks = most < gridDim.x ? most : gridDim.x;
-    RowsPiece* pieces = call.pieces + 2 * blockIdx.x;
+    if (threadIdx.x == 0) {
+        call.pieces[blockIdx.x].more = 0;
+    }
     if (static_cast<int64_t>(blockIdx.x) >= blocks) {
-        if (threadIdx.x < 2) {
-            pieces[threadIdx.x].kind = 0;
-        }
         return;
     }
-    int64_t at = line / blocks * blockIdx.x + line % blocks * blockIdx.x / blocks;
-    const int64_t end = line / blocks * (blockIdx.x + 1) + line % blocks * (blockIdx.x + 1) / blocks;
-    {
+    const int64_t share = line / blocks, over = line % blocks;
+    const auto start_of = [&](int64_t block) { return share * block + over * block / blocks; };
+    int64_t at = start_of(blockIdx.x);
+    const int64_t end = start_of(blockIdx.x + 1);
+    if (seqs <= kRowsThreads) {
+        if (own_before <= at && at < own_before + own) {
+            found_seq = threadIdx.x;
+            found_base = own_before;
+        }
+    } else {
         int64_t base = 0;
         for (int b0 = 0; b0 < seqs; b0 += kRowsThreads) {
             const int b = b0 + static_cast<int>(threadIdx.x);
-            const int64_t own = b < seqs ? sequence_work(call, b, kTile).total : 0;
+            own = b < seqs ? sequence_work(call, b, kTile).total : 0;
             int64_t total;
-            const int64_t first = base + block_sum_before(own, total);
-            if (first <= at && at < first + own) {
+            own_before = base + block_sum_before(own, total);
+            if (own_before <= at && at < own_before + own) {
                 found_seq = b;
-                found_base = first;
+                found_base = own_before;
             }
             base += total;
         }
-        __syncthreads();
     }
+    __syncthreads();
     int seq = found_seq;
     int64_t base = found_base;
-    int kinds[2] = {0, 0};
 
     uint32_t issued = 0;   // 16-token groups of this warp
     uint32_t issue_slot = 0, slot = 0, round = 0;   // of the ring: the next to fill, the next to take and its turn
@@ -359,6 +373,50 @@ attention_i8_rows_kernel(const RowsCall call)
         const int rows = min(kTile, work.s.n * call.group - tile * kTile);
         const int first_pos = work.s.len - work.s.n;
 
+        // This warp's groups of the piece: off + warp, off + warp + 8, ...
+        const int mine = count > warp ? (count - warp + kRowsWarps - 1) / kRowsWarps : 0;
+        const auto group_of = [&](int i) {
+            const int idx = off + warp + i * kRowsWarps;
+            return idx < work.sink_groups ? idx : idx - work.sink_groups + work.first_group;
+        };
+        // Lane i has the i-th of 32 groups at a time: where its codes lie (-1: nowhere), its scales; and asks for them when their turn comes.
+        int64_t ahead = -1;
+        float ahead_k = 0.0f, ahead_log2 = 0.0f, ahead_inv = 0.0f;
+        const auto issue = [&](int i) {
+            if ((i & 31) == 0) {
+                ahead = -1;
+                const int key0 = group_of(i + lane) * 16;
+                if (i + lane < mine && key0 < work.s.len) {
+                    const int page = page_at(a.cache, seq, key0 >> call.page_shift, call.error_word);
+                    if (page >= 0) {
+                        const int64_t s = page * a.cache.scale_page_stride + head;
+                        const float vs = a.cache.v_scale[s], sure = vs < kLeastCacheScale ? kLeastCacheScale : vs;
+                        ahead_k = a.cache.k_scale[s];
+                        ahead_log2 = log2f(sure);
+                        ahead_inv = __fdiv_rn(1.0f, sure);
+                        ahead = page * a.cache.page_stride +
+                                ((static_cast<int64_t>(head) << call.page_shift) + (key0 & ((1 << call.page_shift) - 1))) * D;
+                    }
+                }
+            }
+            if (lane == (i & 31)) {
+                uint64_t* const bar = &full[warp][issue_slot];
+                scales[warp][issue_slot] = StageScales{ahead_k, ahead_log2, ahead_inv, ahead >= 0 ? 1 : 0};
+                if (ahead >= 0) {
+                    uint8_t* const dst = my_ring + issue_slot * Shared::kStageBytes;
+                    mbar_expect_tx(bar, Shared::kStageBytes);
+                    bulk_load_1d(dst, static_cast<const uint8_t*>(a.cache.k) + ahead, 16 * D, bar);
+                    bulk_load_1d(dst + 16 * D, static_cast<const uint8_t*>(a.cache.v) + ahead, 16 * D, bar);
+                } else {
+                    mbar_arrive(bar);
+                }
+            }
+            ++issued;
+            issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
+        };
+        for (int i = 0; i < min(mine, kStages); ++i) {
+            issue(i);
+        }
         // This thread's part of the query rows: row 8 nt + g, dims [c D / 4, + D / 4), in f16 scaled by a power of two.
         uint32_t q[NT][kParts][D / 16][2];
         float factor[NT][2];    // of the columns 2 c and 2 c + 1
@@ -421,50 +479,6 @@ attention_i8_rows_kernel(const RowsCall call)
             }
         }
 
-        // This warp's groups of the piece: off + warp, off + warp + 8, ...
-        const int mine = count > warp ? (count - warp + kRowsWarps - 1) / kRowsWarps : 0;
-        const auto group_of = [&](int i) {
-            const int idx = off + warp + i * kRowsWarps;
-            return idx < work.sink_groups ? idx : idx - work.sink_groups + work.first_group;
-        };
-        // Lane i has the i-th of 32 groups at a time: where its codes lie (-1: nowhere), its scales; and asks for them when their turn comes.
-        int64_t ahead = -1;
-        float ahead_k = 0.0f, ahead_log2 = 0.0f, ahead_inv = 0.0f;
-        const auto issue = [&](int i) {
-            if ((i & 31) == 0) {
-                ahead = -1;
-                const int key0 = group_of(i + lane) * 16;
-                if (i + lane < mine && key0 < work.s.len) {
-                    const int page = page_at(a.cache, seq, key0 >> call.page_shift, call.error_word);
-                    if (page >= 0) {
-                        const int64_t s = page * a.cache.scale_page_stride + head;
-                        const float vs = a.cache.v_scale[s], sure = vs < kLeastCacheScale ? kLeastCacheScale : vs;
-                        ahead_k = a.cache.k_scale[s];
-                        ahead_log2 = log2f(sure);
-                        ahead_inv = __fdiv_rn(1.0f, sure);
-                        ahead = page * a.cache.page_stride +
-                                ((static_cast<int64_t>(head) << call.page_shift) + (key0 & ((1 << call.page_shift) - 1))) * D;
-                    }
-                }
-            }
-            if (lane == (i & 31)) {
-                uint64_t* const bar = &full[warp][issue_slot];
-                scales[warp][issue_slot] = StageScales{ahead_k, ahead_log2, ahead_inv, ahead >= 0 ? 1 : 0};
-                if (ahead >= 0) {
-                    uint8_t* const dst = my_ring + issue_slot * Shared::kStageBytes;
-                    mbar_expect_tx(bar, Shared::kStageBytes);
-                    bulk_load_1d(dst, static_cast<const uint8_t*>(a.cache.k) + ahead, 16 * D, bar);
-                    bulk_load_1d(dst + 16 * D, static_cast<const uint8_t*>(a.cache.v) + ahead, 16 * D, bar);
-                } else {
-                    mbar_arrive(bar);
-                }
-            }
-            ++issued;
-            issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
-        };
-        for (int i = 0; i < min(mine, kStages); ++i) {
-            issue(i);
-        }
         for (int i = 0; i < mine; ++i) {
             if (!wait_every_lane(&full[warp][slot], round, &abort_flag)) {
                 failed = true;
@@ -661,17 +675,20 @@ attention_i8_rows_kernel(const RowsCall call)
                 }
             }
         }
-        if (!(begins && ends)) {
-            kinds[which] = begins ? 1 : ends ? 3 : 2;
-            if (threadIdx.x == 0) {
-                pieces[which] = RowsPiece{kinds[which], seq, head, tile};
+        if (begins && !ends && threadIdx.x == 0) {
+            // The block in which it ends: the one that has the item's last place on the line.
+            const int64_t place = base + (item + 1) * length - 1;
+            int64_t block = place * blocks / line;
+            while (start_of(block + 1) <= place) {
+                ++block;
             }
+            while (start_of(block) > place) {
+                --block;
+            }
+            call.pieces[blockIdx.x] = RowsPiece{static_cast<int32_t>(block - blockIdx.x), head, work.s.row0, tile * kTile, rows, {}};
         }
         fence_proxy_async_smem();
         __syncthreads();
-    }
-    if (threadIdx.x < 2 && kinds[threadIdx.x] == 0) {
-        pieces[threadIdx.x].kind = 0;
     }
 }
 
@@ -680,27 +697,12 @@ template <int D, int TILE>
 __global__ void __launch_bounds__(kRowsThreads) attention_i8_join_kernel(const RowsCall call)
 {
     previous_kernel_done();
-    const RowsPiece mine = call.pieces[2 * blockIdx.x + 1];
-    if (mine.kind != 1) {
+    const RowsPiece mine = call.pieces[blockIdx.x];
+    const int more = mine.more, rows = mine.rows;
+    if (more == 0) {
         return;
     }
     const nnb200_attention_i8_args& a = call.a;
-    const SequenceRows s = sequence_rows(a.cache, mine.seq);
-    const int rows = min(TILE, s.n * call.group - mine.tile * TILE);
-    // How many blocks on it ends, everybody looking at once.
-    __shared__ int ends;
-    if (threadIdx.x == 0) {
-        ends = 0x7FFFFFFF;
-    }
-    __syncthreads();
-    for (int p = blockIdx.x + 1 + threadIdx.x; p < static_cast<int>(gridDim.x); p += kRowsThreads) {
-        if (call.pieces[2 * p].kind == 3) {
-            atomicMin(&ends, p - static_cast<int>(blockIdx.x));
-            break;
-        }
-    }
-    __syncthreads();
-    const int more = min(ends, static_cast<int>(gridDim.x - blockIdx.x) - 1);
     constexpr int64_t kPiece = TILE * (D + 2);
     const float* first = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + 1) * kPiece;
     const float* rest = first + kPiece;   // and every second piece from there
@@ -740,8 +742,8 @@ __global__ void __launch_bounds__(kRowsThreads) attention_i8_join_kernel(const R
                 }
             }
         }
-        const int global = mine.tile * TILE + r;
-        store_row(call, (s.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d, sum, total);
+        const int global = mine.first + r;
+        store_row(call, (mine.row0 + global / call.group) * a.out_stride_row + (mine.head * call.group + global % call.group) * a.out_stride_head + d, sum, total);
     }
 }
 
@@ -772,6 +774,9 @@ cudaError_t launch_rows_dim(const RowsCall& call, int columns, int blocks, cudaS
         return columns == 1 ? launch_rows<D, 1, true>(call, blocks, stream) : launch_rows<D, 2, true>(call, blocks, stream);
     }
     if constexpr (D <= 128) {
+        if (columns == 3) {
+            return launch_rows<D, 3, false>(call, blocks, stream);
+        }
         if (columns == 4) {
             return launch_rows<D, 4, false>(call, blocks, stream);
         }
