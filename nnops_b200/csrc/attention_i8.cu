@@ -29,17 +29,18 @@ int engine_of(const nnb200_attention_i8_args& a)
     return a.force_engine != 0 ? a.force_engine : rows_each(a) > 64 ? kEngineTile : kEngineRows;
 }
 
-// Tiles of 8 to 32 query rows: as many as a sequence has, or the widest.  A wider tile reads the codes for more rows at once
-// and holds more sums in registers (head size 256 and f32 rows: 16 at most).
+// Tiles of 8 to 32 query rows: as few of them as a sequence needs, all as wide.  A wider tile reads the codes for more rows at once
+// and holds more sums in registers.
 RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
 {
     const nnb200_cache_i8& c = a.cache;
     const int64_t rows = rows_each(a);
     RowsPlan p;
-    const int most = c.dim > 128 || a.float_type == NNB200_FLOAT_F32 ? 2 : 4;
+    const bool split = a.float_type == NNB200_FLOAT_F32;
+    const int most = rows_most_columns(c.dim, split);
     const int64_t tiles = (rows + 8 * most - 1) / (8 * most);
     p.columns = static_cast<int>((rows + 8 * tiles - 1) / (8 * tiles));
-    p.blocks = dev.sm_count * rows_blocks(c.dim, p.columns);
+    p.blocks = dev.sm_count * rows_blocks(c.dim, p.columns, split);
     const size_t blocks = static_cast<size_t>(p.blocks);
     p.bytes = blocks * (sizeof(RowsPiece) + 2 * static_cast<size_t>(8 * p.columns) * static_cast<size_t>(c.dim + 2) * sizeof(float));
     return p;

@@ -29,9 +29,8 @@
 
 namespace nnb200 {
 
-constexpr int kRowsWarps = 8;
-constexpr int kRowsThreads = 32 * kRowsWarps;
-constexpr int kRowsCost = 16;     // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
+constexpr int kRowsThreads = 256; // of the joining kernel's blocks
+constexpr int kRowsCost = 16;         // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
 constexpr float kGrowth = 8.0f;   // log2 of what a weight may be
 
 // A row tile of a head that begins in a block and ends in a later one.  What a block leaves of its sums: [0] the end or the middle of
@@ -230,18 +229,29 @@ __device__ __forceinline__ bool wait_every_lane(uint64_t* bar, uint32_t parity, 
 }
 
 // Bytes of shared memory: the warps' rings, which hold the warps' sums when a piece is joined; barriers; per-stage scales.
-// Blocks on an SM: two where their registers and rings have room.
-constexpr int rows_blocks(int64_t dim, int columns) { return dim == 64 ? (columns <= 3 ? 2 : 1) : dim <= 128 && columns == 1 ? 2 : 1; }
+// What a warp's queries and sums take, in values a lane has 32nd parts of; and by that blocks on an SM and warps of a block: 16 warps with
+// 128 registers a thread, 12 with 168 or 8 with 255.
+constexpr int rows_weight(int64_t dim, int columns, bool split) { return static_cast<int>(dim) * columns * (split ? 3 : 2) / 2; }
+constexpr int rows_blocks(int64_t dim, int columns, bool split) { return columns == 1 && rows_weight(dim, columns, split) <= 128 ? 2 : 1; }
+constexpr int rows_warps(int64_t dim, int columns, bool split)
+{
+    return rows_blocks(dim, columns, split) == 1 && rows_weight(dim, columns, split) <= 192 ? 12 : 8;
+}
 
-template <int D, int NT>
+// Beyond these the sums no longer fit the registers.
+constexpr int rows_most_columns(int64_t dim, bool split) { return split ? (dim > 128 ? 1 : 2) : dim > 128 ? 2 : dim > 96 ? 3 : 4; }
+
+template <int D, int NT, bool SPLIT>
 struct RowsShared {
+    static constexpr int kWarps = rows_warps(D, NT, SPLIT);
+    static constexpr int kThreads = 32 * kWarps;
     static constexpr int kStageBytes = 2 * 16 * D;
-    static constexpr int kJoinBytes = kRowsWarps * 8 * NT * D * 4;
-    static constexpr int kWanted = (rows_blocks(D, NT) == 2 ? 96 : 192) * 1024;
-    static constexpr int kStages = kWanted / (kRowsWarps * kStageBytes) > 8 ? 8 : kWanted / (kRowsWarps * kStageBytes);
-    static constexpr int kRing = kRowsWarps * kStages * kStageBytes;
+    static constexpr int kJoinBytes = kWarps * 8 * NT * D * 4;
+    static constexpr int kWanted = (rows_blocks(D, NT, SPLIT) == 2 ? 96 : 192) * 1024;
+    static constexpr int kStages = kWanted / (kWarps * kStageBytes) > 8 ? 8 : kWanted / (kWarps * kStageBytes);
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kBytes = kRing > kJoinBytes ? kRing : kJoinBytes;
-    static_assert(kStages >= 2 && rows_blocks(D, NT) * kBytes <= 200 * 1024, "ring");
+    static_assert(kStages >= 2 && rows_blocks(D, NT, SPLIT) * kBytes <= 200 * 1024, "ring");
 };
 
 struct StageScales {
@@ -250,18 +260,18 @@ struct StageScales {
 };
 
 template <int D, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kRowsThreads, rows_blocks(D, NT))
+__global__ void __launch_bounds__(RowsShared<D, NT, SPLIT>::kThreads, rows_blocks(D, NT, SPLIT))
 attention_i8_rows_kernel(const RowsCall call)
 {
-    using Shared = RowsShared<D, NT>;
-    constexpr int kStages = Shared::kStages;
+    using Shared = RowsShared<D, NT, SPLIT>;
+    constexpr int kStages = Shared::kStages, kWarps = Shared::kWarps, kThreads = Shared::kThreads;
     constexpr int kTile = 8 * NT;
     constexpr int kParts = SPLIT ? 2 : 1;
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ __align__(8) uint64_t full[kRowsWarps][kStages];
-    __shared__ StageScales scales[kRowsWarps][kStages];
-    __shared__ float join_m[kRowsWarps][kTile], join_l[kRowsWarps][kTile];
-    __shared__ int64_t scan[kRowsWarps + 1];
+    __shared__ __align__(8) uint64_t full[kWarps][kStages];
+    __shared__ StageScales scales[kWarps][kStages];
+    __shared__ float join_m[kWarps][kTile], join_l[kWarps][kTile];
+    __shared__ int64_t scan[kWarps + 1];
     __shared__ int64_t found_base;
     __shared__ int found_seq;
     __shared__ int abort_flag;
@@ -270,7 +280,7 @@ attention_i8_rows_kernel(const RowsCall call)
     const int g = lane / 4, c = lane & 3;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int i = 0; i < kRowsWarps * kStages; ++i) {
+        for (int i = 0; i < kWarps * kStages; ++i) {
             mbar_init(&full[0][0] + i, 1);
         }
         mbar_init_fence();
@@ -295,7 +305,7 @@ attention_i8_rows_kernel(const RowsCall call)
         __syncthreads();
         int64_t before = up - v;
         total = 0;
-        for (int i = 0; i < kRowsWarps; ++i) {
+        for (int i = 0; i < kWarps; ++i) {
             before += i < warp ? scan[i] : 0;
             total += scan[i];
         }
@@ -303,7 +313,7 @@ attention_i8_rows_kernel(const RowsCall call)
     };
     // Up to so many threads: everyone has its own sequence's place at once.
     int64_t line = 0, own = 0, own_before = 0;
-    for (int b0 = 0; b0 < seqs; b0 += kRowsThreads) {
+    for (int b0 = 0; b0 < seqs; b0 += kThreads) {
         const int b = b0 + static_cast<int>(threadIdx.x);
         int64_t total;
         own = b < seqs ? sequence_work(call, b, kTile).total : 0;
@@ -311,7 +321,7 @@ attention_i8_rows_kernel(const RowsCall call)
         line += total;
     }
     // No fewer than a group a warp for a block, besides half of what an item costs.
-    const int64_t share_at_least = kRowsWarps + kRowsCost / 2;
+    const int64_t share_at_least = kWarps + kRowsCost / 2;
     const int64_t most = (line + share_at_least - 1) / share_at_least;
     const int64_t blocks = most < gridDim.x ? most : gridDim.x;
     if (threadIdx.x == 0) {
@@ -324,14 +334,14 @@ attention_i8_rows_kernel(const RowsCall call)
     const auto start_of = [&](int64_t block) { return share * block + over * block / blocks; };
     int64_t at = start_of(blockIdx.x);
     const int64_t end = start_of(blockIdx.x + 1);
-    if (seqs <= kRowsThreads) {
+    if (seqs <= kThreads) {
         if (own_before <= at && at < own_before + own) {
             found_seq = threadIdx.x;
             found_base = own_before;
         }
     } else {
         int64_t base = 0;
-        for (int b0 = 0; b0 < seqs; b0 += kRowsThreads) {
+        for (int b0 = 0; b0 < seqs; b0 += kThreads) {
             const int b = b0 + static_cast<int>(threadIdx.x);
             own = b < seqs ? sequence_work(call, b, kTile).total : 0;
             int64_t total;
@@ -374,9 +384,9 @@ attention_i8_rows_kernel(const RowsCall call)
         const int first_pos = work.s.len - work.s.n;
 
         // This warp's groups of the piece: off + warp, off + warp + 8, ...
-        const int mine = count > warp ? (count - warp + kRowsWarps - 1) / kRowsWarps : 0;
+        const int mine = count > warp ? (count - warp + kWarps - 1) / kWarps : 0;
         const auto group_of = [&](int i) {
-            const int idx = off + warp + i * kRowsWarps;
+            const int idx = off + warp + i * kWarps;
             return idx < work.sink_groups ? idx : idx - work.sink_groups + work.first_group;
         };
         // Lane i has the i-th of 32 groups at a time: where its codes lie (-1: nowhere), its scales; and asks for them when their turn comes.
@@ -644,18 +654,18 @@ attention_i8_rows_kernel(const RowsCall call)
         const bool begins = off == 0, ends = off + count == work.groups;
         const int which = begins ? 1 : 0;
         float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kTile * (D + 2));
-        for (int i = threadIdx.x; i < rows * (D / 4); i += kRowsThreads) {
+        for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             float top = join_m[0][r];
 #pragma unroll
-            for (int w = 1; w < kRowsWarps; ++w) {
+            for (int w = 1; w < kWarps; ++w) {
                 top = fmaxf(top, join_m[w][r]);
             }
             const float safe = top == -INFINITY ? 0.0f : top;
             float total = 0.0f;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) {
+            for (int w = 0; w < kWarps; ++w) {
                 const float share = exp2_fast(join_m[w][r] - safe);
                 const float4 v = *reinterpret_cast<const float4*>(join_o + (w * kTile + r) * D + d);
                 total = __fmaf_rn(join_l[w][r], share, total);
@@ -750,14 +760,14 @@ __global__ void __launch_bounds__(kRowsThreads) attention_i8_join_kernel(const R
 template <int D, int NT, bool SPLIT>
 cudaError_t launch_rows(const RowsCall& call, int blocks, cudaStream_t stream)
 {
-    using Shared = RowsShared<D, NT>;
+    using Shared = RowsShared<D, NT, SPLIT>;
     const auto kernel = attention_i8_rows_kernel<D, NT, SPLIT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared::kBytes);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return e;
     }
-    e = launch_overlapping(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kRowsThreads), Shared::kBytes, stream, 1, call);
+    e = launch_overlapping(kernel, dim3(static_cast<unsigned>(blocks)), dim3(Shared::kThreads), Shared::kBytes, stream, 1, call);
     note_launch();
     if (e != cudaSuccess) {
         return e;
@@ -767,21 +777,22 @@ cudaError_t launch_rows(const RowsCall& call, int blocks, cudaStream_t stream)
     return e;
 }
 
+template <int D, bool SPLIT, int NT = 1>
+cudaError_t launch_rows_columns(const RowsCall& call, int columns, int blocks, cudaStream_t stream)
+{
+    if constexpr (NT < rows_most_columns(D, SPLIT)) {
+        if (columns > NT) {
+            return launch_rows_columns<D, SPLIT, NT + 1>(call, columns, blocks, stream);
+        }
+    }
+    return launch_rows<D, NT, SPLIT>(call, blocks, stream);
+}
+
 template <int D>
 cudaError_t launch_rows_dim(const RowsCall& call, int columns, int blocks, cudaStream_t stream)
 {
-    if (call.a.float_type == NNB200_FLOAT_F32) {
-        return columns == 1 ? launch_rows<D, 1, true>(call, blocks, stream) : launch_rows<D, 2, true>(call, blocks, stream);
-    }
-    if constexpr (D <= 128) {
-        if (columns == 3) {
-            return launch_rows<D, 3, false>(call, blocks, stream);
-        }
-        if (columns == 4) {
-            return launch_rows<D, 4, false>(call, blocks, stream);
-        }
-    }
-    return columns == 1 ? launch_rows<D, 1, false>(call, blocks, stream) : launch_rows<D, 2, false>(call, blocks, stream);
+    return call.a.float_type == NNB200_FLOAT_F32 ? launch_rows_columns<D, true>(call, columns, blocks, stream)
+                                                 : launch_rows_columns<D, false>(call, columns, blocks, stream);
 }
 
 // One translation unit for each head size.
