@@ -30,7 +30,7 @@
 namespace nnb200 {
 
 constexpr int kRowsThreads = 256; // of the joining kernel's blocks
-constexpr int kRowsCost = 16;         // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
+constexpr int kRowsCost = 32;         // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
 constexpr float kGrowth = 8.0f;   // log2 of what a weight may be
 
 // A row tile of a head that begins in a block and ends in a later one.  What a block leaves of its sums: [0] the end or the middle of
@@ -320,8 +320,8 @@ attention_i8_rows_kernel(const RowsCall call)
         own_before = line + block_sum_before(own, total);
         line += total;
     }
-    // No fewer than a group a warp for a block, besides half of what an item costs.
-    const int64_t share_at_least = kWarps + kRowsCost / 2;
+    // Two groups a warp for a block, of eight, where there is no more to do: latency is what counts then.
+    const int64_t share_at_least = 16;
     const int64_t most = (line + share_at_least - 1) / share_at_least;
     const int64_t blocks = most < gridDim.x ? most : gridDim.x;
     if (threadIdx.x == 0) {

@@ -3,8 +3,9 @@
 // A unit of work is one page of one head, keys or values: it has one scale, so whoever quantises its new tokens has to see all
 // of them.  A unit belongs to 1, 4, 8 or 16 warps, as many as let each thread hold its 64 values in registers: the values are
 // read once, their largest magnitude is taken, and the codes are made from the registers.  Both directions are bound by memory
-// (write: 3 bytes a value with f16, read: 3) once there are pages enough; a decode step's write touches one
-// token in each of a few hundred units and costs its launch.
+// (write: 3 bytes a value with f16, read: 3) once there are pages enough, and by the chain of loads before a unit's values are
+// found (sequence, page, values) when there are few; a decode step's write touches one token in each of a few hundred
+// units and costs its launch.  Small units come four to a block, those of neighbouring heads, and find their page together.
 //
 // The pages a call touches are counted on the device, as their number follows `cu` and `lens`.  With n rows in a
 // sequence they are at most n / T + 2 (T tokens a page), so the places of sequence b are those from
@@ -30,20 +31,17 @@ struct Unit {
     int zero_row, zero_rows;   // rows without a token, which this unit answers for
 };
 
-// Warp-collective.
-__device__ __forceinline__ Unit find_unit(const nnb200_cache_i8& c, int64_t index, int32_t* error_word)
+// Warp-collective: the unit of `place` (a page that the call may touch) and `part` (head, keys or values).
+__device__ __forceinline__ Unit find_unit(const nnb200_cache_i8& c, int place, int part, int32_t* error_word)
 {
     Unit u;
-    u.values = static_cast<int>(index & 1);
-    index >>= 1;
+    u.values = part & 1;
+    u.head = part / 2;
     const int tokens = static_cast<int>(c.page_tokens), seqs = static_cast<int>(c.seqs);
-    u.head = static_cast<int>(index % c.heads);
-    const int64_t place = index / c.heads;
-    int b;
-    int64_t j;
+    int b, j;
     if (c.cu == nullptr) {
-        const int64_t slots = (c.rows / c.seqs + tokens - 2) / tokens + 1;
-        b = static_cast<int>(place / slots);
+        const int slots = (static_cast<int>(c.rows) / seqs + tokens - 2) / tokens + 1;
+        b = place / slots;
         j = place - b * slots;
     } else {
         // The last b whose places begin at or before this one, 32 probes at a time.
@@ -57,11 +55,12 @@ __device__ __forceinline__ Unit find_unit(const nnb200_cache_i8& c, int64_t inde
             count = min(step, count - last);
         }
         b = low;
-        j = place - begin(low);
+        const int64_t from = begin(low);
+        j = from <= place ? static_cast<int>(place - from) : -1;
     }
     const SequenceRows s = sequence_rows(c, b);
     const int first = max(s.len - s.n, 0);   // position of the first row that has a token
-    const int64_t slot = first / tokens + j;
+    const int64_t slot = static_cast<int64_t>(first / tokens) + j;
     u.page = -1;
     u.zero_row = s.row0;
     u.zero_rows = j == 0 ? max(s.n - s.len, 0) : 0;
@@ -105,16 +104,16 @@ constexpr int block_threads(int warps) { return warps == 1 ? 128 : 32 * warps; }
 // `wide`: rows and heads of the floating side are 16-byte aligned.
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(block_threads(WARPS))
-cache_write_kernel(const nnb200_cache_rows_args a, const int64_t units, const int wide, int32_t* error_word)
+cache_write_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* error_word)
 {
     previous_kernel_done();
     constexpr int kThreads = 32 * WARPS;
     const nnb200_cache_i8& c = a.cache;
-    const int64_t index = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32 : blockIdx.x;
-    if (index >= units) {
+    const int part = WARPS == 1 ? static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x) / 32 : static_cast<int>(blockIdx.y);
+    if (part >= 2 * c.heads) {
         return;
     }
-    const Unit u = find_unit(c, index, error_word);
+    const Unit u = find_unit(c, static_cast<int>(blockIdx.x), part, error_word);
     if (u.page < 0) {
         return;
     }
@@ -127,16 +126,24 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int64_t units, const in
     int8_t* codes = static_cast<int8_t*>(u.values ? c.v : c.k) + u.page * c.page_stride + static_cast<int64_t>(u.head) * c.page_tokens * dim;
 
     const float before = u.begins ? 0.0f : *scale;
-    float f[kVectors][8];
-    uint32_t top = 0;
+    Eight<T> x[kVectors];
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
         const int at = t + i * kThreads;
         if (at < count) {
-            load8(src + at / per_token * stride_row + at % per_token * 8, wide != 0, f[i]);
+            const int token = at / per_token;
+            x[i].load(src + token * stride_row + (at - token * per_token) * 8, wide != 0);
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+        if (t + i * kThreads < count) {
+            float f[8];
+            x[i].values(f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                top = max(top, magnitude_bits(f[i][e]));
+                top = max(top, magnitude_bits(f[e]));
             }
         }
     }
@@ -149,9 +156,10 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int64_t units, const in
     for (int i = 0; i < kVectors; ++i) {
         const int at = t + i * kThreads;
         if (at < count) {
-            const uint2 q = make_uint2(codes4(f[i][0] * inv, f[i][1] * inv, f[i][2] * inv, f[i][3] * inv),
-                                       codes4(f[i][4] * inv, f[i][5] * inv, f[i][6] * inv, f[i][7] * inv));
-            *reinterpret_cast<uint2*>(codes + u.from * dim + at * 8) = q;
+            float f[8];
+            x[i].values(f);
+            *reinterpret_cast<uint2*>(codes + u.from * dim + at * 8) = make_uint2(codes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                                                                                 codes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
         }
     }
     if (after == before) {
@@ -174,25 +182,30 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int64_t units, const in
     }
 }
 
+// A thread takes 16 codes at a time, all of its loads before its first store.
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(block_threads(WARPS))
-cache_read_kernel(const nnb200_cache_rows_args a, const int64_t units, const int wide, int32_t* error_word)
+cache_read_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* error_word)
 {
     previous_kernel_done();
     constexpr int kThreads = 32 * WARPS;
     const nnb200_cache_i8& c = a.cache;
-    const int64_t index = WARPS == 1 ? static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32 : blockIdx.x;
-    if (index >= units) {
+    const int part = WARPS == 1 ? static_cast<int>(blockIdx.y) * 4 + static_cast<int>(threadIdx.x) / 32 : static_cast<int>(blockIdx.y);
+    if (part >= 2 * c.heads) {
         return;
     }
-    const Unit u = find_unit(c, index, error_word);
+    const Unit u = find_unit(c, static_cast<int>(blockIdx.x), part, error_word);
     const int t = threadIdx.x % kThreads;
-    const int dim = static_cast<int>(c.dim), per_token = dim / 8;
+    const int dim = static_cast<int>(c.dim), per_token = dim / 16;
     const int64_t stride_row = u.values ? a.v_stride_row : a.k_stride_row;
     T* dst = static_cast<T*>(u.values ? a.v : a.k) + u.head * (u.values ? a.v_stride_head : a.k_stride_head);
+    const auto store16 = [&](T* p, const float (&f)[16]) {
+        store8(p, wide != 0, *reinterpret_cast<const float(*)[8]>(f));
+        store8(p + 8, wide != 0, *reinterpret_cast<const float(*)[8]>(f + 8));
+    };
     for (int64_t at = t; at < static_cast<int64_t>(u.zero_rows) * per_token; at += kThreads) {
-        const float none[8] = {};
-        store8(dst + (u.zero_row + at / per_token) * stride_row + at % per_token * 8, wide != 0, none);
+        const float none[16] = {};
+        store16(dst + (u.zero_row + at / per_token) * stride_row + at % per_token * 16, none);
     }
     if (u.page < 0) {
         return;
@@ -202,41 +215,39 @@ cache_read_kernel(const nnb200_cache_rows_args a, const int64_t units, const int
     const int8_t* codes = static_cast<const int8_t*>(u.values ? c.v : c.k) + u.page * c.page_stride +
                           (static_cast<int64_t>(u.head) * c.page_tokens + u.from) * dim;
     dst += u.row * stride_row;
-    uint2 q[kVectors];
+    uint4 q[kVectors / 2];
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
+    for (int i = 0; i < kVectors / 2; ++i) {
         const int at = t + i * kThreads;
         if (at < count) {
-            q[i] = *reinterpret_cast<const uint2*>(codes + at * 8);
+            q[i] = *reinterpret_cast<const uint4*>(codes + at * 16);
         }
     }
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
+    for (int i = 0; i < kVectors / 2; ++i) {
         const int at = t + i * kThreads;
         if (at < count) {
-            float f[8];
+            const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+            float f[16];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f[e] = code_at(e < 4 ? q[i].x : q[i].y, e & 3) * scale;
+            for (int e = 0; e < 16; ++e) {
+                f[e] = code_at(w[e / 4], e & 3) * scale;
             }
-            store8(dst + at / per_token * stride_row + at % per_token * 8, wide != 0, f);
+            const int token = at / per_token;
+            store16(dst + token * stride_row + (at - token * per_token) * 16, f);
         }
     }
 }
 
 template <typename T, int WARPS, bool WRITE>
-cudaError_t run_units(const nnb200_cache_rows_args& a, int64_t units, int wide, const DeviceInfo& dev, cudaStream_t stream)
+cudaError_t run_units(const nnb200_cache_rows_args& a, int64_t places, int wide, const DeviceInfo& dev, cudaStream_t stream)
 {
-    const int64_t blocks = WARPS == 1 ? (units + 3) / 4 : units;
-    if (blocks > 0x7FFFFFFF) {
-        return cudaErrorInvalidConfiguration;
-    }
+    const int64_t parts = 2 * a.cache.heads;
+    const dim3 grid(static_cast<unsigned>(places), static_cast<unsigned>(WARPS == 1 ? (parts + 3) / 4 : parts));
     if constexpr (WRITE) {
-        return launch_overlapping(cache_write_kernel<T, WARPS>, dim3(static_cast<unsigned>(blocks)), dim3(block_threads(WARPS)), 0, stream, 1, a,
-                                  units, wide, dev.error_word);
+        return launch_overlapping(cache_write_kernel<T, WARPS>, grid, dim3(block_threads(WARPS)), 0, stream, 1, a, wide, dev.error_word);
     } else {
-        return launch_overlapping(cache_read_kernel<T, WARPS>, dim3(static_cast<unsigned>(blocks)), dim3(block_threads(WARPS)), 0, stream, 1, a,
-                                  units, wide, dev.error_word);
+        return launch_overlapping(cache_read_kernel<T, WARPS>, grid, dim3(block_threads(WARPS)), 0, stream, 1, a, wide, dev.error_word);
     }
 }
 
@@ -245,8 +256,7 @@ cudaError_t run_typed(const nnb200_cache_rows_args& a, const DeviceInfo& dev, cu
 {
     const nnb200_cache_i8& c = a.cache;
     const int64_t each = c.cu == nullptr ? c.rows / c.seqs : c.rows;   // a sequence has at most so many rows
-    const int64_t places = c.cu == nullptr ? c.seqs * ((each + c.page_tokens - 2) / c.page_tokens + 1) : c.rows / c.page_tokens + 2 * c.seqs;
-    const int64_t units = places * c.heads * 2;
+    const int64_t places = cache_places(c);
     const int64_t values = (each < c.page_tokens ? each : c.page_tokens) * c.dim;
     const auto aligned = [](const void* p, int64_t s0, int64_t s1) {
         constexpr int64_t kPer = 16 / sizeof(T);
@@ -254,10 +264,10 @@ cudaError_t run_typed(const nnb200_cache_rows_args& a, const DeviceInfo& dev, cu
     };
     const int wide = aligned(a.k, a.k_stride_row, a.k_stride_head) && aligned(a.v, a.v_stride_row, a.v_stride_head) ? 1 : 0;
     constexpr int kPerWarp = 32 * 8 * kVectors;
-    return values <= kPerWarp       ? run_units<T, 1, WRITE>(a, units, wide, dev, stream)
-           : values <= 4 * kPerWarp ? run_units<T, 4, WRITE>(a, units, wide, dev, stream)
-           : values <= 8 * kPerWarp ? run_units<T, 8, WRITE>(a, units, wide, dev, stream)
-                                    : run_units<T, 16, WRITE>(a, units, wide, dev, stream);
+    return values <= kPerWarp       ? run_units<T, 1, WRITE>(a, places, wide, dev, stream)
+           : values <= 4 * kPerWarp ? run_units<T, 4, WRITE>(a, places, wide, dev, stream)
+           : values <= 8 * kPerWarp ? run_units<T, 8, WRITE>(a, places, wide, dev, stream)
+                                    : run_units<T, 16, WRITE>(a, places, wide, dev, stream);
 }
 
 template <bool WRITE>

@@ -12,6 +12,12 @@ namespace nnb200 {
 
 constexpr float kLeastCacheScale = 8.673617379884035e-19f;  // 2^-60
 
+// Pages that the rows of a call may touch, in all sequences.
+inline int64_t cache_places(const nnb200_cache_i8& c)
+{
+    return c.cu == nullptr ? c.seqs * ((c.rows / c.seqs + c.page_tokens - 2) / c.page_tokens + 1) : c.rows / c.page_tokens + 2 * c.seqs;
+}
+
 int launch_cache_write_i8(const nnb200_cache_rows_args& a, const DeviceInfo& dev, cudaStream_t stream);
 int launch_cache_read_i8(const nnb200_cache_rows_args& a, const DeviceInfo& dev, cudaStream_t stream);
 int launch_rms_norm_i8(const nnb200_rms_norm_i8_args& a, const DeviceInfo& dev, cudaStream_t stream);
@@ -97,6 +103,51 @@ __device__ __forceinline__ void store8(T* p, bool wide, const float (&f)[8])
         *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
     }
 }
+
+// Eight values as they lie in memory, and one by one.
+template <typename T>
+struct Eight {
+    uint4 raw[sizeof(T) / 2];
+
+    __device__ __forceinline__ void load(const T* p, bool wide)
+    {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+                raw[i] = reinterpret_cast<const uint4*>(p)[i];
+            }
+        } else {
+            uint32_t w[2 * sizeof(T)];
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+                } else {
+                    w[i] = static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[2 * i]) | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[2 * i + 1]) << 16;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+                raw[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(T) == 4) {
+                    f[4 * i + k] = __uint_as_float(w[k]);
+                } else {
+                    unpack2<T>(w[k], f[2 * k], f[2 * k + 1]);
+                }
+            }
+        }
+    }
+};
 
 // Round half to even into s8, saturating; NaN gives 0.
 __device__ __forceinline__ uint32_t code_of(float v)

@@ -1221,6 +1221,9 @@ int check_cache_rows(const nnb200_cache_rows_args* a, bool* empty)
     if (status != NNB200_OK || *empty) {
         return status;
     }
+    if (cache_places(a->cache) > 0x7FFFFFFF || a->cache.heads > 32767) {   // what a grid has
+        return NNB200_UNSUPPORTED;
+    }
     const uintptr_t bytes = float_bytes(a->float_type);
     if (a->k == nullptr || a->v == nullptr || !aligned(a->k, bytes) || !aligned(a->v, bytes)) {
         return NNB200_INVALID_ARGUMENT;

@@ -59,9 +59,9 @@ __device__ __forceinline__ float finish_row(const RowStats& s, int64_t cols, flo
     return __fdiv_rn(127.0f, top);
 }
 
-// VECS vectors of 8 elements a thread; WARP: a row is a warp's.
-template <typename T, typename W, int VECS, bool WARP>
-__global__ void rms_norm_i8_kernel(const nnb200_rms_norm_i8_args a)
+// VECS vectors of 8 elements a thread, THREADS at most; WARP: a row is a warp's.
+template <typename T, typename W, int VECS, bool WARP, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_norm_i8_kernel(const nnb200_rms_norm_i8_args a)
 {
     previous_kernel_done();
     const int per_row = WARP ? 32 : static_cast<int>(blockDim.x);
@@ -74,37 +74,50 @@ __global__ void rms_norm_i8_kernel(const nnb200_rms_norm_i8_args a)
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* residual = static_cast<const T*>(a.residual) + row * a.residual_stride;
     const W* weight = static_cast<const W*>(a.weight);
-    float h[VECS][8], w[VECS][8], r[VECS][8];
+    Eight<T> raw[VECS], more[VECS];
+    Eight<W> w[VECS];
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
         const int at = t + i * per_row;
         if (at < vectors) {
-            load8(x + at * 8, true, h[i]);
+            raw[i].load(x + at * 8, true);
             if (a.residual != nullptr) {
-                load8(residual + at * 8, true, r[i]);
+                more[i].load(residual + at * 8, true);
             }
-            load8(weight + at * 8, true, w[i]);
         }
     }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+        const int at = t + i * per_row;
+        if (at < vectors) {
+            w[i].load(weight + at * 8, true);
+        }
+    }
+    float h[VECS][8];
     RowStats s{0.0, 0u};
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
         const int at = t + i * per_row;
         if (at < vectors) {
+            raw[i].values(h[i]);
             if (a.residual != nullptr) {
+                float r[8];
+                more[i].values(r);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    h[i][e] += r[i][e];
+                    h[i][e] += r[e];
                 }
             }
             if (a.residual_out != nullptr) {
                 store8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + at * 8, true, h[i]);
             }
+            float f[8];
+            w[i].values(f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const double d = h[i][e];
                 s.squares = fma(d, d, s.squares);
-                h[i][e] *= w[i][e];
+                h[i][e] *= f[e];
                 s.top = max(s.top, magnitude_bits(h[i][e]));
             }
         }
@@ -180,14 +193,17 @@ cudaError_t run_typed(const nnb200_rms_norm_i8_args& a, const DeviceInfo& dev, c
     const auto threads = [&](int per) { return dim3(static_cast<unsigned>((vectors + 32 * per - 1) / (32 * per) * 32)); };
     if (vectors <= 64) {
         const dim3 grid((rows + 3) / 4);
-        return vectors <= 32 ? launch_overlapping(rms_norm_i8_kernel<T, W, 1, true>, grid, dim3(128), 0, stream, 1, a)
-                             : launch_overlapping(rms_norm_i8_kernel<T, W, 2, true>, grid, dim3(128), 0, stream, 1, a);
+        return vectors <= 32 ? launch_overlapping(rms_norm_i8_kernel<T, W, 1, true, 128>, grid, dim3(128), 0, stream, 1, a)
+                             : launch_overlapping(rms_norm_i8_kernel<T, W, 2, true, 128>, grid, dim3(128), 0, stream, 1, a);
     }
-    if (vectors <= 1024) {
-        return launch_overlapping(rms_norm_i8_kernel<T, W, 1, false>, dim3(rows), threads(1), 0, stream, 1, a);
-    }
-    return vectors <= 2048 ? launch_overlapping(rms_norm_i8_kernel<T, W, 2, false>, dim3(rows), threads(2), 0, stream, 1, a)
-                           : launch_overlapping(rms_norm_i8_twice_kernel<T, W>, dim3(rows), dim3(1024), 0, stream, 1, a);
+    // Few rows: as many threads as there are vectors, for the latency.  Many: few threads with several vectors each, so that an
+    // SM has more rows under way, some loading while others are summed or stored.
+    const int64_t least = a.rows <= 2 * dev.sm_count ? 1 : (vectors + 255) / 256;
+    const int64_t need = (vectors + 1023) / 1024, per = least > need ? least : need;
+    return per <= 1         ? launch_overlapping(rms_norm_i8_kernel<T, W, 1, false, 1024>, dim3(rows), threads(1), 0, stream, 1, a)
+           : per <= 2       ? launch_overlapping(rms_norm_i8_kernel<T, W, 2, false, 1024>, dim3(rows), threads(2), 0, stream, 1, a)
+           : vectors <= 2048 ? launch_overlapping(rms_norm_i8_kernel<T, W, 4, false, 512>, dim3(rows), threads(4), 0, stream, 1, a)
+                             : launch_overlapping(rms_norm_i8_kernel<T, W, 4, false, 1024>, dim3(rows), threads(4), 0, stream, 1, a);
 }
 
 }  // namespace

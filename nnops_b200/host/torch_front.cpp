@@ -823,34 +823,58 @@ bool head_rows(const at::Tensor& t, int64_t rows, int64_t heads, int64_t dim)
     return t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == dim && t.stride(2) == 1;
 }
 
-// cache_rows_i8(handle, k, v, page_table, lens, cu, write)
-PyObject* cache_rows_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+PyObject* cache_rows(PyObject* handle, const at::Tensor& k, const at::Tensor& v, PyObject* table, PyObject* lens, PyObject* cu, bool write, const c10::Device& dev)
+{
+    nnb200_cache_rows_args a;
+    std::memset(&a, 0, sizeof(a));
+    cache_of(a.cache, handle, table, lens, cu, k.size(0), dev);
+    if (!head_rows(k, a.cache.rows, a.cache.heads, a.cache.dim) || !head_rows(v, a.cache.rows, a.cache.heads, a.cache.dim) ||
+        v.scalar_type() != k.scalar_type()) {
+        elsewhere();
+    }
+    a.float_type = float_type_of(k.scalar_type());
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.k_stride_row = k.stride(0);
+    a.k_stride_head = k.stride(1);
+    a.v_stride_row = v.stride(0);
+    a.v_stride_head = v.stride(1);
+    enqueue(write ? g_lib.cache_write : g_lib.cache_read, &a, dev, write ? "nnb200_cache_write_i8" : "nnb200_cache_read_i8");
+    if (write) {
+        Py_RETURN_TRUE;
+    }
+    return tuple_of({k, v});
+}
+
+// cache_write_i8(handle, k, v, page_table, lens, cu)
+PyObject* cache_write_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     return guarded([&]() -> PyObject* {
-        expect(nargs, 7);
+        expect(nargs, 6);
         const c10::Device dev = current_device(args[1]);
         const at::Tensor& k = plain(args[1], dev);
-        const at::Tensor& v = plain(args[2], dev);
         if (k.dim() != 3) {
             elsewhere();
         }
-        nnb200_cache_rows_args a;
-        std::memset(&a, 0, sizeof(a));
-        cache_of(a.cache, args[0], args[3], args[4], args[5], k.size(0), dev);
-        if (!head_rows(k, a.cache.rows, a.cache.heads, a.cache.dim) || !head_rows(v, a.cache.rows, a.cache.heads, a.cache.dim) ||
-            v.scalar_type() != k.scalar_type()) {
+        return cache_rows(args[0], k, plain(args[2], dev), args[3], args[4], args[5], true, dev);
+    });
+}
+
+// cache_read_i8(handle, page_table, lens, rows, cu, out_dtype)
+PyObject* cache_read_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject* {
+        expect(nargs, 6);
+        const c10::Device dev = current_device(args[1]);
+        if (!PyTuple_CheckExact(args[0]) || PyTuple_GET_SIZE(args[0]) != 11) {
             elsewhere();
         }
-        a.float_type = float_type_of(k.scalar_type());
-        a.k = k.data_ptr();
-        a.v = v.data_ptr();
-        a.k_stride_row = k.stride(0);
-        a.k_stride_head = k.stride(1);
-        a.v_stride_row = v.stride(0);
-        a.v_stride_head = v.stride(1);
-        const bool write = flag(args[6], true);
-        enqueue(write ? g_lib.cache_write : g_lib.cache_read, &a, dev, write ? "nnb200_cache_write_i8" : "nnb200_cache_read_i8");
-        Py_RETURN_TRUE;
+        const int64_t rows = whole(args[3]), heads = whole(PyTuple_GET_ITEM(args[0], 8)), dim = whole(PyTuple_GET_ITEM(args[0], 10));
+        const at::ScalarType type = dtype_of(args[5], at::kHalf);
+        if (rows < 0 || float_type_of(type) < 0) {
+            elsewhere();
+        }
+        return cache_rows(args[0], empty({rows, heads, dim}, type, dev), empty({rows, heads, dim}, type, dev), args[1], args[2], args[4], false, dev);
     });
 }
 
@@ -943,7 +967,8 @@ PyMethodDef g_methods[] = {
     {"linear_fp_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_fp_act)), METH_FASTCALL, nullptr},
     {"conv2d_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(conv2d_i8)), METH_FASTCALL, nullptr},
     {"rms_norm_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rms_norm_i8)), METH_FASTCALL, nullptr},
-    {"cache_rows_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_rows_i8)), METH_FASTCALL, nullptr},
+    {"cache_write_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_write_i8)), METH_FASTCALL, nullptr},
+    {"cache_read_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_read_i8)), METH_FASTCALL, nullptr},
     {"attention_i8_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention_i8_cache)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

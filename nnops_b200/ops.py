@@ -626,7 +626,7 @@ def cache_write_i8(cache: CacheI8, k: torch.Tensor, v: torch.Tensor, page_table:
                    cu: torch.Tensor | None = None) -> CacheI8:
     """Quantise the rows ``k``, ``v`` [rows, heads, dim] (f32 / f16 / bf16) into ``cache`` on the current CUDA stream, as the last tokens of
     their sequences."""
-    if (_native or _front()).cache_rows_i8(cache._handle, k, v, page_table, lens, cu, True) is not None:
+    if (_native or _front()).cache_write_i8(cache._handle, k, v, page_table, lens, cu) is not None:
         return cache
     kind = _float_type(k, "k")
     if v.dtype is not k.dtype:
@@ -646,10 +646,11 @@ def cache_read_i8(cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, 
     if out is None:
         if rows is None:
             raise ValueError("rows or out is needed")
+        made = (_native or _front()).cache_read_i8(cache._handle, page_table, lens, rows, cu, out_dtype)
+        if made is not None:
+            return made
         out = tuple(torch.empty((rows, cache.heads, cache.dim), dtype=out_dtype, device=cache.device) for _ in range(2))
     k, v = out
-    if (_native or _front()).cache_rows_i8(cache._handle, k, v, page_table, lens, cu, False) is not None:
-        return k, v
     kind = _float_type(k, "out")
     if v.dtype is not k.dtype or (rows is not None and rows != k.shape[0]):
         raise ValueError("the outputs must be of one type, and have the rows asked for")
