@@ -8,6 +8,7 @@ namespace {
 
 constexpr int kEngineRows = 1;
 constexpr int kEngineTile = 2;
+constexpr int64_t kClusterTokens = 16384;
 
 // Query rows that share a sequence's head, on average where their numbers are the device's.
 int64_t rows_each(const nnb200_attention_i8_args& a)
@@ -41,6 +42,20 @@ RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
     const int64_t tiles = (rows + 8 * most - 1) / (8 * most);
     p.columns = static_cast<int>((rows + 8 * tiles - 1) / (8 * tiles));
     p.blocks = dev.sm_count * rows_blocks(c.dim, p.columns, split);
+    // Clusters where all of them are under way at once and a warp has few groups whatever the lengths are: the most that the table,
+    // or the window, has room for.
+    int64_t most_tokens = c.table_pages * c.page_tokens;
+    if (a.window > 0 && a.window < most_tokens) {
+        const int64_t seen = a.window + (a.sinks < most_tokens ? a.sinks : most_tokens) + c.rows / c.seqs + 32;
+        most_tokens = seen < most_tokens ? seen : most_tokens;
+    }
+    const int64_t clusters = c.seqs * c.heads * tiles;
+    p.tiles = c.cu == nullptr && clusters * kRowsCluster <= p.blocks && most_tokens <= kClusterTokens ? static_cast<int>(tiles) : 0;
+    if (p.tiles > 0) {
+        p.blocks = static_cast<int>(clusters) * kRowsCluster;
+        p.bytes = 0;
+        return p;
+    }
     const size_t blocks = static_cast<size_t>(p.blocks);
     p.bytes = blocks * (sizeof(RowsPiece) + 2 * static_cast<size_t>(8 * p.columns) * static_cast<size_t>(c.dim + 2) * sizeof(float));
     return p;
@@ -82,6 +97,7 @@ int run_rows(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.wide = multiple(a.q, 16, a.q_stride_row, a.q_stride_head, per);
     call.wide_out = multiple(a.out, 128 / per / 2, a.out_stride_row, a.out_stride_head, 4);
     call.page_shift = page_shift(a);
+    call.tiles = p.tiles;
     call.pieces = static_cast<RowsPiece*>(a.workspace);
     call.sums = reinterpret_cast<float*>(call.pieces + p.blocks);
     switch (a.cache.dim) {

@@ -23,9 +23,13 @@
 // The work of all sequences, row tiles and heads is one line of 16-token groups, cut into equal pieces, one for each block, so
 // that lengths of any mix keep every SM busy to the end.  A row tile of a head that is cut leaves (m, l, sums) in the
 // workspace, in a fixed order of blocks; a second kernel joins them, in that order: results do not depend on timing.
+//
+// A few row tiles over contexts that cannot be long, all sequences with as many rows, go to a cluster of eight blocks each instead:
+// their sums meet in shared memory, without a workspace, a search for one's place or a second kernel.
 #pragma once
 
 #include "cache_i8.cuh"
+#include "ptx_pair.cuh"
 
 namespace nnb200 {
 
@@ -47,6 +51,7 @@ struct RowsPiece {
 struct RowsPlan {
     int blocks;    // of the first kernel
     int columns;   // query rows of a tile / 8
+    int tiles;     // of every sequence, if each row tile of a head has a cluster of its own; else 0
     size_t bytes;  // of the workspace: the pieces, then their sums ([tile rows][dim], m and l of each row)
 };
 
@@ -58,6 +63,7 @@ struct RowsCall {
     int wide;            // q's rows and heads are 16-byte aligned
     int wide_out;        // out's are, to four values
     int page_shift;      // log2 of the tokens of a page
+    int tiles;           // of every sequence, in clusters
     RowsPiece* pieces;   // [blocks]
     float* sums;         // [blocks][2][piece]
 };
@@ -157,25 +163,15 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
     }
 }
 
-// COUNT consecutive values from element i on; `wide`: their address is 16-byte aligned.
-template <int COUNT, typename T>
-__device__ __forceinline__ void load_values(const T* p, bool wide, float (&v)[COUNT])
+// Four words, or eight 16-bit values, as they are; `wide`: the address is 16-byte aligned.
+__device__ __forceinline__ uint4 four_words(const uint32_t* p, bool wide) { return wide ? *reinterpret_cast<const uint4*>(p) : make_uint4(p[0], p[1], p[2], p[3]); }
+__device__ __forceinline__ uint4 eight_of(const uint16_t* p, bool wide)
 {
-#pragma unroll
-    for (int i = 0; i < COUNT; i += 8) {
-        load8(p + i, wide, *reinterpret_cast<float(*)[8]>(v + i));
+    if (wide) {
+        return *reinterpret_cast<const uint4*>(p);
     }
-}
-template <int COUNT>
-__device__ __forceinline__ void load_floats(const void* p, int64_t i, int type, bool wide, float (&v)[COUNT])
-{
-    if (type == NNB200_FLOAT_F32) {
-        load_values(static_cast<const float*>(p) + i, wide, v);
-    } else if (type == NNB200_FLOAT_F16) {
-        load_values(static_cast<const __half*>(p) + i, wide, v);
-    } else {
-        load_values(static_cast<const __nv_bfloat16*>(p) + i, wide, v);
-    }
+    const auto two = [&](int i) { return static_cast<uint32_t>(p[i]) | static_cast<uint32_t>(p[i + 1]) << 16; };
+    return make_uint4(two(0), two(2), two(4), two(6));
 }
 
 template <typename T>
@@ -250,7 +246,9 @@ struct RowsShared {
     static constexpr int kWanted = (rows_blocks(D, NT, SPLIT) == 2 ? 96 : 192) * 1024;
     static constexpr int kStages = kWanted / (kWarps * kStageBytes) > 8 ? 8 : kWanted / (kWarps * kStageBytes);
     static constexpr int kRing = kWarps * kStages * kStageBytes;
-    static constexpr int kBytes = kRing > kJoinBytes ? kRing : kJoinBytes;
+    static constexpr int kSumBytes = 8 * NT * (D + 2) * 4;   // in a cluster: of a block
+    static constexpr int kBytes = (kRing > kJoinBytes ? kRing : kJoinBytes);
+    static constexpr int kClusterBytes = kRing > kJoinBytes + kSumBytes ? kRing : kJoinBytes + kSumBytes;
     static_assert(kStages >= 2 && rows_blocks(D, NT, SPLIT) * kBytes <= 200 * 1024, "ring");
 };
 
@@ -259,7 +257,28 @@ struct StageScales {
     int there;
 };
 
-template <int D, int NT, bool SPLIT>
+constexpr int kRowsCluster = 8;
+
+// Of numbers that are not negative: by 32-bit arithmetic where they allow it, which takes a fraction of the time.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
+{
+    return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+__device__ __forceinline__ float4 ld_shared_cluster_f32x4(uint32_t cluster_addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_shared_cluster_float(uint32_t cluster_addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+template <int D, int NT, bool SPLIT, bool CLUSTER>
 __global__ void __launch_bounds__(RowsShared<D, NT, SPLIT>::kThreads, rows_blocks(D, NT, SPLIT))
 attention_i8_rows_kernel(const RowsCall call)
 {
@@ -273,89 +292,100 @@ attention_i8_rows_kernel(const RowsCall call)
     __shared__ float join_m[kWarps][kTile], join_l[kWarps][kTile];
     __shared__ int64_t scan[kWarps + 1];
     __shared__ int64_t found_base;
+    __shared__ int64_t cut[3];   // of the line: blocks, the least share of one, how many groups are over
     __shared__ int found_seq;
     __shared__ int abort_flag;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int g = lane / 4, c = lane & 3;
+    static_assert(kWarps * kStages <= kThreads, "a barrier a thread");
+    if (threadIdx.x < kWarps * kStages) {
+        mbar_init(&full[0][0] + threadIdx.x, 1);
+        mbar_init_fence();
+    }
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int i = 0; i < kWarps * kStages; ++i) {
-            mbar_init(&full[0][0] + i, 1);
-        }
-        mbar_init_fence();
     }
     __syncthreads();
     previous_kernel_done();
     const nnb200_attention_i8_args& a = call.a;
     const int seqs = static_cast<int>(a.cache.seqs);
 
-    // The line's length, and the sequence in which this block's piece begins.
-    const auto block_sum_before = [&](int64_t v, int64_t& total) {   // of the threads before this one
-        int64_t up = v;
+    int seq = 0;
+    int64_t base = 0, at = 0, end = 1;
+    const auto start_of = [&](int64_t block) { return cut[1] * block + quotient(cut[2] * block, cut[0]); };
+    if constexpr (!CLUSTER) {
+        // The line's length, and the sequence in which this block's piece begins.
+        const auto block_sum_before = [&](int64_t v, int64_t& total) {   // of the threads before this one
+            int64_t up = v;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t other = __shfl_up_sync(0xFFFFFFFFu, up, o);
-            up += lane >= o ? other : 0;
-        }
-        __syncthreads();
-        if (lane == 31) {
-            scan[warp] = up;
-        }
-        __syncthreads();
-        int64_t before = up - v;
-        total = 0;
-        for (int i = 0; i < kWarps; ++i) {
-            before += i < warp ? scan[i] : 0;
-            total += scan[i];
-        }
-        return before;
-    };
-    // Up to so many threads: everyone has its own sequence's place at once.
-    int64_t line = 0, own = 0, own_before = 0;
-    for (int b0 = 0; b0 < seqs; b0 += kThreads) {
-        const int b = b0 + static_cast<int>(threadIdx.x);
-        int64_t total;
-        own = b < seqs ? sequence_work(call, b, kTile).total : 0;
-        own_before = line + block_sum_before(own, total);
-        line += total;
-    }
-    // Two groups a warp for a block, of eight, where there is no more to do: latency is what counts then.
-    const int64_t share_at_least = 16;
-    const int64_t most = (line + share_at_least - 1) / share_at_least;
-    const int64_t blocks = most < gridDim.x ? most : gridDim.x;
-    if (threadIdx.x == 0) {
-        call.pieces[blockIdx.x].more = 0;
-    }
-    if (static_cast<int64_t>(blockIdx.x) >= blocks) {
-        return;
-    }
-    const int64_t share = line / blocks, over = line % blocks;
-    const auto start_of = [&](int64_t block) { return share * block + over * block / blocks; };
-    int64_t at = start_of(blockIdx.x);
-    const int64_t end = start_of(blockIdx.x + 1);
-    if (seqs <= kThreads) {
-        if (own_before <= at && at < own_before + own) {
-            found_seq = threadIdx.x;
-            found_base = own_before;
-        }
-    } else {
-        int64_t base = 0;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t other = __shfl_up_sync(0xFFFFFFFFu, up, o);
+                up += lane >= o ? other : 0;
+            }
+            __syncthreads();
+            if (lane == 31) {
+                scan[warp] = up;
+            }
+            __syncthreads();
+            int64_t before = up - v;
+            total = 0;
+            for (int i = 0; i < kWarps; ++i) {
+                before += i < warp ? scan[i] : 0;
+                total += scan[i];
+            }
+            return before;
+        };
+        // Up to so many threads: everyone has its own sequence's place at once.
+        int64_t line = 0, own = 0, own_before = 0;
         for (int b0 = 0; b0 < seqs; b0 += kThreads) {
             const int b = b0 + static_cast<int>(threadIdx.x);
-            own = b < seqs ? sequence_work(call, b, kTile).total : 0;
             int64_t total;
-            own_before = base + block_sum_before(own, total);
+            own = b < seqs ? sequence_work(call, b, kTile).total : 0;
+            own_before = line + block_sum_before(own, total);
+            line += total;
+        }
+        // Two groups a warp for a block, of eight, where there is no more to do: latency is what counts then.
+        const int64_t share_at_least = 16;
+        const int64_t most = (line + share_at_least - 1) / share_at_least;
+        const int64_t blocks = most < gridDim.x ? most : gridDim.x;
+        if (threadIdx.x == 0) {
+            call.pieces[blockIdx.x].more = 0;
+        }
+        if (static_cast<int64_t>(blockIdx.x) >= blocks) {
+            return;
+        }
+        if (threadIdx.x == 0) {
+            cut[0] = blocks;
+            cut[1] = quotient(line, blocks);
+            cut[2] = line - cut[1] * blocks;
+        }
+        __syncthreads();
+        at = start_of(blockIdx.x);
+        end = start_of(blockIdx.x + 1);
+        if (seqs <= kThreads) {
             if (own_before <= at && at < own_before + own) {
-                found_seq = b;
+                found_seq = threadIdx.x;
                 found_base = own_before;
             }
-            base += total;
+        } else {
+            int64_t base = 0;
+            for (int b0 = 0; b0 < seqs; b0 += kThreads) {
+                const int b = b0 + static_cast<int>(threadIdx.x);
+                own = b < seqs ? sequence_work(call, b, kTile).total : 0;
+                int64_t total;
+                own_before = base + block_sum_before(own, total);
+                if (own_before <= at && at < own_before + own) {
+                    found_seq = b;
+                    found_base = own_before;
+                }
+                base += total;
+            }
         }
+        __syncthreads();
+        seq = found_seq;
+        base = found_base;
     }
-    __syncthreads();
-    int seq = found_seq;
-    int64_t base = found_base;
 
     uint32_t issued = 0;   // 16-token groups of this warp
     uint32_t issue_slot = 0, slot = 0, round = 0;   // of the ring: the next to fill, the next to take and its turn
@@ -363,22 +393,40 @@ attention_i8_rows_kernel(const RowsCall call)
     bool failed = false;
 
     while (at < end) {
-        const SequenceWork work = sequence_work(call, seq, kTile);
-        if (at >= base + work.total) {
-            base += work.total;
-            ++seq;
-            continue;
+        SequenceWork work;
+        int head, tile, off, count, length = 0;
+        int64_t item = 0;
+        if constexpr (CLUSTER) {
+            // Sequence by sequence, tile by tile, head by head; as many tiles in each.
+            const int cluster = static_cast<int>(blockIdx.x) / kRowsCluster, rank = static_cast<int>(blockIdx.x) % kRowsCluster;
+            const int heads = static_cast<int>(a.cache.heads), each = cluster / heads;
+            head = cluster - each * heads;
+            seq = each / call.tiles;
+            tile = each - seq * call.tiles;
+            work = sequence_work(call, seq, kTile);
+            off = static_cast<int>(static_cast<int64_t>(work.groups) * rank / kRowsCluster);
+            count = static_cast<int>(static_cast<int64_t>(work.groups) * (rank + 1) / kRowsCluster) - off;
+            at = end;
+        } else {
+            work = sequence_work(call, seq, kTile);
+            if (at >= base + work.total) {
+                base += work.total;
+                ++seq;
+                continue;
+            }
+            length = work.groups + kRowsCost;
+            item = quotient(at - base, length);
+            const int from = static_cast<int>(at - base - item * length);
+            const int to = static_cast<int>(from + (end - at) < length ? from + (end - at) : length);
+            at += to - from;
+            off = max(from - kRowsCost, 0);
+            count = max(to - kRowsCost, 0) - off;
+            if (count <= 0) {
+                continue;
+            }
+            head = static_cast<int>(quotient(item, work.tiles));
+            tile = static_cast<int>(item - static_cast<int64_t>(head) * work.tiles);
         }
-        const int length = work.groups + kRowsCost;
-        const int64_t item = (at - base) / length;
-        const int from = static_cast<int>((at - base) % length);
-        const int to = static_cast<int>(from + (end - at) < length ? from + (end - at) : length);
-        at += to - from;
-        const int off = max(from - kRowsCost, 0), count = max(to - kRowsCost, 0) - off;
-        if (count <= 0) {
-            continue;
-        }
-        const int head = static_cast<int>(item / work.tiles), tile = static_cast<int>(item % work.tiles);
 
         const int rows = min(kTile, work.s.n * call.group - tile * kTile);
         const int first_pos = work.s.len - work.s.n;
@@ -424,25 +472,47 @@ attention_i8_rows_kernel(const RowsCall call)
             ++issued;
             issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
         };
+        // The query rows are asked for before the pages are looked up: this thread's part of row 8 nt + g, dims [c D / 4, + D / 4).
+        uint4 raw[NT][SPLIT ? D / 16 : D / 32];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g, global = tile * kTile + r, token = global / call.group;
+            const int64_t src = (work.s.row0 + token) * a.q_stride_row + (head * call.group + global - token * call.group) * a.q_stride_head + c * (D / 4);
+#pragma unroll
+            for (int i = 0; i < (SPLIT ? D / 16 : D / 32); ++i) {
+                raw[nt][i] = make_uint4(0u, 0u, 0u, 0u);
+                if (r < rows) {
+                    if constexpr (SPLIT) {
+                        raw[nt][i] = four_words(static_cast<const uint32_t*>(a.q) + src + 4 * i, call.wide != 0);
+                    } else {
+                        raw[nt][i] = eight_of(static_cast<const uint16_t*>(a.q) + src + 8 * i, call.wide != 0);
+                    }
+                }
+            }
+        }
         for (int i = 0; i < min(mine, kStages); ++i) {
             issue(i);
         }
-        // This thread's part of the query rows: row 8 nt + g, dims [c D / 4, + D / 4), in f16 scaled by a power of two.
+        // In f16, scaled by a power of two.
         uint32_t q[NT][kParts][D / 16][2];
         float factor[NT][2];    // of the columns 2 c and 2 c + 1
         int pos[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 8 + g;
-            const int global = tile * kTile + r;
-            const int64_t src = (work.s.row0 + global / call.group) * a.q_stride_row + (head * call.group + global % call.group) * a.q_stride_head + c * (D / 4);
             float v[D / 4];
 #pragma unroll
-            for (int i = 0; i < D / 4; ++i) {
-                v[i] = 0.0f;
-            }
-            if (r < rows) {
-                load_floats(a.q, src, a.float_type, call.wide != 0, v);
+            for (int i = 0; i < (SPLIT ? D / 16 : D / 32); ++i) {
+                const uint32_t w[4] = {raw[nt][i].x, raw[nt][i].y, raw[nt][i].z, raw[nt][i].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (SPLIT) {
+                        v[4 * i + k] = __uint_as_float(w[k]);
+                    } else if (a.float_type == NNB200_FLOAT_F16) {
+                        unpack2<__half>(w[k], v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
+                    } else {
+                        unpack2<__nv_bfloat16>(w[k], v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
+                    }
+                }
             }
             uint32_t top = 0;
 #pragma unroll
@@ -651,7 +721,7 @@ attention_i8_rows_kernel(const RowsCall call)
             }
         }
         __syncthreads();
-        const bool begins = off == 0, ends = off + count == work.groups;
+        const bool begins = off == 0, ends = off + count == work.groups;   // (of no account in a cluster)
         const int which = begins ? 1 : 0;
         float* piece = call.sums + (2 * static_cast<int64_t>(blockIdx.x) + which) * (kTile * (D + 2));
         for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
@@ -674,7 +744,14 @@ attention_i8_rows_kernel(const RowsCall call)
                 sum.z = __fmaf_rn(v.z, share, sum.z);
                 sum.w = __fmaf_rn(v.w, share, sum.w);
             }
-            if (begins && ends) {
+            if constexpr (CLUSTER) {
+                float* mine_of = join_o + kWarps * kTile * D;   // behind the warps' sums
+                *reinterpret_cast<float4*>(mine_of + r * D + d) = sum;
+                if (d == 0) {
+                    mine_of[kTile * D + r] = top;
+                    mine_of[kTile * D + kTile + r] = total;
+                }
+            } else if (begins && ends) {
                 const int global = tile * kTile + r;
                 store_row(call, (work.s.row0 + global / call.group) * a.out_stride_row + (head * call.group + global % call.group) * a.out_stride_head + d, sum, total);
             } else {
@@ -685,15 +762,48 @@ attention_i8_rows_kernel(const RowsCall call)
                 }
             }
         }
+        if constexpr (CLUSTER) {
+            // Every block takes an eighth of the row tile's sums, out of all eight.
+            __syncwarp();
+            cluster_sync_all();
+            const uint32_t rank = cluster_cta_rank(), here = smem_u32(join_o + kWarps * kTile * D);
+            for (int i = static_cast<int>(rank * kThreads + threadIdx.x); i < rows * (D / 4); i += kRowsCluster * kThreads) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float4 v[kRowsCluster];
+                float m_of[kRowsCluster], l_of[kRowsCluster], top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < kRowsCluster; ++k) {
+                    const uint32_t there = map_to_cta(here, k);
+                    v[k] = ld_shared_cluster_f32x4(there + static_cast<uint32_t>(r * D + d) * 4);
+                    m_of[k] = ld_shared_cluster_float(there + static_cast<uint32_t>(kTile * D + r) * 4);
+                    l_of[k] = ld_shared_cluster_float(there + static_cast<uint32_t>(kTile * D + kTile + r) * 4);
+                    top = fmaxf(top, m_of[k]);
+                }
+                const float safe = top == -INFINITY ? 0.0f : top;
+                float total = 0.0f;
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int k = 0; k < kRowsCluster; ++k) {
+                    const float part = exp2_fast(m_of[k] - safe);
+                    total = __fmaf_rn(l_of[k], part, total);
+                    sum.x = __fmaf_rn(v[k].x, part, sum.x);
+                    sum.y = __fmaf_rn(v[k].y, part, sum.y);
+                    sum.z = __fmaf_rn(v[k].z, part, sum.z);
+                    sum.w = __fmaf_rn(v[k].w, part, sum.w);
+                }
+                const int global = tile * kTile + r;
+                store_row(call, (work.s.row0 + global / call.group) * a.out_stride_row + (head * call.group + global % call.group) * a.out_stride_head + d, sum, total);
+            }
+            __syncwarp();
+            cluster_sync_all();   // nobody leaves while his sums are read
+            return;
+        }
         if (begins && !ends && threadIdx.x == 0) {
             // The block in which it ends: the one that has the item's last place on the line.
             const int64_t place = base + (item + 1) * length - 1;
-            int64_t block = place * blocks / line;
+            int64_t block = quotient(place, cut[1] + 1);   // or a later one
             while (start_of(block + 1) <= place) {
                 ++block;
-            }
-            while (start_of(block) > place) {
-                --block;
             }
             call.pieces[blockIdx.x] = RowsPiece{static_cast<int32_t>(block - blockIdx.x), head, work.s.row0, tile * kTile, rows, {}};
         }
@@ -757,19 +867,20 @@ __global__ void __launch_bounds__(kRowsThreads) attention_i8_join_kernel(const R
     }
 }
 
-template <int D, int NT, bool SPLIT>
+template <int D, int NT, bool SPLIT, bool CLUSTER>
 cudaError_t launch_rows(const RowsCall& call, int blocks, cudaStream_t stream)
 {
     using Shared = RowsShared<D, NT, SPLIT>;
-    const auto kernel = attention_i8_rows_kernel<D, NT, SPLIT>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared::kBytes);
+    constexpr int kBytes = CLUSTER ? Shared::kClusterBytes : Shared::kBytes;
+    const auto kernel = attention_i8_rows_kernel<D, NT, SPLIT, CLUSTER>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return e;
     }
-    e = launch_overlapping(kernel, dim3(static_cast<unsigned>(blocks)), dim3(Shared::kThreads), Shared::kBytes, stream, 1, call);
+    e = launch_overlapping(kernel, dim3(static_cast<unsigned>(blocks)), dim3(Shared::kThreads), kBytes, stream, CLUSTER ? kRowsCluster : 1, call);
     note_launch();
-    if (e != cudaSuccess) {
+    if (e != cudaSuccess || CLUSTER) {
         return e;
     }
     e = launch_overlapping(attention_i8_join_kernel<D, 8 * NT>, dim3(static_cast<unsigned>(blocks)), dim3(kRowsThreads), 0, stream, 1, call);
@@ -785,7 +896,7 @@ cudaError_t launch_rows_columns(const RowsCall& call, int columns, int blocks, c
             return launch_rows_columns<D, SPLIT, NT + 1>(call, columns, blocks, stream);
         }
     }
-    return launch_rows<D, NT, SPLIT>(call, blocks, stream);
+    return call.tiles > 0 ? launch_rows<D, NT, SPLIT, true>(call, blocks, stream) : launch_rows<D, NT, SPLIT, false>(call, blocks, stream);
 }
 
 template <int D>

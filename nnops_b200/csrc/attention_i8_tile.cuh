@@ -342,18 +342,6 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b)
 // The same in every lane, and in a uniform register: what a reduction gives is, what a shuffle gives is not.
 __device__ __forceinline__ uint32_t in_uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
 
-// Eight 16-bit values as they are; `wide`: the address is 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ uint4 eight_of(const T* p, bool wide)
-{
-    if (wide) {
-        return *reinterpret_cast<const uint4*>(p);
-    }
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-    const auto two = [&](int i) { return static_cast<uint32_t>(h[i]) | static_cast<uint32_t>(h[i + 1]) << 16; };
-    return make_uint4(two(0), two(2), two(4), two(6));
-}
-
 // 16 codes as f16 into the swizzled tile: row `key`, dims [16 segment, + 16).
 template <int D>
 __device__ __forceinline__ void store_codes(uint8_t* tile, int key, int segment, const uint4& codes)
@@ -462,7 +450,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 const T* src = static_cast<const T*>(a.q) + (row_there ? source(r, a.q_stride_row, a.q_stride_head) : 0) + lane % 4 * 8;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
-                    raw[i][c] = row_there ? eight_of(src + c * 32, call.wide != 0) : make_uint4(0u, 0u, 0u, 0u);
+                    raw[i][c] = row_there ? eight_of(reinterpret_cast<const uint16_t*>(src + c * 32), call.wide != 0) : make_uint4(0u, 0u, 0u, 0u);
                 }
             }
 #pragma unroll

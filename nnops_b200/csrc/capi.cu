@@ -1336,14 +1336,15 @@ int nnb200_attention_i8(const nnb200_attention_i8_args* args, void* stream)
     if (status != NNB200_OK || empty) {
         return status;
     }
-    if (args->workspace == nullptr || !aligned(args->workspace, 16)) {
+    if (!aligned(args->workspace, 16)) {
         return NNB200_INVALID_ARGUMENT;
     }
     const DeviceInfo* dev = current_device_info();
     if (dev == nullptr) {
         return NNB200_INTERNAL;
     }
-    if (args->workspace_bytes < attention_i8_workspace_bytes(*args, *dev)) {
+    const size_t need = attention_i8_workspace_bytes(*args, *dev);
+    if (need > 0 && (args->workspace == nullptr || args->workspace_bytes < need)) {
         return NNB200_INVALID_ARGUMENT;
     }
     return launch_attention_i8(*args, *dev, static_cast<cudaStream_t>(stream));

@@ -74,7 +74,7 @@ def test_cache_arguments(nnb200_lib, entry):
 
 def test_attention_arguments(nnb200_lib):
     call = nnb200_lib.nnb200_attention_i8
-    for over in (dict(q_heads=0), dict(q_heads=3), dict(window=-1), dict(sinks=-1), dict(window=4, causal=0), dict(force_engine=9), dict(workspace=None),
+    for over in (dict(q_heads=0), dict(q_heads=3), dict(window=-1), dict(sinks=-1), dict(window=4, causal=0), dict(force_engine=9),
                  dict(workspace=BASE + 8, workspace_bytes=1 << 40)):
         assert call(C.byref(_cache(capi.AttentionI8Args, **over)), None) == capi.INVALID_ARGUMENT, over
     for dim in (16, 80, 112, 160):
