@@ -27,7 +27,11 @@ int engine_of(const nnb200_attention_i8_args& a)
     if (a.float_type == NNB200_FLOAT_F32) {
         return kEngineRows;   // the tiles hold queries and weights as one f16
     }
-    return a.force_engine != 0 ? a.force_engine : rows_each(a) > 64 ? kEngineTile : kEngineRows;
+    // The tiles take as long for one row as for all of theirs, the rows' kernel the longer the more rows and the larger the heads.
+    // Heads of 64, 128 and 256, rows against tiles in us: 8 sequences of 4096 tokens, 64 and 96 rows 48 / 54 and 65 / 54; 48 and 64 rows
+    // 61 / 62 and 83 / 63; 16 and 32 rows 65 / 80 and 96 / 82; one of 32768 tokens, 96 and 128 rows 59 / 64 and 73 / 65; 48 and 64
+    // rows 60 / 72 and 76 / 72; 16 and 32 rows 68 / 91 and 93 / 91.
+    return a.force_engine != 0 ? a.force_engine : rows_each(a) * a.cache.dim > 6144 ? kEngineTile : kEngineRows;
 }
 
 // Tiles of 8 to 32 query rows: as few of them as a sequence needs, all as wide.  A wider tile reads the codes for more rows at once

@@ -595,31 +595,43 @@ attention_i8_rows_kernel(const RowsCall call)
                 const bool all_seen = key0 + 15 < work.s.len && key0 + 15 <= least_pos &&
                                       (a.window == 0 || key0 > most_pos - a.window || key0 + 15 < a.sinks);
                 uint32_t pb[NT][kParts][2];
+                // Element e of a tile of eight rows: token g (e < 2) or g + 8, column 2 c + (e & 1).
+                float x[NT][4], largest = -INFINITY;
+                uint32_t hidden = 0;   // a bit an element
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    // Element e: token g (e < 2) or g + 8, column 2 c + (e & 1).
                     const float kf[2] = {sc.k * factor[nt][0], sc.k * factor[nt][1]};
                     const float less[2] = {sc.v_log2 - m[nt][0], sc.v_log2 - m[nt][1]};   // +infinity until a row has seen something
-                    float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        x[e] = __fmaf_rn(s[nt][e], kf[e & 1], less[e & 1]);
+                        x[nt][e] = __fmaf_rn(s[nt][e], kf[e & 1], less[e & 1]);
                     }
-                    bool seen[4] = {true, true, true, true};
-                    if (!all_seen) {
+                }
+                if (!all_seen) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int key = key0 + g + (e < 2 ? 0 : 8), at_pos = pos[nt][e & 1];
-                            seen[e] = key < work.s.len && key <= at_pos && (a.window == 0 || key > at_pos - a.window || key < a.sinks);
-                            x[e] = seen[e] ? x[e] : -INFINITY;
+                            const bool seen = key < work.s.len && key <= at_pos && (a.window == 0 || key > at_pos - a.window || key < a.sinks);
+                            x[nt][e] = seen ? x[nt][e] : -INFINITY;
+                            hidden |= seen ? 0u : 1u << (nt * 4 + e);
                         }
                     }
-                    if (__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kGrowth)) {
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    largest = fmaxf(largest, fmaxf(fmaxf(x[nt][0], x[nt][1]), fmaxf(x[nt][2], x[nt][3])));
+                }
+                if (__any_sync(0xFFFFFFFFu, largest > kGrowth)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
                         float alpha[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const float t0 = seen[j] ? __fmaf_rn(s[nt][j], kf[j], sc.v_log2) : -INFINITY;
-                            const float t1 = seen[j + 2] ? __fmaf_rn(s[nt][j + 2], kf[j], sc.v_log2) : -INFINITY;
+                            const float kf = sc.k * factor[nt][j];
+                            const float t0 = (hidden >> (nt * 4 + j) & 1) == 0 ? __fmaf_rn(s[nt][j], kf, sc.v_log2) : -INFINITY;
+                            const float t1 = (hidden >> (nt * 4 + j + 2) & 1) == 0 ? __fmaf_rn(s[nt][j + 2], kf, sc.v_log2) : -INFINITY;
                             float top = fmaxf(t0, t1);
                             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
@@ -628,8 +640,8 @@ attention_i8_rows_kernel(const RowsCall call)
                             alpha[j] = exp2_fast(m[nt][j] - safe);
                             m[nt][j] = next;
                             l[nt][j] *= alpha[j];
-                            x[j] = t0 - safe;
-                            x[j + 2] = t1 - safe;
+                            x[nt][j] = t0 - safe;
+                            x[nt][j + 2] = t1 - safe;
                         }
 #pragma unroll
                         for (int d = 0; d < D / 16; ++d) {
@@ -639,20 +651,23 @@ attention_i8_rows_kernel(const RowsCall call)
                             o[nt][d][3] *= alpha[1];
                         }
                     }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        x[j] = exp2_fast(x[j]);
-                        x[j + 2] = exp2_fast(x[j + 2]);
-                        const float both = x[j] + x[j + 2];
+                        x[nt][j] = exp2_fast(x[nt][j]);
+                        x[nt][j + 2] = exp2_fast(x[nt][j + 2]);
+                        const float both = x[nt][j] + x[nt][j + 2];
                         l[nt][j] += both == 0.0f ? 0.0f : both * sc.v_inv;   // (not 0 times what a block that is masked has for a scale)
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const __half2 h = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                        const __half2 h = __floats2half2_rn(x[nt][2 * j], x[nt][2 * j + 1]);
                         pb[nt][0][j] = transposed_8x8(*reinterpret_cast<const uint32_t*>(&h));
                         if constexpr (SPLIT) {
                             const float2 f = __half22float2(h);
-                            pb[nt][kParts - 1][j] = transposed_8x8(pack2<__half>(x[2 * j] - f.x, x[2 * j + 1] - f.y));
+                            pb[nt][kParts - 1][j] = transposed_8x8(pack2<__half>(x[nt][2 * j] - f.x, x[nt][2 * j + 1] - f.y));
                         }
                     }
                 }
