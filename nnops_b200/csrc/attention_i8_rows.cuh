@@ -226,12 +226,13 @@ __device__ __forceinline__ bool wait_every_lane(uint64_t* bar, uint32_t parity, 
 
 // Bytes of shared memory: the warps' rings, which hold the warps' sums when a piece is joined; barriers; per-stage scales.
 // What a warp's queries and sums take, in values a lane has 32nd parts of; and by that blocks on an SM and warps of a block: 16 warps with
-// 128 registers a thread, 12 with 168 or 8 with 255.
+// 128 registers a thread, 12 with 168 or 8 with 255.  (24 rows of heads of 64, 16 sequences behind a window of 4096: 8 warps 41 us, 10
+// or 12, whose registers do not hold everything, 43 to 44.)
 constexpr int rows_weight(int64_t dim, int columns, bool split) { return static_cast<int>(dim) * columns * (split ? 3 : 2) / 2; }
 constexpr int rows_blocks(int64_t dim, int columns, bool split) { return columns == 1 && rows_weight(dim, columns, split) <= 128 ? 2 : 1; }
 constexpr int rows_warps(int64_t dim, int columns, bool split)
 {
-    return rows_blocks(dim, columns, split) == 1 && rows_weight(dim, columns, split) <= 192 ? 12 : 8;
+    return rows_blocks(dim, columns, split) == 1 && rows_weight(dim, columns, split) <= 128 ? 12 : 8;
 }
 
 // Beyond these the sums no longer fit the registers.

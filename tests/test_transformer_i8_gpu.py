@@ -318,6 +318,37 @@ def test_without_causality_and_with_a_scale(cuda_device, nnb200_lib, dtype, dim)
     _check_attention(_gen(dim), dtype, 2, 4, dim, 32, [3, 100, 0, 65], [7, 30, 1, 2], causal=False, scale=0.03)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,group,new", [(64, 2, 3, 5), (128, 1, 8, 1), (128, 2, 4, 9), (96, 1, 5, 7), (256, 1, 3, 3), (64, 1, 1, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (33, 5), (300, 40)])
+def test_as_many_rows_in_every_sequence(cuda_device, nnb200_lib, dtype, dim, heads, group, new, window, sinks):
+    """Without cu, few row tiles and a short table: a cluster of blocks for each.  With cu, one line for all: the same to a rounding or two."""
+    g = _gen(dim + new)
+    lens = [new, 0, 1, 777, 1500]
+    if heads * group * new > 60:
+        lens = lens[2:]
+    got = _check_attention(g, dtype, heads, group, dim, 16, lens, [new] * len(lens), window=window, sinks=sinks, uniform=True, engine="rows")
+    assert got.isfinite().all()
+    _check_attention(_gen(dim + new), dtype, heads, group, dim, 16, lens, [new] * len(lens), window=window, sinks=sinks, engine="rows")
+
+
+@pytest.mark.parametrize("tokens", [15, 16, 17, 127, 129, 1024, 9000])
+def test_one_sequence_of_any_length(cuda_device, nnb200_lib, tokens):
+    """A cluster whose blocks have many groups, one or none; a table too wide for clusters; every kernel has it right."""
+    for dtype in TYPES:
+        _check_attention(_gen(tokens), dtype, 2, 2, 64, 16, [tokens], [1], uniform=True)
+    g = _gen(tokens)
+    table, pages = _tables(g, [tokens], 16)
+    cache = _filled(g, pages, 2, 16, 64)
+    q = _randn(g, 1, 4, 64).half()
+    want, tol = _attention_reference(q, cache, table, [tokens], [0, 1], 2, True, 0, 0, 1 / 8)
+    wide = torch.full((1, 2000), -1, dtype=torch.int32, device="cuda")
+    wide[:, : len(table[0])] = _i32(table)
+    for engine in ("auto", "rows", "tile"):
+        got = ops.attention_i8_cache(q.cuda(), cache, wide, _i32([tokens]), engine=engine)
+        assert ((got.cpu().double() - want).abs() <= tol).all(), engine
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("dim,new", [(128, 300), (64, 513), (96, 150), (256, 140)])
 def test_prompts(cuda_device, nnb200_lib, dtype, dim, new):
