@@ -538,7 +538,7 @@ typedef struct nnb200_cache_i8 {
  * not overwritten becomes round_half_even(code * (old / new)).  New codes: round_half_even(x * (1 / scale)).  A NaN or
  * an infinity among the new values makes the page's scale NaN until it begins anew: every value of it then reads as NaN.
  * A page that a call writes belongs to one sequence, and stands once in its row of the table: otherwise what
- * it holds afterwards is not defined.
+ * it holds afterwards is not defined.  Rows that read writes may not overlap.
  */
 typedef struct nnb200_cache_rows_args {
     nnb200_cache_i8 cache;
@@ -556,10 +556,12 @@ NNB200_API int nnb200_cache_read_i8(const nnb200_cache_rows_args* args, void* st
  * and query head a over the keys and values of head a / (q_heads / heads):
  *   out = sum_j softmax_j(scale * q . k_j) v_j   over the visible tokens j < lens[b]:
  *   causal: j <= p, and with window > 0 also j > p - window or j < sinks; else all of them.
- * A row that sees no token gives zeros.  dim 64, 96, 128 or 256.  The products take q and the softmax weights as f16,
- * each row's q scaled by a power of two (f32 q: as the sum of two f16 values, 2^-22 of the row's largest), codes exactly, and
- * sum in f32; the softmax is f32.  A block whose v scale is under 2^-60 counts as having that scale.
- * The workspace (16-byte aligned device memory) is dead when the call's work has completed on the stream.
+ * A row that sees no token gives zeros, whatever its q holds.  dim 64, 96, 128 or 256.  The products take q and the softmax weights as
+ * f16 (f16 q as it is, bf16 q scaled by a power of two of its row's, f32 q and its weights as the sum of two f16 values, 2^-22 of the
+ * row's largest; weights relative to a running maximum, 2^8 at most), codes exactly, and sum in f32; the softmax is
+ * f32.  A page whose v scale is under 2^-60 counts as having that scale.  Rows of out may not overlap, nor any of them an input.
+ * The workspace is 16-byte aligned device memory of as many bytes as the query says for the same call, which may be none (then NULL);
+ * calls that may run at the same time need one each, and it is dead when the call's work has completed on the stream.
  */
 typedef struct nnb200_attention_i8_args {
     nnb200_cache_i8 cache;

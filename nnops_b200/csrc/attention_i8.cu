@@ -9,6 +9,7 @@ namespace {
 constexpr int kEngineRows = 1;
 constexpr int kEngineTile = 2;
 constexpr int64_t kClusterTokens = 16384;
+constexpr int64_t kMostTokens = int64_t{1} << 31;   // a sequence has fewer
 
 // Query rows that share a sequence's head, on average where their numbers are the device's.
 int64_t rows_each(const nnb200_attention_i8_args& a)
@@ -68,6 +69,7 @@ RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
 // Where the parts of the tile kernels' workspace lie, each at a multiple of 16 bytes.
 struct TilePlan {
     size_t tiles, first_tile, pieces, sums, bytes;   // the line's lengths are at 0
+    int64_t most_tiles;
 };
 
 TilePlan tile_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
@@ -78,6 +80,7 @@ TilePlan tile_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
     const auto up = [](size_t v) { return (v + 15) / 16 * 16; };
     const size_t pieces = 2 * static_cast<size_t>(dev.sm_count);
     TilePlan p;
+    p.most_tiles = most;
     p.tiles = 16;
     p.first_tile = p.tiles + up(static_cast<size_t>(most) * sizeof(TileInfo));
     p.pieces = p.first_tile + up(static_cast<size_t>(c.seqs + 1) * sizeof(int32_t));
@@ -127,6 +130,7 @@ int run_tile(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStrea
     call.wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.out_stride_row % 16 == 0 && a.out_stride_head % 16 == 0 ? 1 : 0;
     call.page_shift = page_shift(a);
     uint8_t* const base = static_cast<uint8_t*>(a.workspace);
+    call.most_tiles = p.most_tiles;
     call.line = reinterpret_cast<int64_t*>(base);
     call.tiles = reinterpret_cast<TileInfo*>(base + p.tiles);
     call.first_tile = reinterpret_cast<int32_t*>(base + p.first_tile);
@@ -149,7 +153,10 @@ size_t attention_i8_workspace_bytes(const nnb200_attention_i8_args& a, const Dev
 
 int launch_attention_i8(const nnb200_attention_i8_args& a, const DeviceInfo& dev, cudaStream_t stream)
 {
-    return engine_of(a) == kEngineTile ? run_tile(a, dev, stream) : run_rows(a, dev, stream);
+    nnb200_attention_i8_args bounded = a;   // a window beyond every token is none; differences of positions and it stay within 64 bits
+    bounded.window = a.window < kMostTokens ? a.window : kMostTokens;
+    bounded.sinks = a.sinks < kMostTokens ? a.sinks : kMostTokens;
+    return engine_of(a) == kEngineTile ? run_tile(bounded, dev, stream) : run_rows(bounded, dev, stream);
 }
 
 }  // namespace nnb200

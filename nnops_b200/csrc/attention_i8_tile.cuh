@@ -56,6 +56,7 @@ struct TileCall {
     int wide;             // q's and out's rows and heads are 16-byte aligned
     int wide_out;         // out's 32-byte aligned
     int page_shift;       // log2 of the tokens of a page
+    int64_t most_tiles;   // that `tiles` has room for: as many as the rows can make, unless `cu` names some of them twice
     int64_t* line;        // [0] tiles, [1] length of all tiles, of one head
     TileInfo* tiles;
     int32_t* first_tile;  // [seqs + 1]: tiles before each sequence's
@@ -136,15 +137,17 @@ __global__ void __launch_bounds__(1024) attention_i8_plan_kernel(const TileCall 
         }
         const int64_t first = tiles + before((s.n * call.group + ROWS - 1) / ROWS, total);
         if (b < seqs) {
-            call.first_tile[b] = static_cast<int32_t>(first);
+            const int held = static_cast<int>(min(first, call.most_tiles));
+            call.first_tile[b] = held;
             if (b < kKept) {
-                kept_first[b] = static_cast<int>(first);
+                kept_first[b] = held;
                 kept_rows[b] = s;
             }
         }
         tiles += total;
     }
     __syncthreads();
+    tiles = min(tiles, call.most_tiles);
     int64_t line = 0;
     for (int i0 = 0; i0 < tiles; i0 += 1024) {
         const int i = i0 + static_cast<int>(threadIdx.x);
@@ -900,7 +903,8 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             for (int j = 0; j < count; ++j, ++n) {
                 // Lanes 0..7 have a group each.
                 const int idx = (off + j) * kTileGroups + lane;
-                GroupMeta of{0.0f, -INFINITY, 0.0f, 0};
+                // Where there is no group, or no page: behind every token, so that not even a query that is no number makes a weight of it.
+                GroupMeta of{0.0f, -INFINITY, 0.0f, 0x7FFFFFF0 | (kHalves == 2 ? 3 : 1)};
                 int64_t at = -1;
                 if (lane < kTileGroups && idx < range.groups) {
                     const int key0 = (idx < range.sink_groups ? idx : idx - range.sink_groups + range.first_group) * 16;
@@ -922,7 +926,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                     }
                 }
                 // A scale below zero turns the order of its scores round: those too are looked at one by one.
-                const int odd = __reduce_or_sync(0xFFFFFFFFu, (of.key0 & 3) | (of.k * call.factor < 0.0f ? 3 : 0));
+                const int odd = __reduce_or_sync(0xFFFFFFFFu, lane >= kTileGroups ? 0 : (of.key0 & 3) | (of.k * call.factor < 0.0f ? 3 : 0));
                 const uint32_t slot = n % kMetaSlots;
                 if (!wait_every_lane(&meta_empty[slot], (n / kMetaSlots & 1) ^ 1, &abort_flag)) {
                     ok = false;

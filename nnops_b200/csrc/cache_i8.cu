@@ -73,9 +73,9 @@ __device__ __forceinline__ Unit find_unit(const nnb200_cache_i8& c, int place, i
     u.row = s.row0 + (start + u.from) - (s.len - s.n);
     u.begins = u.from == 0 && start >= first;
     u.page = page_at(c, b, static_cast<int>(slot), error_word);
-    if (u.page < 0) {   // the tokens' rows have no page
-        u.zero_row = u.row;
-        u.zero_rows = u.to - u.from;
+    if (u.page < 0) {   // the tokens' rows have no page; rows without a token stand directly before them
+        u.zero_row = u.row - u.zero_rows;
+        u.zero_rows += u.to - u.from;
     }
     return u;
 }

@@ -1212,6 +1212,15 @@ int check_cache(const nnb200_cache_i8& c, bool* empty)
     return NNB200_OK;
 }
 
+// Whether two of an output's rows of `dim` values, heads to a row, could be the same memory.
+bool rows_overlap(int64_t rows, int64_t stride_row, int64_t heads, int64_t stride_head, int64_t dim)
+{
+    if (rows == 1 || heads == 1) {
+        return rows * heads > 1 && (rows > 1 ? stride_row : stride_head) < dim;
+    }
+    return stride_row < stride_head ? stride_row < dim || stride_head / rows < stride_row : stride_head < dim || stride_row / heads < stride_head;
+}
+
 int check_cache_rows(const nnb200_cache_rows_args* a, bool* empty)
 {
     if (a == nullptr || !float_type_ok(a->float_type)) {
@@ -1250,14 +1259,15 @@ int check_attention(const nnb200_attention_i8_args* a, bool* empty)
     if (c.dim != 64 && c.dim != 96 && c.dim != 128 && c.dim != 256) {
         return NNB200_UNSUPPORTED;
     }
-    if (c.rows > 0x7FFFFFFF / (a->q_heads / c.heads)) {
+    if (c.rows > (0x7FFFFFFF - 1024) / (a->q_heads / c.heads)) {   // a tile's last row is counted in 32 bits
         return NNB200_UNSUPPORTED;
     }
     if (*empty) {
         return NNB200_OK;
     }
     const uintptr_t bytes = float_bytes(a->float_type);
-    if (a->q == nullptr || a->out == nullptr || !aligned(a->q, bytes) || !aligned(a->out, bytes)) {
+    if (a->q == nullptr || a->out == nullptr || !aligned(a->q, bytes) || !aligned(a->out, bytes) ||
+        rows_overlap(c.rows, a->out_stride_row, a->q_heads, a->out_stride_head, c.dim)) {
         return NNB200_INVALID_ARGUMENT;
     }
     return NNB200_OK;
@@ -1311,6 +1321,10 @@ int nnb200_cache_read_i8(const nnb200_cache_rows_args* args, void* stream)
     const int status = check_cache_rows(args, &empty);
     if (status != NNB200_OK || empty) {
         return status;
+    }
+    const nnb200_cache_i8& c = args->cache;
+    if (rows_overlap(c.rows, args->k_stride_row, c.heads, args->k_stride_head, c.dim) || rows_overlap(c.rows, args->v_stride_row, c.heads, args->v_stride_head, c.dim)) {
+        return NNB200_INVALID_ARGUMENT;
     }
     const DeviceInfo* dev = current_device_info();
     if (dev == nullptr) {

@@ -84,6 +84,19 @@ def test_attention_arguments(nnb200_lib):
     assert nnb200_lib.nnb200_attention_i8_workspace_bytes(None) == 0
 
 
+def test_outputs_whose_rows_overlap(nnb200_lib):
+    """rows = 6 of 2 heads (read) or 4 (attention) of 64 values."""
+    read, attention = nnb200_lib.nnb200_cache_read_i8, nnb200_lib.nnb200_attention_i8
+    for row, head in ((0, 64), (64, 64), (127, 64), (128, 0), (128, 63), (64, 383), (-128, 64)):
+        for name in "kv":
+            over = {f"{name}_stride_row": row, f"{name}_stride_head": head}
+            assert read(C.byref(_cache(capi.CacheRowsArgs, **over)), None) == capi.INVALID_ARGUMENT, over
+    for row, head in ((0, 64), (64, 64), (255, 64), (256, 63), (64, 383), (1, 1)):
+        over = dict(out_stride_row=row, out_stride_head=head)
+        assert attention(C.byref(_cache(capi.AttentionI8Args, **over)), None) == capi.INVALID_ARGUMENT, over
+    assert attention(C.byref(_cache(capi.AttentionI8Args, rows=1, seqs=1, cu=None, out_stride_row=0, out_stride_head=63)), None) == capi.INVALID_ARGUMENT
+
+
 def test_blocks_agree_with_the_header():
     assert C.sizeof(capi.CacheRowsArgs) == 17 * 8 + 6 * 8 + 8
     assert C.sizeof(capi.AttentionI8Args) == 17 * 8 + 9 * 8 + 16 + 16

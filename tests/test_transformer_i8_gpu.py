@@ -1,5 +1,6 @@
 """RMS norm into 8 bits, the 8-bit key/value cache and the attention over it, against plain implementations: codes, scales and
 values read back bit for bit, sums against 64 bits."""
+import ctypes as C
 import math
 
 import pytest
@@ -496,6 +497,87 @@ def test_what_is_masked_may_be_anything(cuda_device, nnb200_lib, dtype, engine):
     assert torch.equal(got[rest], want[rest])
 
 
+@pytest.mark.parametrize("engine", ["rows", "tile"])
+def test_rows_that_see_nothing_whatever_they_hold(cuda_device, nnb200_lib, engine):
+    """The padding of a batch: rows before their sequence's first token, and of sequences without one, give zeros."""
+    g = _gen(17)
+    for dim in (64, 256):
+        cache = _filled(g, 4, 1, 16, dim)
+        q = _randn(g, 12, 2, dim).half().cuda()
+        table, lens, cu = _i32([[0, 1], [2, 3]]), _i32([0, 5]), _i32([0, 4, 12])
+        want = ops.attention_i8_cache(q, cache, table, lens, cu=cu, engine=engine)
+        assert (want[:7] == 0).all() and (want[7:] != 0).any()
+        for bad in (math.nan, math.inf):
+            q[:7] = bad
+            assert torch.equal(ops.attention_i8_cache(q, cache, table, lens, cu=cu, engine=engine), want)
+            assert (ops.attention_i8_cache(q[:4], cache, table[:1], _i32([0]), causal=False, engine=engine) == 0).all()
+
+
+@pytest.mark.parametrize("engine", ["rows", "tile"])
+@pytest.mark.parametrize("window", [100, 2 ** 31, 2 ** 62, 2 ** 63 - 1])
+def test_a_window_beyond_everything(cuda_device, nnb200_lib, engine, window):
+    g = _gen(18)
+    cache = _filled(g, 4, 1, 16, 64)
+    q = _randn(g, 60, 2, 64).half().cuda()
+    for lens, cu in ((_i32([60]), None), (_i32([50]), None), (_i32([60]), _i32([0, 60]))):    # (50: ten rows stand before the sequence)
+        want = ops.attention_i8_cache(q, cache, _i32([[0, 1, 2, 3]]), lens, cu=cu, engine=engine)
+        for sinks in (0, 2 ** 63 - 1):
+            assert torch.equal(ops.attention_i8_cache(q, cache, _i32([[0, 1, 2, 3]]), lens, cu=cu, window=window, sinks=sinks, engine=engine), want)
+
+
+def test_no_page_for_a_sequence_that_begins_behind_rows_without_a_token(cuda_device, nnb200_lib):
+    """Read: rows before the sequence and rows whose first page is wrong are zeros, all of them."""
+    g = _gen(19)
+    cache = _filled(g, 3, 2, 16, 64)
+    out = tuple(torch.full((40, 2, 64), math.nan, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.cache_read_i8(cache, _i32([[-1, 2]]), _i32([20]), out=out)
+    assert capi.take_device_error() == capi.DEVICE_ERROR_BAD_PAGE
+    for x in out:
+        assert (x[:36] == 0).all() and x.isfinite().all() and (x[36:] != 0).any()
+
+
+@pytest.mark.parametrize("engine", [1, 2])
+def test_rows_that_several_sequences_claim(cuda_device, nnb200_lib, engine):
+    """`cu` that goes up and down: what such rows hold is not defined, but the workspace is enough and nobody else's rows change."""
+    g = _gen(20)
+    seqs, rows = 50, 600
+    cache = _filled(g, 4, 1, 16, 64)
+    q = _randn(g, rows + 8, 2, 64).half().cuda()
+    out = torch.full_like(q, 7.0)
+    table, lens, cu = _i32([[0, 1, 2, 3]] * seqs), _i32([64] * seqs), _i32([0, rows] * (seqs // 2) + [0])
+    a = capi.block(capi.AttentionI8Args, *ops._sequences(cache, table, lens, cu, rows), q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2], 2, 0, 0,
+                   0.125, 1, capi.FLOAT_F16, engine)
+    need = nnb200_lib.nnb200_attention_i8_workspace_bytes(C.byref(a))
+    space = torch.full((need + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = space.data_ptr(), need
+    capi.check(nnb200_lib.nnb200_attention_i8(C.byref(a), None), "nnb200_attention_i8")
+    torch.cuda.synchronize()
+    assert (space[need:] == 0x5A).all() and (out[rows:] == 7).all() and out.isfinite().all() and capi.take_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 96, 256])
+def test_strided_rows_in_tiles(cuda_device, nnb200_lib, dtype, dim):
+    """Queries and outputs off the 16-byte rule, and off the 32-byte one only; heads before rows."""
+    g = _gen(22)
+    lens, new, group = [500, 21], [290, 2], 3
+    table, pages = _tables(g, lens, 32)
+    cache = _filled(g, pages, 2, 32, dim)
+    rest = (_i32(table), _i32(lens))
+    dense = _randn(g, 292, 6, dim).to(dtype).cuda()
+    want = ops.attention_i8_cache(dense, cache, *rest, cu=_i32(_cu(new)), engine="tile")
+    for shape, at in (((292, 6, dim + 3), 1), ((292, 6, dim + 8), 8)):
+        q = torch.zeros(shape, dtype=dtype, device="cuda")[..., at: at + dim].copy_(dense)
+        out = torch.full(shape, 9.0, dtype=dtype, device="cuda")
+        got = ops.attention_i8_cache(q, cache, *rest, cu=_i32(_cu(new)), out=out[..., at: at + dim], engine="tile")
+        assert torch.equal(got, want) and (out[..., :at] == 9).all() and (out[..., at + dim:] == 9).all()
+    turned = dense.transpose(0, 1).contiguous().transpose(0, 1)
+    out = torch.empty((6, 292, dim), dtype=dtype, device="cuda").transpose(0, 1)
+    for engine in ("tile", "rows"):
+        got = ops.attention_i8_cache(turned, cache, *rest, cu=_i32(_cu(new)), out=out, engine=engine)
+        assert torch.equal(got, want if engine == "tile" else ops.attention_i8_cache(dense, cache, *rest, cu=_i32(_cu(new)), engine="rows"))
+
+
 def test_lengths_and_pages_that_are_wrong(cuda_device, nnb200_lib):
     """Nothing outside the arrays is touched: wrong pages are left out and recorded, wrong lengths and rows are cut."""
     g = _gen(2)
@@ -559,6 +641,42 @@ def test_captured_calls_follow_their_arrays(cuda_device, nnb200_lib):
         assert _same(cache, plain)
         want, tol = _attention_reference(fresh[0].half(), cache, table.tolist(), lens.tolist(), [0, 1, 2, 3], group, True, 0, 0, 1 / math.sqrt(dim))
         assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("engine,new", [("tile", 90), ("rows", 2)])
+def test_two_graphs_and_eager_calls_between_them(cuda_device, nnb200_lib, engine, new):
+    """Captured calls whose tables, lengths and rows change between replays; two graphs on two streams at once, and eager calls on a third:
+    each has a workspace of its own."""
+    g = _gen(23)
+    heads, group, dim, tokens, seqs = 2, 4, 64, 32, 3
+    table, pages = _tables(g, [2000, 1500, 900], tokens)
+    cache = _filled(g, pages, heads, tokens, dim)
+    table = _i32(table)
+    streams, graphs, calls = [torch.cuda.Stream() for _ in range(3)], [], []
+    for i in range(2):
+        lens, cu, q = _i32([1, 1, 1]), _i32([0, 1, 2, 3]), torch.zeros((seqs * new, heads * group, dim), dtype=torch.float16, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out = ops.attention_i8_cache(q, cache, table, lens, cu=cu, engine=engine)
+        graphs.append(graph)
+        calls.append((q, lens, cu, out))
+    for step in range(6):
+        want = []
+        for i, (q, lens, cu, out) in enumerate(calls):
+            q.copy_(_randn(g, *q.shape))
+            lens.copy_(torch.tensor([2000 - 300 * step, 10 + 200 * step, 900 - i]))
+            cu.copy_(torch.tensor([0, new - step % 2, 2 * new - step % 2, 3 * new]))
+            out.zero_()
+            want.append(ops.attention_i8_cache(q, cache, table, lens, cu=cu, engine=engine))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = ops.attention_i8_cache(calls[0][0], cache, table, calls[0][1], cu=calls[0][2], engine=engine)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0]) and all(torch.equal(call[3], w) for call, w in zip(calls, want)), step
 
 
 @pytest.mark.parametrize("name", ["norm", "norm, residual", "norm, buffers", "write", "read", "attention", "attention, window"])
