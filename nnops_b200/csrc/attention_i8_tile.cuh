@@ -427,10 +427,12 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         const uint32_t o_addr = tmem + static_cast<uint32_t>((warp & 3) * 32 << 16) + static_cast<uint32_t>(Shared::kOutColumn + half * 128);
         uint32_t n = 0;   // blocks
         int kinds[2] = {0, 0};
-        // The row of the part that is next: its place in out, its range of tokens, its factor.
+        // The row of the part that is next: its place in out, its tokens (those before `end`, and not before `low` unless before
+        // `sinks`), its factor.
         bool there = false;
-        int pos = 0;
-        int64_t low = 0, place = 0;
+        int end = 0, low = 0;
+        const int sinks = static_cast<int>(min(a.sinks, int64_t{0x7FFFFFFF}));
+        int64_t place = 0;
         float factor = 0.0f;
         const auto load_queries = [&] {
             const int first = walk.info.tile * kRows + half * 128 + (warp & 3) * 32, all = walk.info.n * call.group;
@@ -440,9 +442,9 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             };
             there = first + lane < all;
             place = there ? source(lane, a.out_stride_row, a.out_stride_head) : 0;
-            pos = a.causal != 0 ? walk.info.len - walk.info.n + (first + lane) / call.group : 0x7FFFFFFF;
-            pos = pos < walk.info.len ? pos : walk.info.len - 1;
-            low = a.window > 0 && there ? static_cast<int64_t>(pos) - a.window + 1 : INT64_MIN;
+            const int pos = walk.info.len - walk.info.n + (first + lane) / call.group;
+            end = a.causal != 0 && pos < walk.info.len ? max(pos + 1, 0) : walk.info.len;
+            low = a.window > 0 ? static_cast<int>(max(end - a.window, int64_t{0})) : 0;
             factor = call.factor;
             // Four lanes to a row, eight rows at a time: 64 bytes of each next to each other.  All are asked for before any is looked at.
             uint4 raw[4][D / 32];
@@ -587,16 +589,19 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
 #pragma unroll 1
                     for (int g = 0; g < kPartGroups; ++g) {
                         const GroupMeta of = groups[g];
-                        uint32_t s[16];
-                        tile_tmem_ld_16(part_addr + static_cast<uint32_t>(g * 16), s);
-                        tmem_ld_wait();
-                        const bool masked = (of.key0 >> half & 1) != 0;
                         const int key0 = of.key0 & ~15;
+                        const auto first_bits = [&](int tokens) { return (1u << min(max(tokens - key0, 0), 16)) - 1u; };
+                        // A bit for each token that the row sees.
+                        const uint32_t seen = (of.key0 >> half & 1) == 0 ? 0xFFFFu : first_bits(end) & (~first_bits(low) | first_bits(sinks));
+                        uint32_t s[16];
+                        if (__any_sync(0xFFFFFFFFu, seen != 0)) {
+                            tile_tmem_ld_16(part_addr + static_cast<uint32_t>(g * 16), s);
+                            tmem_ld_wait();
+                        }
+                        const float k = of.k * factor;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const int key = key0 + e;
-                            const float t = __fmaf_rn(__uint_as_float(s[e]), of.k * factor, of.v_log2);
-                            s[e] = __float_as_uint(!masked || (key <= pos && (key >= low || key < a.sinks)) ? t : -INFINITY);
+                            s[e] = (seen >> e & 1) != 0 ? __float_as_uint(__fmaf_rn(__uint_as_float(s[e]), k, of.v_log2)) : __float_as_uint(-INFINITY);
                         }
                         tile_tmem_st_16(part_addr + static_cast<uint32_t>(g * 16), s);
                     }
