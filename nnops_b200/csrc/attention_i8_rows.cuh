@@ -163,6 +163,24 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[WORDS
     }
 }
 
+// Where a token's 16 codes number `chunk` lie in a stage.  A product takes a chunk of 8 x 4 lanes at a time: for keys each of eight
+// tokens' chunks of four places, for values the chunks of eight places of each of four tokens.  In rows one behind the other these are in
+// the same banks (heads of 128: 2 and 4 times over); so the chunks of a row change places by the row's number, and each
+// access takes as long as its bytes.  Heads of 96, whose rows begin in different banks, stay as they are.
+template <int D>
+__device__ __forceinline__ int code_offset(int row, int chunk)
+{
+    if constexpr (D == 64) {
+        return (row >> 1) * 128 + (((row & 1) * 4 + chunk) ^ (row & 6)) * 16;
+    } else if constexpr (D == 128) {
+        return row * 128 + (chunk ^ (row & 7)) * 16;
+    } else if constexpr (D == 256) {
+        return row * 256 + (chunk >> 3) * 128 + ((chunk & 7) ^ (chunk >> 3) ^ ((row & 1) << 1 | (row >> 1 & 1) | (row & 4))) * 16;
+    } else {
+        return row * D + chunk * 16;
+    }
+}
+
 // Four words, or eight 16-bit values, as they are; `wide`: the address is 16-byte aligned.
 __device__ __forceinline__ uint4 four_words(const uint32_t* p, bool wide) { return wide ? *reinterpret_cast<const uint4*>(p) : make_uint4(p[0], p[1], p[2], p[3]); }
 __device__ __forceinline__ uint4 eight_of(const uint16_t* p, bool wide)
@@ -188,6 +206,37 @@ __device__ __forceinline__ void store_four(T* p, bool wide, float4 v)
         *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
     }
 }
+// This lane's part of a token's keys (those of `row`, dims [c D / 4, + D / 4)) and values (dims [g D / 8, + D / 8)).
+template <int D>
+__device__ __forceinline__ void load_keys(const uint8_t* stage, int row, int c, uint32_t (&w)[D / 16])
+{
+    if constexpr (D == 96) {
+        load_words(stage + row * D + c * (D / 4), w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + code_offset<D>(row, c * (D / 64) + i));
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ void load_values(const uint8_t* stage, int row, int g, uint32_t (&w)[D / 32])
+{
+    if constexpr (D == 96) {
+        load_words(stage + row * D + g * (D / 8), w);
+    } else if constexpr (D == 64) {
+        const uint2 v = *reinterpret_cast<const uint2*>(stage + code_offset<D>(row, g >> 1) + (g & 1) * 8);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + code_offset<D>(row, g * (D / 128) + i));
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    }
+}
+
 // sum / total, or zeros where nothing was seen.
 __device__ __forceinline__ void store_row(const RowsCall& call, int64_t i, float4 sum, float total)
 {
@@ -288,26 +337,15 @@ attention_i8_rows_kernel(const RowsCall call)
     constexpr int kTile = 8 * NT;
     constexpr int kParts = SPLIT ? 2 : 1;
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ __align__(8) uint64_t full[kWarps][kStages];
     __shared__ StageScales scales[kWarps][kStages];
     __shared__ float join_m[kWarps][kTile], join_l[kWarps][kTile];
     __shared__ int64_t scan[kWarps + 1];
     __shared__ int64_t found_base;
     __shared__ int64_t cut[3];   // of the line: blocks, the least share of one, how many groups are over
     __shared__ int found_seq;
-    __shared__ int abort_flag;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int g = lane / 4, c = lane & 3;
-    static_assert(kWarps * kStages <= kThreads, "a barrier a thread");
-    if (threadIdx.x < kWarps * kStages) {
-        mbar_init(&full[0][0] + threadIdx.x, 1);
-        mbar_init_fence();
-    }
-    if (threadIdx.x == 0) {
-        abort_flag = 0;
-    }
-    __syncthreads();
     previous_kernel_done();
     const nnb200_attention_i8_args& a = call.a;
     const int seqs = static_cast<int>(a.cache.seqs);
@@ -388,10 +426,8 @@ attention_i8_rows_kernel(const RowsCall call)
         base = found_base;
     }
 
-    uint32_t issued = 0;   // 16-token groups of this warp
-    uint32_t issue_slot = 0, slot = 0, round = 0;   // of the ring: the next to fill, the next to take and its turn
+    uint32_t issue_slot = 0, slot = 0;   // of the ring: the next to fill, the next to take
     uint8_t* const my_ring = ring + warp * kStages * Shared::kStageBytes;
-    bool failed = false;
 
     while (at < end) {
         SequenceWork work;
@@ -458,19 +494,21 @@ attention_i8_rows_kernel(const RowsCall call)
                     }
                 }
             }
+            const int64_t from = __shfl_sync(0xFFFFFFFFu, ahead, i & 31);
             if (lane == (i & 31)) {
-                uint64_t* const bar = &full[warp][issue_slot];
                 scales[warp][issue_slot] = StageScales{ahead_k, ahead_log2, ahead_inv, ahead >= 0 ? 1 : 0};
-                if (ahead >= 0) {
-                    uint8_t* const dst = my_ring + issue_slot * Shared::kStageBytes;
-                    mbar_expect_tx(bar, Shared::kStageBytes);
-                    bulk_load_1d(dst, static_cast<const uint8_t*>(a.cache.k) + ahead, 16 * D, bar);
-                    bulk_load_1d(dst + 16 * D, static_cast<const uint8_t*>(a.cache.v) + ahead, 16 * D, bar);
-                } else {
-                    mbar_arrive(bar);
+            }
+            if (from >= 0) {
+                uint8_t* const dst = my_ring + issue_slot * Shared::kStageBytes;
+                const uint8_t* const k = static_cast<const uint8_t*>(a.cache.k) + from + lane * 16;
+                const uint8_t* const v = static_cast<const uint8_t*>(a.cache.v) + from + lane * 16;
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    const int to = code_offset<D>((j * 32 + lane) / (D / 16), (j * 32 + lane) % (D / 16));
+                    cp_async_16(dst + to, k + j * 512, 16);
+                    cp_async_16(dst + 16 * D + to, v + j * 512, 16);
                 }
             }
-            ++issued;
             issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
         };
         // The query rows are asked for before the pages are looked up: this thread's part of row 8 nt + g, dims [c D / 4, + D / 4).
@@ -491,8 +529,12 @@ attention_i8_rows_kernel(const RowsCall call)
                 }
             }
         }
-        for (int i = 0; i < min(mine, kStages); ++i) {
-            issue(i);
+        // A group is committed for every turn, also without copies: what is waited for is then always the oldest of kStages.
+        for (int i = 0; i < kStages; ++i) {
+            if (i < mine) {
+                issue(i);
+            }
+            cp_async_commit();
         }
         // In f16, scaled by a power of two.
         uint32_t q[NT][kParts][D / 16][2];
@@ -561,10 +603,8 @@ attention_i8_rows_kernel(const RowsCall call)
         }
 
         for (int i = 0; i < mine; ++i) {
-            if (!wait_every_lane(&full[warp][slot], round, &abort_flag)) {
-                failed = true;
-                break;
-            }
+            cp_async_wait_group<kStages - 1>();
+            __syncwarp();
             const StageScales sc = scales[warp][slot];
             if (sc.there != 0) {
                 const uint8_t* kp = my_ring + slot * Shared::kStageBytes;
@@ -576,8 +616,8 @@ attention_i8_rows_kernel(const RowsCall call)
                 }
                 {
                     uint32_t x[D / 16], y[D / 16];
-                    load_words(kp + g * D + c * (D / 4), x);
-                    load_words(kp + (g + 8) * D + c * (D / 4), y);
+                    load_keys<D>(kp, g, c, x);
+                    load_keys<D>(kp + 8 * D, g, c, y);
 #pragma unroll
                     for (int w = 0; w < D / 16; ++w) {
                         uint32_t f[4];
@@ -673,10 +713,10 @@ attention_i8_rows_kernel(const RowsCall call)
                     }
                 }
                 uint32_t v0[D / 32], v1[D / 32], v2[D / 32], v3[D / 32];
-                load_words(vp + 2 * c * D + g * (D / 8), v0);
-                load_words(vp + (2 * c + 1) * D + g * (D / 8), v1);
-                load_words(vp + (2 * c + 8) * D + g * (D / 8), v2);
-                load_words(vp + (2 * c + 9) * D + g * (D / 8), v3);
+                load_values<D>(vp, 2 * c, g, v0);
+                load_values<D>(vp, 2 * c + 1, g, v1);
+                load_values<D>(vp + 8 * D, 2 * c, g, v2);
+                load_values<D>(vp + 8 * D, 2 * c + 1, g, v3);
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w) {
                     uint32_t e0[4], e1[4];
@@ -696,21 +736,9 @@ attention_i8_rows_kernel(const RowsCall call)
             if (i + kStages < mine) {
                 issue(i + kStages);
             }
-            if (++slot == kStages) {
-                slot = 0;
-                round ^= 1;
-            }
+            cp_async_commit();
+            slot = slot + 1 == kStages ? 0 : slot + 1;
         }
-        if (failed) {
-            if (lane == 0) {
-                atomicCAS(call.error_word, 0, kErrProducerWait);
-                if (!drain_ring(full[warp], kStages, issued)) {
-                    atomicCAS(call.error_word, 0, kErrDrainWait);
-                }
-            }
-            __syncwarp();
-        }
-
         // The warps' sums, joined through the ring: every copy into it has been taken.
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -823,7 +851,6 @@ attention_i8_rows_kernel(const RowsCall call)
             }
             call.pieces[blockIdx.x] = RowsPiece{static_cast<int32_t>(block - blockIdx.x), head, work.s.row0, tile * kTile, rows, {}};
         }
-        fence_proxy_async_smem();
         __syncthreads();
     }
 }
