@@ -80,6 +80,13 @@ __device__ __forceinline__ Unit find_unit(const nnb200_cache_i8& c, int place, i
     return u;
 }
 
+// Division of numbers up to 4096 (the vectors of a unit) by one up to 32: n / 2^20 of the rounded-up 2^20 / d is off by less than 1 / 256.
+struct Quotient {
+    uint32_t by;
+    __device__ __forceinline__ explicit Quotient(int d) : by(((1u << 20) + static_cast<uint32_t>(d) - 1u) / static_cast<uint32_t>(d)) {}
+    __device__ __forceinline__ int operator()(int n) const { return static_cast<int>(static_cast<uint32_t>(n) * by >> 20); }
+};
+
 template <int WARPS>
 __device__ __forceinline__ uint32_t largest_of_unit(uint32_t v)
 {
@@ -120,6 +127,7 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* erro
     const int t = threadIdx.x % kThreads;
     const int dim = static_cast<int>(c.dim), per_token = dim / 8;
     const int count = (u.to - u.from) * per_token;
+    const Quotient divided(per_token);
     const int64_t stride_row = u.values ? a.v_stride_row : a.k_stride_row;
     const T* src = static_cast<const T*>(u.values ? a.v : a.k) + u.row * stride_row + u.head * (u.values ? a.v_stride_head : a.k_stride_head);
     float* scale = (u.values ? c.v_scale : c.k_scale) + u.page * c.scale_page_stride + u.head;
@@ -131,7 +139,7 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* erro
     for (int i = 0; i < kVectors; ++i) {
         const int at = t + i * kThreads;
         if (at < count) {
-            const int token = at / per_token;
+            const int token = divided(at);
             x[i].load(src + token * stride_row + (at - token * per_token) * 8, wide != 0);
         }
     }
@@ -152,14 +160,15 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* erro
     float after = top >= kInfinityBits ? __uint_as_float(0x7FC00000u) : fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), kLeastCacheScale);
     after = before >= after || before != before ? before : after;
     const float inv = __frcp_rn(after);
+    const bool number = after == after;   // else codes are zeros
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
         const int at = t + i * kThreads;
         if (at < count) {
             float f[8];
             x[i].values(f);
-            *reinterpret_cast<uint2*>(codes + u.from * dim + at * 8) = make_uint2(codes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                                                                                 codes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+            *reinterpret_cast<uint2*>(codes + u.from * dim + at * 8) = make_uint2(number ? codes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv) : 0u,
+                                                                                 number ? codes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv) : 0u);
         }
     }
     if (after == before) {
@@ -175,8 +184,8 @@ cache_write_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* erro
             if (at < skip_from || at >= skip_to) {
                 uint2* p = reinterpret_cast<uint2*>(codes + at * 8);
                 const uint2 q = *p;
-                *p = make_uint2(codes4(code_at(q.x, 0) * ratio, code_at(q.x, 1) * ratio, code_at(q.x, 2) * ratio, code_at(q.x, 3) * ratio),
-                                codes4(code_at(q.y, 0) * ratio, code_at(q.y, 1) * ratio, code_at(q.y, 2) * ratio, code_at(q.y, 3) * ratio));
+                const auto four = [&](uint32_t w) { return number ? codes4(code_at(w, 0) * ratio, code_at(w, 1) * ratio, code_at(w, 2) * ratio, code_at(w, 3) * ratio) : 0u; };
+                *p = make_uint2(four(q.x), four(q.y));
             }
         }
     }
@@ -211,6 +220,7 @@ cache_read_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* error
         return;
     }
     const int count = (u.to - u.from) * per_token;
+    const Quotient divided(per_token);
     const float scale = (u.values ? c.v_scale : c.k_scale)[u.page * c.scale_page_stride + u.head];
     const int8_t* codes = static_cast<const int8_t*>(u.values ? c.v : c.k) + u.page * c.page_stride +
                           (static_cast<int64_t>(u.head) * c.page_tokens + u.from) * dim;
@@ -233,7 +243,7 @@ cache_read_kernel(const nnb200_cache_rows_args a, const int wide, int32_t* error
             for (int e = 0; e < 16; ++e) {
                 f[e] = code_at(w[e / 4], e & 3) * scale;
             }
-            const int token = at / per_token;
+            const int token = divided(at);
             store16(dst + token * stride_row + (at - token * per_token) * 16, f);
         }
     }

@@ -157,9 +157,13 @@ __device__ __forceinline__ uint32_t code_of(float v)
     return static_cast<uint32_t>(q) & 0xFFu;
 }
 
+// The same of four values of which each rounds to a code: added to 1.5 * 2^23 they are rounded to an integer, whose low byte is the code.
+// (Conversions take four times an addition's time.)
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d)
 {
-    return code_of(a) | (code_of(b) << 8) | (code_of(c) << 16) | (code_of(d) << 24);
+    constexpr float kInteger = 12582912.0f;
+    const auto bits = [](float v) { return __float_as_uint(__fadd_rn(v, kInteger)); };
+    return __byte_perm(__byte_perm(bits(a), bits(b), 0x0040), __byte_perm(bits(c), bits(d), 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ float code_at(uint32_t word, int byte) { return static_cast<float>(static_cast<int8_t>(word >> (8 * byte))); }

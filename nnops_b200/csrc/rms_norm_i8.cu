@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(THREADS) rms_norm_i8_kernel(const nnb200_rms_n
     for (int i = 0; i < VECS; ++i) {
         const int at = t + i * per_row;
         if (at < vectors) {
-            const uint2 q = make_uint2(codes4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv),
-                                       codes4(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv));
+            const uint2 q = make_uint2(inv != 0.0f ? codes4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv) : 0u,
+                                       inv != 0.0f ? codes4(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv) : 0u);
             *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.out) + row * a.out_stride + at * 8) = q;
         }
     }
