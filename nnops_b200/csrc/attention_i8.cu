@@ -8,6 +8,9 @@ namespace {
 
 constexpr int kEngineRows = 1;
 constexpr int kEngineTile = 2;
+// Clusters or the line with its second kernel, us, heads of 128, 8 of them: one sequence of 4096, 8192, 16384 and 32768 tokens 9.3 / 14.7, 12.4 / 17.4,
+// 18.8 / 19.4 and 31.7 / 23.9; two of 4096, 8192 and 16384 12.1 / 15.7, 17.1 / 17.5 and 27.3 / 21.8; four 12.4 / 16.6, 17.3 / 21.0 and 28.6 / 35.4.
+// What is known here is the table's reach, which sequences seldom fill.
 constexpr int64_t kClusterTokens = 16384;
 constexpr int64_t kMostTokens = int64_t{1} << 31;   // a sequence has fewer
 
@@ -47,15 +50,16 @@ RowsPlan rows_plan(const nnb200_attention_i8_args& a, const DeviceInfo& dev)
     const int64_t tiles = (rows + 8 * most - 1) / (8 * most);
     p.columns = static_cast<int>((rows + 8 * tiles - 1) / (8 * tiles));
     p.blocks = dev.sm_count * rows_blocks(c.dim, p.columns, split);
-    // Clusters where all of them are under way at once and a warp has few groups whatever the lengths are: the most that the table,
-    // or the window, has room for.
+    // Clusters where a warp has few groups whatever the lengths are: the most that the table, or the window, has room for.
     int64_t most_tokens = c.table_pages * c.page_tokens;
     if (a.window > 0 && a.window < most_tokens) {
         const int64_t seen = a.window + (a.sinks < most_tokens ? a.sinks : most_tokens) + c.rows / c.seqs + 32;
         most_tokens = seen < most_tokens ? seen : most_tokens;
     }
-    const int64_t clusters = c.seqs * c.heads * tiles;
-    p.tiles = c.cu == nullptr && clusters * kRowsCluster <= p.blocks && most_tokens <= kClusterTokens ? static_cast<int>(tiles) : 0;
+    // And where all of them are under way at once.  Eight blocks have to be on neighbouring SMs, so not every SM finds a cluster that it
+    // fits: 32 of two blocks to an SM do, 16 of one do not (32 rows of 128 over 4096 tokens 22.0 us, on the line 15.8), 8 do.
+    const int64_t clusters = c.seqs * c.heads * tiles, room = p.blocks > dev.sm_count ? p.blocks / 8 * 7 : p.blocks / 2;
+    p.tiles = c.cu == nullptr && clusters * kRowsCluster <= room && most_tokens <= kClusterTokens ? static_cast<int>(tiles) : 0;
     if (p.tiles > 0) {
         p.blocks = static_cast<int>(clusters) * kRowsCluster;
         p.bytes = 0;

@@ -10,22 +10,27 @@
 // One pass over the tokens, with the running maximum; the sums are rescaled only when that has grown by more than 2^8, so
 // weights are at most 2^8, and the lanes of a row compare their maxima only then.
 //
-// A warp takes 16 tokens at a time and is on its own: it copies their codes into its part of shared memory
-// (cp.async.bulk; 16 tokens never leave a page, and one head's share of a page is contiguous), turns bytes into f16
+// A warp takes 16 tokens at a time and is on its own: it copies their codes into its part of shared memory, a few groups ahead
+// (16 tokens never leave a page, and one head's share of a page is contiguous), turns bytes into f16
 // integers, which is exact, and feeds mma.m16n8k16 with the TOKENS as the 16-row operand: eight query rows (the heads
 // of a group, a few proposed tokens) fill the narrow side, nothing is padded to 16 or 128.  The transposition between the
 // two products is one movmatrix for 8 x 8 weights.  The order along dim and along the tokens inside an MMA is
-// free, and chosen so that every thread's bytes are contiguous.
+// free, and chosen so that every thread's bytes are contiguous; where 16-byte pieces lie in shared memory is, too (code_offset),
+// which is why the lanes copy 16 bytes each instead of one lane a block: with the rows as they come, accesses to shared memory took
+// three times as long and the kernel 7 to 14 % longer.
 //
-// Bound by the reading of the codes: D bytes of K and of V for a token and head, against some 300 instructions of a warp for
-// 16 tokens.
+// Bound by the reading of the codes, 2 D bytes for a token and head, and close behind it by instructions: about 280 of a warp for 16
+// tokens of 64 dims and 8 rows, 370 of 128 dims, 60 more for each 8 rows more.  Measured on one B200: 64 sequences of 64 to 8192 tokens, 8 heads of
+// 128, 8 rows: 95.5 us, 5.7 TB/s (0.88 of the measured copy rate; 107 us with nothing left in L2); 64 sequences of 4096 tokens, 8 heads: heads of
+// 64 with 8, 16 and 32 rows 62, 87 and 132 us, heads of 128 with 8 rows 98 us; 16 sequences behind a window of 4096, 24 rows of 64: 37 us.
 //
 // The work of all sequences, row tiles and heads is one line of 16-token groups, cut into equal pieces, one for each block, so
 // that lengths of any mix keep every SM busy to the end.  A row tile of a head that is cut leaves (m, l, sums) in the
 // workspace, in a fixed order of blocks; a second kernel joins them, in that order: results do not depend on timing.
 //
 // A few row tiles over contexts that cannot be long, all sequences with as many rows, go to a cluster of eight blocks each instead:
-// their sums meet in shared memory, without a workspace, a search for one's place or a second kernel.
+// their sums meet in shared memory, without a workspace, a search for one's place or a second kernel.  One sequence of 4096 tokens, 8 heads of
+// 128: 9.1 us, with the line and its second kernel 14.
 #pragma once
 
 #include "cache_i8.cuh"
@@ -34,7 +39,9 @@
 namespace nnb200 {
 
 constexpr int kRowsThreads = 256; // of the joining kernel's blocks
-constexpr int kRowsCost = 32;         // groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps
+// Groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps.  With 16, 32 and 64, 8 heads of 128: 64 sequences of
+// 128 to 8192 tokens 114, 96 and 98 us, 255 of 16 to 128 and one of 30000 70, 65 and 78, 120 of 100 and 8 of 20000 94, 78 and 95.
+constexpr int kRowsCost = 32;
 constexpr float kGrowth = 8.0f;   // log2 of what a weight may be
 
 // A row tile of a head that begins in a block and ends in a later one.  What a block leaves of its sums: [0] the end or the middle of
@@ -251,7 +258,7 @@ __device__ __forceinline__ void store_row(const RowsCall& call, int64_t i, float
     }
 }
 
-// Every lane polls: the data behind the barrier is then every lane's.  Without a hint how long to sleep, which costs a
+// (For the tiles' kernel.)  Every lane polls: the data behind the barrier is then every lane's.  Without a hint how long to sleep, which costs a
 // hundred cycles on a barrier that is all but ready; within the limit that mbar_wait has.
 __device__ __forceinline__ bool wait_every_lane(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
 {
@@ -273,7 +280,6 @@ __device__ __forceinline__ bool wait_every_lane(uint64_t* bar, uint32_t parity, 
     return true;
 }
 
-// Bytes of shared memory: the warps' rings, which hold the warps' sums when a piece is joined; barriers; per-stage scales.
 // What a warp's queries and sums take, in values a lane has 32nd parts of; and by that blocks on an SM and warps of a block: 16 warps with
 // 128 registers a thread, 12 with 168 or 8 with 255.  (24 rows of heads of 64, 16 sequences behind a window of 4096: 8 warps 41 us, 10
 // or 12, whose registers do not hold everything, 43 to 44.)
@@ -288,12 +294,13 @@ constexpr int rows_warps(int64_t dim, int columns, bool split)
 constexpr int rows_most_columns(int64_t dim, bool split) { return split ? (dim > 128 ? 1 : 2) : dim > 128 ? 2 : dim > 96 ? 3 : 4; }
 
 template <int D, int NT, bool SPLIT>
-struct RowsShared {
+struct RowsShared {   // bytes of the warps' rings, which hold the warps' sums when a piece is joined
     static constexpr int kWarps = rows_warps(D, NT, SPLIT);
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kStageBytes = 2 * 16 * D;
     static constexpr int kJoinBytes = kWarps * 8 * NT * D * 4;
     static constexpr int kWanted = (rows_blocks(D, NT, SPLIT) == 2 ? 96 : 192) * 1024;
+    // Groups on their way or at work, of each warp.
     static constexpr int kStages = kWanted / (kWarps * kStageBytes) > 8 ? 8 : kWanted / (kWarps * kStageBytes);
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kSumBytes = 8 * NT * (D + 2) * 4;   // in a cluster: of a block

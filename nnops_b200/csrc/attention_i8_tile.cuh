@@ -8,16 +8,26 @@
 //     P = 2^(t - m)       a thread has a row: no exchange between threads; P f16 over S in tensor memory
 //     O += P V            P from tensor memory, V f16 in shared memory (its dim contiguous: the MN-major form)
 //
-// The cache stays in 8 bits up to the SM: four warps load codes, turn them into f16 integers (exact) and store them in the
+// The cache stays in 8 bits up to the SM: four warps copy codes, turn them into f16 integers (exact) and store them in the
 // 128-byte-swizzled order that the MMAs read.  That work serves 256 rows, and is done while the tensor cores and the two
 // groups of four softmax warps work on the block before.  The two halves of the rows alternate: one half's weights are computed while
-// the other half's products run.  Every block's scales come along in shared memory, one for each 16 tokens.
+// the other half's products run, and a half hands its weights over in two parts of 64 tokens, so that the products of the first run
+// while the second is computed.  One warp issues all MMAs, in the order that the halves take turns in: scores come over the weights whose
+// products it has issued before.  Another, the scout, looks up each block's pages and scales (one for each 16 tokens) ahead of everyone,
+// marks blocks that some row does not see all of, and asks for the queries that come next.  Softmax warps need more registers than
+// the rest: the groups of four trade them (152, 112 and 96 of a thread's; 128 at launch).
 //
 // The sums are rescaled only when a row's maximum has grown by more than 2^8 since they were last: until then weights are at
 // most 2^8, which f16 and the f32 sums hold as well as 1.
 //
 // Sequences, tiles and heads are one line of 128-token blocks, cut into equal pieces, as in attention_i8_rows.cuh; a first
 // kernel writes down which tiles there are.
+//
+// Bound by the chain from scores over weights to products, of which two are under way, on warps that issue in 46 % of the cycles; tensor cores, exponentials and
+// integer units are busy for 38 % of the time each.  Measured on one B200: 8192 rows of 32 heads of 128, causal: 650 us, 845 TFLOP/s (0.50 of the measured
+// bf16 rate); 8 chunks of 288 rows over 9216 tokens 398 us; 2048 rows 76 us; 8192 rows of 64: 545 us; 4096 of 256: 490 us.  Not faster: scores of 64
+// tokens at a time, also into tensor memory of their own (for heads of 64); one part or four instead of two; two threads to a row; a part of the exponentials as polynomials
+// (one in eight 2 % slower, half 13 %); one issuing warp for each half, which would also need an order between the two.
 #pragma once
 
 #include "attention_i8_rows.cuh"
@@ -29,7 +39,8 @@ constexpr int kTileGroups = kTileKeys / 16;
 constexpr int kParts = 2;       // of a block: the products of one with V run while the softmax is at the next
 constexpr int kPartKeys = kTileKeys / kParts;
 constexpr int kPartGroups = kPartKeys / 16;
-constexpr int kTileCost = 4;    // blocks that a part of a tile costs besides its own: queries, first products, sums
+// Blocks that a part of a tile costs besides its own: queries, first products, sums.  (2, 3, 8 and 12 were no faster.)
+constexpr int kTileCost = 4;
 constexpr int kMetaSlots = 4;   // blocks whose scales are kept: the one the softmax is at, and those the converters are ahead by
 
 // One tile of query rows, of every head.

@@ -6,7 +6,8 @@
 // scale does, and one pass over the row finds both what the sum and what the maximum need.  Squares are summed in
 // 64 bits, which no f32 row can overflow.
 //
-// Bound by memory: with f16 rows 2 + 2 + 2 + 1 bytes an element.  A row is held in registers by one block (one warp, four rows
+// Bound by memory: with f16 rows 2 + 2 + 2 + 1 bytes an element.  4096 rows of 8192 with a residual: 37 us, 6.3 TB/s (0.98 of the measured copy
+// rate); one row costs its launch.  A row is held in registers by one block (one warp, four rows
 // a block, where a row has few vectors), every vector loaded before any is used; rows off the 16-byte rule, or longer
 // than 1024 threads hold, are read twice by an element-at-a-time kernel with the same arithmetic.
 
