@@ -509,7 +509,8 @@ NNB200_API int nnb200_rms_norm_i8(const nnb200_rms_norm_i8_args* args, void* str
  * page_table, lens and cu are device arrays, so that a captured call follows them.  They are checked where they
  * are used: a page outside 0 .. pages - 1 is never touched, what a call wanted of it is left out (a write drops the
  * token, a read gives zeros, attention does not see its keys), and NNB200_DEVICE_ERROR_BAD_PAGE (9) is recorded for
- * nnb200_take_device_error; rows outside 0 .. rows - 1 are ignored.
+ * nnb200_take_device_error; rows outside 0 .. rows - 1 are ignored.  cu ascends: what a row that several sequences claim
+ * ends up with is not defined, here and in the outputs.
  */
 #define NNB200_DEVICE_ERROR_BAD_PAGE 9
 typedef struct nnb200_cache_i8 {
@@ -573,7 +574,7 @@ typedef struct nnb200_attention_i8_args {
     float scale;
     int32_t causal;
     int32_t float_type;       /* of q and out */
-    int32_t force_engine;     /* 0 auto, 1 few rows on warp MMAs, 2 tiles of 128 rows on tcgen05 (not f32) */
+    int32_t force_engine;     /* 0 auto, 1 few rows on warp MMAs, 2 tiles of rows on tcgen05 (not f32) */
     void* workspace;
     size_t workspace_bytes;
 } nnb200_attention_i8_args;

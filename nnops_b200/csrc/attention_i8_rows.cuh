@@ -20,7 +20,7 @@
 // three times as long and the kernel 7 to 14 % longer.
 //
 // Bound by the reading of the codes, 2 D bytes for a token and head, and close behind it by instructions: about 280 of a warp for 16
-// tokens of 64 dims and 8 rows, 370 of 128 dims, 60 more for each 8 rows more.  Measured on one B200: 64 sequences of 64 to 8192 tokens, 8 heads of
+// tokens of 64 dims and 8 rows, 440 of 128 dims, 50 to 75 more for each 8 rows more.  Measured on one B200: 64 sequences of 128 to 8192 tokens, 8 heads of
 // 128, 8 rows: 95.5 us, 5.7 TB/s (0.88 of the measured copy rate; 107 us with nothing left in L2); 64 sequences of 4096 tokens, 8 heads: heads of
 // 64 with 8, 16 and 32 rows 62, 87 and 132 us, heads of 128 with 8 rows 98 us; 16 sequences behind a window of 4096, 24 rows of 64: 37 us.
 //

@@ -26,7 +26,8 @@
 // Bound by the chain from scores over weights to products, of which two are under way, on warps that issue in 46 % of the cycles; tensor cores, exponentials and
 // integer units are busy for 38 % of the time each.  Measured on one B200: 8192 rows of 32 heads of 128, causal: 650 us, 845 TFLOP/s (0.50 of the measured
 // bf16 rate); 8 chunks of 288 rows over 9216 tokens 398 us; 2048 rows 76 us; 8192 rows of 64: 545 us; 4096 of 256: 490 us.  Not faster: scores of 64
-// tokens at a time, also into tensor memory of their own (for heads of 64); one part or four instead of two; two threads to a row; a part of the exponentials as polynomials
+// tokens at a time, also into tensor memory of their own (for heads of 64); one part instead of two; weights ahead of the maximum, made up for
+// afterwards; two threads to a row; what a row sees of a block applied to registers instead of to tensor memory; a part of the exponentials as polynomials
 // (one in eight 2 % slower, half 13 %); one issuing warp for each half, which would also need an order between the two.
 #pragma once
 
