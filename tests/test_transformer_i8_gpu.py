@@ -720,6 +720,67 @@ def test_same_bytes_from_the_python_code(cuda_device, nnb200_lib, monkeypatch, n
     assert len(got) == len(want) and all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("new,ragged", [(1, False), (1, True), (5, True), (90, True), (90, False)])
+def test_a_stream_of_steps_without_waiting(cuda_device, nnb200_lib, new, ragged, captured):
+    """Kernels that begin while the one before ends: each step's calls read what the last call wrote and write over what the one before it
+    read, buffers and scratch the same ones again and again.  With a synchronisation behind each call, without, and as one graph."""
+    g = _gen(31 + new)
+    seqs, width, heads, group, dim, tokens, steps = 4, 512, 2, 4, 64, 16, 6
+    rows = seqs * new
+    w_qkv = torch.randint(-127, 128, ((group + 2) * heads * dim, width), generator=g, dtype=torch.int32).to(torch.int8).cuda()
+    w_out = torch.randint(-127, 128, (width, heads * group * dim), generator=g, dtype=torch.int32).to(torch.int8).cuda()
+    norms = [(1 + 0.1 * _randn(g, width)).half().cuda() for _ in range(2)]
+    x0 = _randn(g, rows, width).half().cuda()
+    table = _i32(torch.randperm(seqs * 64, generator=g).view(seqs, 64).tolist())
+    starts = _i32([3, 200, 17, 64])
+    cu = _i32(_cu([new] * seqs)) if ragged else None
+    cache = ops.CacheI8.empty(seqs * 64, heads, tokens, dim, "cuda")
+    before = _randn(g, 284, heads, dim).half().cuda()
+    per_row, zeros = torch.full((rows,), 0.02, device="cuda"), torch.zeros(rows, dtype=torch.int8, device="cuda")
+
+    def chain(after):
+        ops.cache_write_i8(cache, before, before, table, starts, cu=_starts)
+        after()
+        x, lens, seen = x0.clone(), starts.clone(), []
+        codes, scale = torch.empty((rows, width), dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+        o = torch.empty((rows, heads * group, dim), dtype=torch.float16, device="cuda")
+        for _ in range(steps):
+            lens += new
+            ops.rms_norm_i8(x, norms[0], out=codes, scale=scale)
+            after()
+            qkv = ops.gemm_i8(codes, w_qkv, out_kind="f16", scale_a=scale, scale_w=1e-3).view(rows, -1, dim)
+            after()
+            ops.cache_write_i8(cache, qkv[:, heads * group: -heads], qkv[:, -heads:], table, lens, cu=cu)
+            after()
+            ops.attention_i8_cache(qkv[:, : heads * group], cache, table, lens, cu=cu, out=o)
+            after()
+            q = ops.quantize_linear(o.view(rows, -1), per_row, zeros)
+            after()
+            y = ops.gemm_i8(q, w_out, out_kind="f16", scale_a=0.02, scale_w=1e-3)
+            after()
+            ops.rms_norm_i8(y, norms[1], residual=x, residual_out=x, out=codes, scale=scale)
+            after()
+            seen += [codes.clone(), scale.clone(), x.clone(), o.clone(), ops.cache_read_i8(cache, table, lens, rows=rows, cu=cu)[1]]
+            after()
+        return seen + [cache.k.clone(), cache.v_scale.clone()]
+
+    _starts = _i32(_cu(starts.tolist()))
+    want = [t.clone() for t in chain(torch.cuda.synchronize)]
+    assert all(t.float().isfinite().all() for t in want) and not torch.equal(want[0], want[5])
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            got = chain(lambda: None)
+    for _ in range(4):
+        if captured:
+            graph.replay()
+        else:
+            got = chain(lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
 def test_a_block_of_a_model(cuda_device, nnb200_lib):
     """Norm, int8 product into q, k and v, cache, attention, int8 product, norm: a prompt and then tokens one by one."""
     g = _gen(21)
