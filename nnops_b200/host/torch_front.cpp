@@ -780,23 +780,29 @@ const int32_t* words(PyObject* o, int64_t dim, const c10::Device& dev)
     return static_cast<const int32_t*>(t.data_ptr());
 }
 
-// `handle`: CacheI8's device index, addresses, distances and sizes.
-void cache_of(nnb200_cache_i8& c, PyObject* handle, PyObject* table, PyObject* lens, PyObject* cu, int64_t rows, const c10::Device& dev)
+// `tensors`: CacheI8's codes of keys and of values, and their scales.
+void cache_of(nnb200_cache_i8& c, PyObject* const* tensors, PyObject* table, PyObject* lens, PyObject* cu, int64_t rows, const c10::Device& dev)
 {
-    if (!PyTuple_CheckExact(handle) || PyTuple_GET_SIZE(handle) != 11 || whole(PyTuple_GET_ITEM(handle, 0)) != dev.index()) {
+    const at::Tensor &k = plain(tensors[0], dev), &v = plain(tensors[1], dev), &k_scale = plain(tensors[2], dev), &v_scale = plain(tensors[3], dev);
+    if (k.scalar_type() != at::kChar || v.scalar_type() != at::kChar || k_scale.scalar_type() != at::kFloat || v_scale.scalar_type() != at::kFloat ||
+        k.dim() != 4 || k_scale.dim() != 2 || v.sizes() != k.sizes() || v.strides() != k.strides() || v_scale.sizes() != k_scale.sizes() ||
+        v_scale.strides() != k_scale.strides()) {
         elsewhere();
     }
-    const auto field = [&](int i) { return whole(PyTuple_GET_ITEM(handle, i)); };
-    c.k = reinterpret_cast<void*>(field(1));
-    c.v = reinterpret_cast<void*>(field(2));
-    c.k_scale = reinterpret_cast<float*>(field(3));
-    c.v_scale = reinterpret_cast<float*>(field(4));
-    c.pages = field(5);
-    c.page_stride = field(6);
-    c.scale_page_stride = field(7);
-    c.heads = field(8);
-    c.page_tokens = field(9);
-    c.dim = field(10);
+    c.pages = k.size(0);
+    c.heads = k.size(1);
+    c.page_tokens = k.size(2);
+    c.dim = k.size(3);
+    c.page_stride = k.stride(0);
+    c.scale_page_stride = k_scale.stride(0);
+    if (k_scale.size(0) != c.pages || k_scale.size(1) != c.heads || (c.heads > 1 && k_scale.stride(1) != 1) || k.stride(1) != c.page_tokens * c.dim ||
+        k.stride(2) != c.dim || k.stride(3) != 1) {
+        elsewhere();
+    }
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.k_scale = static_cast<float*>(k_scale.data_ptr());
+    c.v_scale = static_cast<float*>(v_scale.data_ptr());
     c.page_table = words(table, 2, dev);
     c.lens = words(lens, 1, dev);
     const at::Tensor& t = THPVariable_Unpack(table);
@@ -823,11 +829,11 @@ bool head_rows(const at::Tensor& t, int64_t rows, int64_t heads, int64_t dim)
     return t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == dim && t.stride(2) == 1;
 }
 
-PyObject* cache_rows(PyObject* handle, const at::Tensor& k, const at::Tensor& v, PyObject* table, PyObject* lens, PyObject* cu, bool write, const c10::Device& dev)
+PyObject* cache_rows(PyObject* const* tensors, const at::Tensor& k, const at::Tensor& v, PyObject* table, PyObject* lens, PyObject* cu, bool write, const c10::Device& dev)
 {
     nnb200_cache_rows_args a;
     std::memset(&a, 0, sizeof(a));
-    cache_of(a.cache, handle, table, lens, cu, k.size(0), dev);
+    cache_of(a.cache, tensors, table, lens, cu, k.size(0), dev);
     if (!head_rows(k, a.cache.rows, a.cache.heads, a.cache.dim) || !head_rows(v, a.cache.rows, a.cache.heads, a.cache.dim) ||
         v.scalar_type() != k.scalar_type()) {
         elsewhere();
@@ -846,43 +852,42 @@ PyObject* cache_rows(PyObject* handle, const at::Tensor& k, const at::Tensor& v,
     return tuple_of({k, v});
 }
 
-// cache_write_i8(handle, k, v, page_table, lens, cu)
+// cache_write_i8(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, page_table, lens, cu)
 PyObject* cache_write_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     return guarded([&]() -> PyObject* {
-        expect(nargs, 6);
-        const c10::Device dev = current_device(args[1]);
-        const at::Tensor& k = plain(args[1], dev);
+        expect(nargs, 9);
+        const c10::Device dev = current_device(args[4]);
+        const at::Tensor& k = plain(args[4], dev);
         if (k.dim() != 3) {
             elsewhere();
         }
-        return cache_rows(args[0], k, plain(args[2], dev), args[3], args[4], args[5], true, dev);
+        return cache_rows(args, k, plain(args[5], dev), args[6], args[7], args[8], true, dev);
     });
 }
 
-// cache_read_i8(handle, page_table, lens, rows, cu, out_dtype)
+// cache_read_i8(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, lens, rows, cu, out_dtype)
 PyObject* cache_read_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     return guarded([&]() -> PyObject* {
-        expect(nargs, 6);
-        const c10::Device dev = current_device(args[1]);
-        if (!PyTuple_CheckExact(args[0]) || PyTuple_GET_SIZE(args[0]) != 11) {
+        expect(nargs, 9);
+        const c10::Device dev = current_device(args[0]);
+        const at::Tensor& codes = plain(args[0], dev);
+        const int64_t rows = whole(args[6]);
+        const at::ScalarType type = dtype_of(args[8], at::kHalf);
+        if (codes.dim() != 4 || rows < 0 || float_type_of(type) < 0) {
             elsewhere();
         }
-        const int64_t rows = whole(args[3]), heads = whole(PyTuple_GET_ITEM(args[0], 8)), dim = whole(PyTuple_GET_ITEM(args[0], 10));
-        const at::ScalarType type = dtype_of(args[5], at::kHalf);
-        if (rows < 0 || float_type_of(type) < 0) {
-            elsewhere();
-        }
-        return cache_rows(args[0], empty({rows, heads, dim}, type, dev), empty({rows, heads, dim}, type, dev), args[1], args[2], args[4], false, dev);
+        const int64_t heads = codes.size(1), dim = codes.size(3);
+        return cache_rows(args, empty({rows, heads, dim}, type, dev), empty({rows, heads, dim}, type, dev), args[4], args[5], args[7], false, dev);
     });
 }
 
-// attention_i8_cache(q, handle, page_table, lens, cu, causal, window, sinks, scale, out, engine)
+// attention_i8_cache(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, lens, cu, causal, window, sinks, scale, out, engine)
 PyObject* attention_i8_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
     return guarded([&]() -> PyObject* {
-        expect(nargs, 11);
+        expect(nargs, 14);
         const c10::Device dev = current_device(args[0]);
         const at::Tensor& q = plain(args[0], dev);
         if (q.dim() != 3) {
@@ -890,24 +895,24 @@ PyObject* attention_i8_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         }
         nnb200_attention_i8_args a;
         std::memset(&a, 0, sizeof(a));
-        cache_of(a.cache, args[1], args[2], args[3], args[4], q.size(0), dev);
+        cache_of(a.cache, args + 1, args[5], args[6], args[7], q.size(0), dev);
         const int64_t rows = a.cache.rows, heads = q.size(1), dim = a.cache.dim;
         if (!head_rows(q, rows, heads, dim) || heads < 1 || a.cache.heads < 1 || heads % a.cache.heads != 0) {
             elsewhere();
         }
         a.float_type = float_type_of(q.scalar_type());
-        a.causal = flag(args[5], true) ? 1 : 0;
-        a.window = whole(args[6]);
-        a.sinks = whole(args[7]);
+        a.causal = flag(args[8], true) ? 1 : 0;
+        a.window = whole(args[9]);
+        a.sinks = whole(args[10]);
         if (a.window < 0 || a.sinks < 0 || (a.window > 0 && a.causal == 0)) {
             elsewhere();
         }
-        a.scale = args[8] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : static_cast<float>(number(args[8]));
+        a.scale = args[11] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim))) : static_cast<float>(number(args[11]));
         static const char* const automatic[] = {"auto"};
-        one_of(args[10], automatic, 0);
+        one_of(args[13], automatic, 0);
         at::Tensor out;
-        if (args[9] != Py_None) {
-            out = plain(args[9], dev);
+        if (args[12] != Py_None) {
+            out = plain(args[12], dev);
             if (!head_rows(out, rows, heads, dim) || out.scalar_type() != q.scalar_type()) {
                 elsewhere();
             }

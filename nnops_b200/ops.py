@@ -575,9 +575,16 @@ class CacheI8:
     """A key/value cache in 8 bits: codes s8 [pages, heads, page tokens, dim], dense within a page, and one f32 scale for each
     page and head [pages, heads] (see nnb200_cache_i8 in nnb200.h).  Which pages a sequence has is its caller's
     business: every call takes ``page_table`` int32 [seqs, n], ``lens`` int32 [seqs], the sequences' tokens with the call's
-    new ones, and, unless each sequence has the same number of rows, ``cu`` int32 [seqs + 1]."""
+    new ones, and, unless each sequence has the same number of rows, ``cu`` int32 [seqs + 1].  ``k``, ``v``, ``k_scale`` and ``v_scale`` may be
+    replaced, by a larger cache's for example; a captured call stays with those that it was captured with."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self._fields()
+
+    def _fields(self) -> tuple:
+        """What the calls hand on: addresses, pages, distances and sizes of the tensors as they are now."""
+        k, v, k_scale, v_scale = self.k, self.v, self.k_scale, self.v_scale
         if k.dim() != 4 or k.dtype != torch.int8 or v.dtype != torch.int8 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
             raise ValueError("codes must be int8 [pages, heads, page tokens, dim], scales f32 [pages, heads]")
         pages, heads, tokens, dim = k.shape
@@ -585,13 +592,25 @@ class CacheI8:
             raise ValueError("keys, values and scales must agree in pages, heads, page tokens and dim")
         if k.stride() != v.stride() or k_scale.stride() != v_scale.stride() or k.stride()[1:] != (tokens * dim, dim, 1) or (heads > 1 and k_scale.stride(1) != 1):
             raise ValueError("pages and their scales must be dense, those of values at the distances of those of keys")
-        if len({k.device, v.device, k_scale.device, v_scale.device}) != 1:
-            raise ValueError("keys, values and scales must be on one device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.pages, self.heads, self.page_tokens, self.dim, self.device = pages, heads, tokens, dim, k.device
-        # What the calls hand on: addresses, pages, distances and sizes.
-        self._fields = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, k.stride(0), k_scale.stride(0), heads, tokens, dim)
-        self._handle = (-1 if k.device.index is None else k.device.index, *self._fields)
+        if any(t.device != self.device for t in (k, v, k_scale, v_scale)):
+            raise ValueError("keys, values and scales must be on one device, the one that the cache was made on")
+        return (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, k.stride(0), k_scale.stride(0), heads, tokens, dim)
+
+    @property
+    def pages(self) -> int:
+        return self.k.shape[0]
+
+    @property
+    def heads(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def page_tokens(self) -> int:
+        return self.k.shape[2]
+
+    @property
+    def dim(self) -> int:
+        return self.k.shape[3]
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_tokens: int, dim: int, device) -> "CacheI8":
@@ -613,7 +632,7 @@ def _sequences(cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, cu:
         raise ValueError("page_table, lens and cu must agree in the number of sequences")
     if cu is None and rows != (rows // seqs * seqs if seqs else 0):
         raise ValueError("without cu every sequence has the same number of rows")
-    return (*cache._fields, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), cu.data_ptr() if cu is not None else 0,
+    return (*cache._fields(), page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), cu.data_ptr() if cu is not None else 0,
             seqs, rows)
 
 
@@ -626,7 +645,7 @@ def cache_write_i8(cache: CacheI8, k: torch.Tensor, v: torch.Tensor, page_table:
                    cu: torch.Tensor | None = None) -> CacheI8:
     """Quantise the rows ``k``, ``v`` [rows, heads, dim] (f32 / f16 / bf16) into ``cache`` on the current CUDA stream, as the last tokens of
     their sequences."""
-    if (_native or _front()).cache_write_i8(cache._handle, k, v, page_table, lens, cu) is not None:
+    if (_native or _front()).cache_write_i8(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, page_table, lens, cu) is not None:
         return cache
     kind = _float_type(k, "k")
     if v.dtype is not k.dtype:
@@ -646,7 +665,7 @@ def cache_read_i8(cache: CacheI8, page_table: torch.Tensor, lens: torch.Tensor, 
     if out is None:
         if rows is None:
             raise ValueError("rows or out is needed")
-        made = (_native or _front()).cache_read_i8(cache._handle, page_table, lens, rows, cu, out_dtype)
+        made = (_native or _front()).cache_read_i8(cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, lens, rows, cu, out_dtype)
         if made is not None:
             return made
         out = tuple(torch.empty((rows, cache.heads, cache.dim), dtype=out_dtype, device=cache.device) for _ in range(2))
@@ -671,7 +690,8 @@ def attention_i8_cache(q: torch.Tensor, cache: CacheI8, page_table: torch.Tensor
     """Attention of the rows ``q`` [rows, query heads, dim] (f32 / f16 / bf16), the last tokens of their sequences, over ``cache`` on the
     current CUDA stream.  Each group of query heads shares a head of the cache.  ``window``: a row sees that many tokens up to
     its own and the first ``sinks``; 0: all up to its own.  ``causal`` false: all of its sequence.  ``scale``: 1 / sqrt(dim)."""
-    made = (_native or _front()).attention_i8_cache(q, cache._handle, page_table, lens, cu, causal, window, sinks, scale, out, engine)
+    made = (_native or _front()).attention_i8_cache(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, lens, cu, causal, window,
+                                                       sinks, scale, out, engine)
     if made is not None:
         return made
     kind = _float_type(q, "q")

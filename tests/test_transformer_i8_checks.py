@@ -164,3 +164,57 @@ def test_what_the_front_end_refuses(nnb200_lib, monkeypatch):
         with pytest.raises(ValueError):
             ops._sequences(cache, *bad, 4)
     assert ops._sequences(cache, table, lens, None, 4)[-2:] == (2, 4)
+
+
+def test_a_cache_whose_tensors_are_replaced(nnb200_lib, monkeypatch):
+    """A call takes the tensors that the cache has then, wherever they lie, and not those it was made with."""
+    cache = ops.CacheI8.empty(4, 2, 16, 64, "cpu")
+    table, lens = torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+    class There:
+        type = "cuda"
+
+        def __eq__(self, other):
+            return other == torch.device("cpu")
+
+        __hash__ = None
+
+    cache.device = There()
+
+    def taken():
+        fields = ops._sequences(cache, table, lens, None, 4)
+        assert fields[:4] == tuple(t.data_ptr() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale))
+        assert fields[4:10] == (cache.k.shape[0], cache.k.stride(0), cache.k_scale.stride(0), *cache.k.shape[1:])
+        assert (cache.pages, cache.heads, cache.page_tokens, cache.dim) == tuple(cache.k.shape)
+
+    taken()
+    old = cache.k, cache.v, cache.k_scale, cache.v_scale
+    cache.k, cache.v = (torch.cat([t, t]) for t in old[:2])    # grown
+    with pytest.raises(ValueError):
+        ops._sequences(cache, table, lens, None, 4)    # its scales are not
+    cache.k_scale, cache.v_scale = (torch.cat([t, t]) for t in old[2:])
+    taken()
+    cache.k.data = torch.zeros_like(cache.k)    # another storage in the same tensor
+    taken()
+    for t in (cache.k, cache.v):
+        t.resize_(9, 2, 16, 64)
+    for t in (cache.k_scale, cache.v_scale):
+        t.resize_(9, 2)
+    taken()
+    cache.v = cache.v.transpose(1, 2)
+    with pytest.raises(ValueError):
+        ops._sequences(cache, table, lens, None, 4)
+    cache.v = old[1].short()
+    with pytest.raises(ValueError):
+        ops._sequences(cache, table, lens, None, 4)
+
+    # The compiled half is handed the same ones.
+    class Front:
+        def __getattr__(self, name):
+            return lambda *args: args
+
+    monkeypatch.setattr(ops, "_native", Front())
+    cache.k, cache.v, cache.k_scale, cache.v_scale = old
+    q = torch.zeros((4, 4, 64))
+    for args in (ops.attention_i8_cache(q, cache, table, lens)[1:], ops.cache_read_i8(cache, table, lens, rows=4)):
+        assert all(a is b for a, b in zip(args[:4], old))

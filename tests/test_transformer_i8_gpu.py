@@ -816,3 +816,29 @@ def test_a_block_of_a_model(cuda_device, nnb200_lib):
         codes, scale, h = ops.rms_norm_i8(y, norms[1].cuda(), residual=x.cuda())
         want, exact, sum_ = _norm_reference(y.cpu(), norms[1], x, 1e-6)
         assert torch.equal(codes.cpu(), want) and torch.equal(h.cpu(), sum_) and ((scale.cpu().double() - exact).abs() <= 2.0 ** -22 * exact).all()
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_a_cache_that_is_given_larger_tensors(cuda_device, nnb200_lib, monkeypatch, compiled):
+    """Between two calls a cache gets more pages: what it held is carried over by its owner, and nobody writes to the old tensors again."""
+    if not compiled:
+        monkeypatch.setattr(ops, "_native", ops._NoFront())
+    g = _gen(29)
+    cache = ops.CacheI8.empty(2, 2, 16, 64, "cuda")
+    x = _randn(g, 70, 2, 64).half().cuda()
+    ops.cache_write_i8(cache, x[:30], x[:30], _i32([[1, 0]]), _i32([30]))
+    old = cache.k, cache.v, cache.k_scale, cache.v_scale
+    kept = [t.clone() for t in old]
+    cache.k, cache.v, cache.k_scale, cache.v_scale = (torch.cat([t, torch.zeros_like(t), torch.zeros_like(t)]) for t in old)
+    assert cache.pages == 6
+    table = _i32([[1, 0, 5, 3, 2]])
+    ops.cache_write_i8(cache, x[30:], x[30:], table, _i32([70]))
+    q = _randn(g, 1, 4, 64).half().cuda()
+    got = ops.attention_i8_cache(q, cache, table, _i32([70]))
+    assert all(torch.equal(a, b) for a, b in zip(old, kept))
+    whole = ops.CacheI8.empty(6, 2, 16, 64, "cuda")
+    for low, high in ((0, 30), (30, 70)):
+        ops.cache_write_i8(whole, x[low:high], x[low:high], table, _i32([high]))
+    assert torch.equal(cache.k, whole.k) and torch.equal(cache.v_scale, whole.v_scale) and capi.take_device_error() == 0
+    assert torch.equal(got, ops.attention_i8_cache(q, whole, table, _i32([70])))
+    assert all(torch.equal(a, b) for a, b in zip(ops.cache_read_i8(cache, table, _i32([70]), rows=70), ops.cache_read_i8(whole, table, _i32([70]), rows=70)))
