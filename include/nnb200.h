@@ -480,7 +480,8 @@ NNB200_API int nnb200_dequantize_linear(const nnb200_quant_linear_args* args, vo
  *   scale = top / (127 * sqrt(mean_i h_i^2 + eps))
  * so out * scale is the normalised row, and (out, scale) are A and scale_a of nnb200_gemm_i8.  A row with a
  * NaN or an infinity in t gets scale NaN and codes 0.  residual_out may be x or residual itself (same
- * strides); no other output may overlap an input.  Strides are row strides in elements.
+ * strides) or lie between their rows, and is refused where it lies over them in another way; no other output may overlap an
+ * input.  Strides are row strides in elements.
  */
 typedef struct nnb200_rms_norm_i8_args {
     const void* x;        /* [rows][cols] */

@@ -1221,6 +1221,31 @@ bool rows_overlap(int64_t rows, int64_t stride_row, int64_t heads, int64_t strid
     return stride_row < stride_head ? stride_row < dim || stride_head / rows < stride_row : stride_head < dim || stride_row / heads < stride_head;
 }
 
+// Whether an output [rows][cols] lies over an input of the same type in another way than row upon row, or between its rows: then a row is
+// written before another block has read it.
+bool written_over(const void* in, int64_t in_stride, const void* out, int64_t out_stride, int64_t rows, int64_t cols, int64_t bytes)
+{
+    if (in == nullptr || out == nullptr || (in == out && (rows == 1 || in_stride == out_stride))) {
+        return false;
+    }
+    int64_t in_last, out_last;   // bytes from the first row to the last
+    if (__builtin_mul_overflow((rows - 1) * bytes, in_stride, &in_last) || __builtin_mul_overflow((rows - 1) * bytes, out_stride, &out_last)) {
+        return true;
+    }
+    const intptr_t a = reinterpret_cast<intptr_t>(in), b = reinterpret_cast<intptr_t>(out);
+    const int64_t row = cols * bytes;
+    const intptr_t a_low = in_last < 0 ? a + in_last : a, a_high = (in_last < 0 ? a : a + in_last) + row;
+    const intptr_t b_low = out_last < 0 ? b + out_last : b, b_high = (out_last < 0 ? b : b + out_last) + row;
+    if (a_high <= b_low || b_high <= a_low) {
+        return false;
+    }
+    if (rows == 1 || in_stride != out_stride) {
+        return true;
+    }
+    const int64_t pitch = out_stride * bytes, ahead = ((b - a) % pitch + pitch) % pitch;   // (an output's stride is at least cols)
+    return ahead < row || pitch - ahead < row;
+}
+
 int check_cache_rows(const nnb200_cache_rows_args* a, bool* empty)
 {
     if (a == nullptr || !float_type_ok(a->float_type)) {
@@ -1293,6 +1318,12 @@ int nnb200_rms_norm_i8(const nnb200_rms_norm_i8_args* args, void* stream)
     const int64_t last = args->rows > 1 ? args->cols : 0;
     if (args->out_stride < last || (args->residual_out != nullptr && args->residual_out_stride < last)) {
         return NNB200_INVALID_ARGUMENT;   // rows of an output that overlap
+    }
+    const auto over = [&](const void* in, int64_t stride) {
+        return written_over(in, stride, args->residual_out, args->residual_out_stride, args->rows, args->cols, static_cast<int64_t>(bytes));
+    };
+    if (over(args->x, args->x_stride) || over(args->residual, args->residual_stride)) {
+        return NNB200_INVALID_ARGUMENT;
     }
     const DeviceInfo* dev = current_device_info();
     if (dev == nullptr) {

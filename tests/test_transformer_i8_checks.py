@@ -218,3 +218,24 @@ def test_a_cache_whose_tensors_are_replaced(nnb200_lib, monkeypatch):
     q = torch.zeros((4, 4, 64))
     for args in (ops.attention_i8_cache(q, cache, table, lens)[1:], ops.cache_read_i8(cache, table, lens, rows=4)):
         assert all(a is b for a, b in zip(args[:4], old))
+
+
+def test_a_norm_that_would_write_over_rows_not_yet_read(nnb200_lib):
+    """residual_out upon x or residual: row for row, or nowhere.  (Rows of 64 f16 values, 128 bytes.)"""
+    call = nnb200_lib.nnb200_rms_norm_i8
+    before = nnb200_lib.nnb200_launch_count()
+    other = BASE + 0x40000
+    for name, at in (("x", BASE), ("residual", other)):
+        base = dict(rows=4, x_stride=128, residual=other, residual_stride=128, residual_out_stride=128)
+        for over in (dict(residual_out=at, residual_out_stride=64), dict(residual_out=at, residual_out_stride=136), dict(residual_out=at + 2),
+                     dict(residual_out=at + 126), dict(residual_out=at - 2), dict(residual_out=at + 256 * 3 + 126), dict(residual_out=at + 256 - 126),
+                     dict(residual_out=at + 128, residual_out_stride=64), {"residual_out": at, f"{name}_stride": 0},
+                     {"residual_out": at - 256 * 3, f"{name}_stride": -128}, {"residual_out": BASE + 0x90000, f"{name}_stride": 1 << 62}):
+            assert call(C.byref(_norm(**(base | over))), None) == capi.INVALID_ARGUMENT, (name, over)
+        assert call(C.byref(_norm(**(base | dict(rows=1, residual_out=at + 64)))), None) == capi.INVALID_ARGUMENT
+        # Row upon row, between the rows, before and behind them: no mistake, but there is no device here.
+        if not torch.cuda.is_available():
+            for over in (dict(residual_out=at), dict(residual_out=at + 128), dict(residual_out=at - 128), dict(residual_out=at - 256 * 3 - 128),
+                         dict(residual_out=at + 256 * 3 + 128, residual_out_stride=64), dict(rows=1, residual_out=at, residual_out_stride=5000)):
+                assert call(C.byref(_norm(**(base | over))), None) == capi.INTERNAL, (name, over)
+    assert nnb200_lib.nnb200_launch_count() == before
