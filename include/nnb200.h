@@ -479,7 +479,7 @@ NNB200_API int nnb200_dequantize_linear(const nnb200_quant_linear_args* args, vo
  *   out = round_half_even(t * (127 / top)) (f32, each step rounded once; the codes need no sum)
  *   scale = top / (127 * sqrt(mean_i h_i^2 + eps))
  * so out * scale is the normalised row, and (out, scale) are A and scale_a of nnb200_gemm_i8.  A row with a
- * NaN or an infinity in t gets scale NaN and codes 0.  residual_out may be x or residual itself (same
+ * NaN or an infinity in t gets scale NaN and codes 0, a row of no columns scale NaN (a mean over nothing).  residual_out may be x or residual itself (same
  * strides) or lie between their rows, and is refused where it lies over them in another way; no other output may overlap an
  * input.  Strides are row strides in elements.
  */

@@ -1306,11 +1306,12 @@ int nnb200_rms_norm_i8(const nnb200_rms_norm_i8_args* args, void* stream)
         (args->weight_type != args->float_type && args->weight_type != NNB200_FLOAT_F32)) {
         return NNB200_INVALID_ARGUMENT;
     }
-    if (args->rows == 0 || args->cols == 0) {
+    if (args->rows == 0) {
         return NNB200_OK;
     }
     const uintptr_t bytes = float_bytes(args->float_type);
-    if (args->x == nullptr || args->weight == nullptr || args->out == nullptr || args->scale == nullptr || !aligned(args->x, bytes) ||
+    const bool without = args->cols > 0 && (args->x == nullptr || args->weight == nullptr || args->out == nullptr);   // rows of nothing still have a scale
+    if (without || args->scale == nullptr || !aligned(args->x, bytes) ||
         !aligned(args->residual, bytes) || !aligned(args->residual_out, bytes) || !aligned(args->weight, float_bytes(args->weight_type)) ||
         !aligned(args->scale, 4)) {
         return NNB200_INVALID_ARGUMENT;

@@ -239,3 +239,12 @@ def test_a_norm_that_would_write_over_rows_not_yet_read(nnb200_lib):
                          dict(residual_out=at + 256 * 3 + 128, residual_out_stride=64), dict(rows=1, residual_out=at, residual_out_stride=5000)):
                 assert call(C.byref(_norm(**(base | over))), None) == capi.INTERNAL, (name, over)
     assert nnb200_lib.nnb200_launch_count() == before
+
+
+def test_a_norm_of_no_columns_is_a_call(nnb200_lib):
+    """Its rows have scales to be written: nothing but those is needed, and it is not answered with nothing done."""
+    call = nnb200_lib.nnb200_rms_norm_i8
+    assert call(C.byref(_norm(cols=0, scale=None)), None) == capi.INVALID_ARGUMENT
+    if not torch.cuda.is_available():
+        assert call(C.byref(_norm(cols=0, x=None, weight=None, out=None)), None) == capi.INTERNAL
+    assert call(C.byref(_norm(rows=0, cols=0, scale=None)), None) == capi.OK

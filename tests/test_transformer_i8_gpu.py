@@ -842,3 +842,17 @@ def test_a_cache_that_is_given_larger_tensors(cuda_device, nnb200_lib, monkeypat
     assert torch.equal(cache.k, whole.k) and torch.equal(cache.v_scale, whole.v_scale) and capi.take_device_error() == 0
     assert torch.equal(got, ops.attention_i8_cache(q, whole, table, _i32([70])))
     assert all(torch.equal(a, b) for a, b in zip(ops.cache_read_i8(cache, table, _i32([70]), rows=70), ops.cache_read_i8(whole, table, _i32([70]), rows=70)))
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_rows_without_columns(cuda_device, nnb200_lib, monkeypatch, dtype, compiled):
+    """A mean over nothing is no number, and says so: the scale is written whatever stood there."""
+    if not compiled:
+        monkeypatch.setattr(ops, "_native", ops._NoFront())
+    x, scale = torch.empty((5, 0), dtype=dtype, device="cuda"), torch.ones(5, device="cuda")
+    for residual in (None, torch.empty((5, 0), dtype=dtype, device="cuda")):
+        scale.fill_(1.0)
+        got = ops.rms_norm_i8(x, torch.empty(0, dtype=dtype, device="cuda"), residual=residual, scale=scale)
+        assert got[1] is scale or got[1].data_ptr() == scale.data_ptr()
+        assert scale.isnan().all() and got[0].shape == (5, 0)
