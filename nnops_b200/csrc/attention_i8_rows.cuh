@@ -7,8 +7,12 @@
 //
 // which is the softmax with each block's V scale moved into the exponent: the weights that meet the codes are then at
 // most 1 and the largest is 1 whatever the scales are, so that f16 holds them, and one exponential serves both sums.
-// One pass over the tokens, with the running maximum; the sums are rescaled only when that has grown by more than 2^8, so
-// weights are at most 2^8, and the lanes of a row compare their maxima only then.
+// One pass over the tokens, with the running maximum; the sums are rescaled only when that has grown by more than 2^8 (f32 rows: 2^2), and the
+// lanes of a row compare their maxima only then.  What is subtracted is not m but m - 7 (f32 rows: m - 13), which the quotient takes out
+// again: the largest weights lie between 2^7 (2^13) and 2^15, the upper end of f16's range, so that half of its least step, which a weight far below the
+// largest may be off by, is 2^-32 (2^-38) of the largest instead of 2^-25.  8192 tokens, the first
+// with nothing for values and a score 14 higher than the others': outputs 1.2e-3 off with weights up to 1 (f16 in tiles 2.5e-3), now 3.3e-4 of
+// f16's own step, 8.6e-7 with f32 rows.
 //
 // A warp takes 16 tokens at a time and is on its own: it copies their codes into its part of shared memory, a few groups ahead
 // (16 tokens never leave a page, and one head's share of a page is contiguous), turns bytes into f16
@@ -42,7 +46,12 @@ constexpr int kRowsThreads = 256; // of the joining kernel's blocks
 // Groups that a part of a row tile costs besides its own: queries, the first copies, joining the warps.  With 16, 32 and 64, 8 heads of 128: 64 sequences of
 // 128 to 8192 tokens 114, 96 and 98 us, 255 of 16 to 128 and one of 30000 70, 65 and 78, 120 of 100 and 8 of 20000 94, 78 and 95.
 constexpr int kRowsCost = 32;
-constexpr float kGrowth = 8.0f;   // log2 of what a weight may be
+constexpr float kMostWeight = 15.0f;   // log2 of what a weight may be: f16 ends at 65504
+// log2 of the largest weight when the sums have just been rescaled.
+constexpr float rows_top_weight(bool split) { return split ? 13.0f : 7.0f; }
+// From here on the steps of f32 are no longer small against the room above 2^15: the largest weight is 1 there.
+constexpr float kCoarse = 4194304.0f;   // 2^22
+__device__ __forceinline__ bool is_coarse(float m) { return fabsf(m) >= kCoarse && fabsf(m) < INFINITY; }
 
 // A row tile of a head that begins in a block and ends in a later one.  What a block leaves of its sums: [0] the end or the middle of
 // one that began in an earlier block, [1] the beginning of one that ends in a later block.
@@ -343,6 +352,7 @@ attention_i8_rows_kernel(const RowsCall call)
     constexpr int kStages = Shared::kStages, kWarps = Shared::kWarps, kThreads = Shared::kThreads;
     constexpr int kTile = 8 * NT;
     constexpr int kParts = SPLIT ? 2 : 1;
+    constexpr float kTop = rows_top_weight(SPLIT);
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ StageScales scales[kWarps][kStages];
     __shared__ float join_m[kWarps][kTile], join_l[kWarps][kTile];
@@ -598,7 +608,7 @@ attention_i8_rows_kernel(const RowsCall call)
         const int least_pos = a.causal != 0 ? first_pos + tile * kTile / call.group : 0x7FFFFFFF;
         const int most_pos = a.causal != 0 ? first_pos + (tile * kTile + rows - 1) / call.group : 0x7FFFFFFF;
 
-        float m[NT][2], l[NT][2], o[NT][D / 16][4];
+        float m[NT][2], l[NT][2], o[NT][D / 16][4];   // m: the maximum less kTop
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = -INFINITY;
@@ -671,7 +681,7 @@ attention_i8_rows_kernel(const RowsCall call)
                 for (int nt = 0; nt < NT; ++nt) {
                     largest = fmaxf(largest, fmaxf(fmaxf(x[nt][0], x[nt][1]), fmaxf(x[nt][2], x[nt][3])));
                 }
-                if (__any_sync(0xFFFFFFFFu, largest > kGrowth)) {
+                if (__any_sync(0xFFFFFFFFu, largest > kMostWeight)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float alpha[2];
@@ -684,7 +694,7 @@ attention_i8_rows_kernel(const RowsCall call)
                             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
                             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
                             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                            const float next = fmaxf(m[nt][j], top), safe = next == -INFINITY ? 0.0f : next;
+                            const float next = fmaxf(m[nt][j], is_coarse(top) ? top : top - kTop), safe = next == -INFINITY ? 0.0f : next;
                             alpha[j] = exp2_fast(m[nt][j] - safe);
                             m[nt][j] = next;
                             l[nt][j] *= alpha[j];

@@ -17,8 +17,8 @@
 // marks blocks that some row does not see all of, and asks for the queries that come next.  Softmax warps need more registers than
 // the rest: the groups of four trade them (152, 112 and 96 of a thread's; 128 at launch).
 //
-// The sums are rescaled only when a row's maximum has grown by more than 2^8 since they were last: until then weights are at
-// most 2^8, which f16 and the f32 sums hold as well as 1.
+// The sums are rescaled only when a row's maximum has grown by more than 2^8 since they were last.  Weights are 2^7 times what the formula has, so
+// that the largest is between 2^7 and 2^15 and f16 holds more of those far below it (attention_i8_rows.cuh).
 //
 // Sequences, tiles and heads are one line of 128-token blocks, cut into equal pieces, as in attention_i8_rows.cuh; a first
 // kernel writes down which tiles there are.
@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
         int which = 0;
         T* dst = nullptr;
         TilePiece about{};
-        float m = 0.0f, l = 0.0f;
+        constexpr float kTop = rows_top_weight(false);
+        float m = 0.0f, l = 0.0f;   // m: the maximum less kTop
         bool ok = true, more = walk.next(call);
         while (more || pending) {
             // The scores of the part before are all there, so its queries may go, and the next one's first products come right
@@ -579,6 +580,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
             }
             m = -INFINITY;
             l = 0.0f;
+            float most = kMostWeight;   // of a weight's log2; less where its own rounding may be more than half
             const int count = walk.count;
 #pragma unroll 1
             for (int i = 0; i < kParts * count; ++i) {
@@ -648,9 +650,10 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                 for (int g = 1; g < kPartGroups; ++g) {
                     top = fmaxf(top, tops[g]);
                 }
-                const bool grown = top > m + 8.0f || (m == -INFINITY && top > m);
+                const bool grown = top - m > most;   // (not top > m + most: a sum that is rounded up would let a larger weight pass)
                 if (__any_sync(0xFFFFFFFFu, grown)) {
-                    const float next = grown ? top : m;
+                    const float next = grown ? (is_coarse(top) ? top : top - kTop) : m;
+                    most = is_coarse(next) ? kMostWeight - kTop : kMostWeight;
                     const float alpha = grown ? exp2_fast(m - next) : 1.0f;
                     m = next;
                     l *= alpha;
