@@ -559,8 +559,9 @@ NNB200_API int nnb200_cache_read_i8(const nnb200_cache_rows_args* args, void* st
  *   out = sum_j softmax_j(scale * q . k_j) v_j   over the visible tokens j < lens[b]:
  *   causal: j <= p, and with window > 0 also j > p - window or j < sinks; else all of them.
  * A row that sees no token gives zeros, whatever its q holds.  dim 64, 96, 128 or 256.  The products take q and the softmax weights as
- * f16 (f16 q as it is, bf16 q scaled by a power of two of its row's, f32 q and its weights as the sum of two f16 values, 2^-22 of the
- * row's largest), codes exactly, and sum in f32; the softmax is f32.  A weight, p_j times the v scale of its page, is off by at most 2^-11
+ * f16 (f16 q as it is, bf16 and f32 q scaled by a power of two of their row's, f32 q and its weights as the sum of two f16 values), codes
+ * exactly, and sum in f32; the softmax is f32.  A value of bf16 q is off by at most 2^-38 of its row's largest (counted as 2^-100 at least), of
+ * f32 q by that or 2^-22 of itself, whichever is more.  A weight, p_j times the v scale of its page, is off by at most 2^-11
  * of itself (f32 q: 2^-22), or 2^-32 (2^-38) of the row's largest where that is more.  Scores, scale * q . k, go up to 2^25: beyond, the
  * steps of f32 exceed what is left of f16's range, and rows of engine 2 may come out as no number.  A page whose v scale is under
  * 2^-60 counts as having that scale.  Rows of out may not overlap, nor any of them an input.

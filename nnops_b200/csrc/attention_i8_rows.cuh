@@ -53,6 +53,11 @@ constexpr float rows_top_weight(bool split) { return split ? 13.0f : 7.0f; }
 constexpr float kCoarse = 4194304.0f;   // 2^22
 __device__ __forceinline__ bool is_coarse(float m) { return fabsf(m) >= kCoarse && fabsf(m) < INFINITY; }
 
+// By which power of two a row of bf16 or f32 is divided to be f16: its largest value, of these bits, comes to 2^13 (2^15 at the end of the range), so
+// that values as far below it as a loud channel leaves the others keep their bits.  (Queries whose first channel is 2^20 times the others, where keys have
+// zeros: 0.027 off with the largest at 1, now 0.0024, bf16's own step; f32 and 2^14: 4.6e-4, now 6.7e-7.)  2^-113 to 2^113: it and its reciprocal are normal.
+__device__ __forceinline__ int row_exponent(uint32_t top) { return min(max(static_cast<int>(top >> 23) - 140, -113), 113); }
+
 // A row tile of a head that begins in a block and ends in a later one.  What a block leaves of its sums: [0] the end or the middle of
 // one that began in an earlier block, [1] the beginning of one that ends in a later block.
 struct RowsPiece {
@@ -553,7 +558,7 @@ attention_i8_rows_kernel(const RowsCall call)
             }
             cp_async_commit();
         }
-        // In f16, scaled by a power of two.
+        // In f16, bf16 and f32 scaled by a power of two.
         uint32_t q[NT][kParts][D / 16][2];
         float factor[NT][2];    // of the columns 2 c and 2 c + 1
         int pos[NT][2];
@@ -581,8 +586,7 @@ attention_i8_rows_kernel(const RowsCall call)
             }
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            int e = a.float_type == NNB200_FLOAT_F16 ? 0 : static_cast<int>(top >> 23) - 127;
-            e = min(max(e, -100), 126);
+            const int e = a.float_type == NNB200_FLOAT_F16 ? 0 : row_exponent(top);
             const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
             const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * call.factor;
 #pragma unroll

@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(TileShared<D>::kThreads, 1) attention_i8_tile_
                     }
                     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                    const int e = min(max(static_cast<int>(top >> 23) - 127, -100), 126);
+                    const int e = row_exponent(top);
                     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
                     const float up = call.factor * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                     const float mine = __shfl_sync(0xFFFFFFFFu, up, lane % 8 * 4);

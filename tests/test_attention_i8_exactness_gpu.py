@@ -1,5 +1,5 @@
-"""Attention over the 8-bit cache where few bits would show: weights far below a row's largest, large scores, long contexts of
-which every token counts.  Each row's output is compared as a vector with 64 bits, relative to its own length."""
+"""Attention over the 8-bit cache where few bits would show: weights far below a row's largest, queries with one loud channel,
+large scores, long contexts of which every token counts.  Each row's output is compared as a vector with 64 bits, relative to its own length."""
 import math
 
 import pytest
@@ -91,6 +91,49 @@ def test_a_first_token_far_above_the_rest(cuda_device, nnb200_lib, dtype, engine
             least[:, a] = (z[:, 0] * 10) * (v.double().square().sum() - 127 ** 2).sqrt() / want[:, a].norm(dim=1)
     off = _distance(got, want)
     assert (off <= _bound(dtype, top, least)).all(), (off.max().item(), _bound(dtype, top, least).min().item())
+
+
+@pytest.mark.parametrize("dtype,engine", [f for f in FORMS if f[0] is not torch.float16])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_a_loud_channel_of_the_queries(cuda_device, nnb200_lib, dtype, engine, dim):
+    """2^14 (f32) or 2^20 (bf16) times the others, where keys have nothing: the scores are the other channels'."""
+    g = torch.Generator().manual_seed(dim)
+    length, tokens, group, n = 500, 16, 2, 40
+    pages = -(-length // tokens)
+    k, v = (torch.randint(-127, 128, (pages, 1, tokens, dim), generator=g, dtype=torch.int32).to(torch.int8) for _ in range(2))
+    k[..., 3] = 0
+    scales = torch.full((pages, 1), 1 / 73.3), torch.full((pages, 1), 0.01)
+    q = torch.randn((n, 2, dim), generator=g)
+    q[..., 3] = 2.0 ** 14 if dtype is torch.float32 else 2.0 ** 20
+    q = q.to(dtype)
+    want, least, top = _exact(q, (k, v), scales, list(range(pages)), length, group)
+    cache = ops.CacheI8(k.cuda(), v.cuda(), *(s.cuda() for s in scales))
+    got = ops.attention_i8_cache(q.cuda(), cache, _i32([list(range(pages))]), _i32([length]), engine=engine).cpu().double()
+    # Besides: a query's values to 2^-22 of each, and its product with a key in dim / 16 steps of 2^-23 of what its terms come to.
+    products = (q.double().abs() @ k.double().abs().flatten(0, 2).T / 73.3 / math.sqrt(dim)).amax(-1)
+    products[...] = products.amax()
+    off = _distance(got, want)
+    bound = _bound(dtype, top, least) + 2 * (2.0 ** -22 + dim / 16 * 2.0 ** -23) * products
+    assert (off <= bound).all(), (off.max().item(), bound.min().item())
+
+
+@pytest.mark.parametrize("dtype,engine", [f for f in FORMS if f[0] is not torch.float16])
+@pytest.mark.parametrize("power", [-113, -100, -60, 60, 100, 113, 126])
+def test_queries_of_any_size(cuda_device, nnb200_lib, dtype, engine, power):
+    """Queries of 2^power against keys of 2^-power: the scores of ordinary ones, from the same bits; nothing overflows on the way."""
+    g = torch.Generator().manual_seed(5)
+    length, dim, tokens, n = 200, 64, 16, 20
+    pages = -(-length // tokens)
+    k, v = (torch.randint(-127, 128, (pages, 1, tokens, dim), generator=g, dtype=torch.int32).to(torch.int8) for _ in range(2))
+    scales = torch.full((pages, 1), 2.0 ** -6), torch.full((pages, 1), 2.0 ** -7)
+    q = torch.randn((n, 2, dim), generator=g).clamp(-1.9, 1.9).to(dtype)
+    want, least, top = _exact(q, (k, v), scales, list(range(pages)), length, 2)
+    cache = ops.CacheI8(k.cuda(), v.cuda(), (scales[0] * 2.0 ** -power).cuda(), scales[1].cuda())
+    got = ops.attention_i8_cache((q.double() * 2.0 ** power).to(dtype).cuda(), cache, _i32([list(range(pages))]), _i32([length]), engine=engine)
+    products = (q.double().abs() @ k.double().abs().flatten(0, 2).T * 2.0 ** -6 / math.sqrt(dim)).amax()
+    off = _distance(got.cpu().double(), want)
+    bound = _bound(dtype, top, least) + 2 * (2.0 ** -22 + dim / 16 * 2.0 ** -23) * products
+    assert (off <= bound).all(), (off.max().item(), bound.min().item())
 
 
 @pytest.mark.parametrize("dtype,engine,dim,lens,new,window,sinks", [
