@@ -540,7 +540,7 @@ typedef struct nnb200_cache_i8 {
  * not overwritten becomes round_half_even(code * (old / new)).  New codes: round_half_even(x * (1 / scale)).  A NaN or
  * an infinity among the new values makes the page's scale NaN until it begins anew: every value of it then reads as NaN.
  * A page that a call writes belongs to one sequence, and stands once in its row of the table: otherwise what
- * it holds afterwards is not defined.  Rows that read writes may not overlap.
+ * it holds afterwards is not defined.  Rows that read writes may not overlap, nor keys' and values'.
  */
 typedef struct nnb200_cache_rows_args {
     nnb200_cache_i8 cache;

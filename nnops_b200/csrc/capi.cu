@@ -1355,7 +1355,8 @@ int nnb200_cache_read_i8(const nnb200_cache_rows_args* args, void* stream)
         return status;
     }
     const nnb200_cache_i8& c = args->cache;
-    if (rows_overlap(c.rows, args->k_stride_row, c.heads, args->k_stride_head, c.dim) || rows_overlap(c.rows, args->v_stride_row, c.heads, args->v_stride_head, c.dim)) {
+    if (args->k == args->v || rows_overlap(c.rows, args->k_stride_row, c.heads, args->k_stride_head, c.dim) ||
+        rows_overlap(c.rows, args->v_stride_row, c.heads, args->v_stride_head, c.dim)) {
         return NNB200_INVALID_ARGUMENT;
     }
     const DeviceInfo* dev = current_device_info();

@@ -248,3 +248,13 @@ def test_a_norm_of_no_columns_is_a_call(nnb200_lib):
     if not torch.cuda.is_available():
         assert call(C.byref(_norm(cols=0, x=None, weight=None, out=None)), None) == capi.INTERNAL
     assert call(C.byref(_norm(rows=0, cols=0, scale=None)), None) == capi.OK
+
+
+def test_keys_and_values_read_into_one_place(nnb200_lib):
+    """Which of the two it would hold depended on timing.  To be written they may be the same."""
+    same = _cache(capi.CacheRowsArgs, rows_k=BASE + 0x40000, rows_v=BASE + 0x40000)
+    assert nnb200_lib.nnb200_cache_read_i8(C.byref(same), None) == capi.INVALID_ARGUMENT
+    if not torch.cuda.is_available():
+        assert nnb200_lib.nnb200_cache_write_i8(C.byref(same), None) == capi.INTERNAL
+        apart = _cache(capi.CacheRowsArgs, k_stride_row=256, v_stride_row=256, rows_v=BASE + 0x40000 + 256)    # in rows of both
+        assert nnb200_lib.nnb200_cache_read_i8(C.byref(apart), None) == capi.INTERNAL
