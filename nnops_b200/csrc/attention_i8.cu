@@ -14,7 +14,9 @@ constexpr int kEngineTile = 2;
 constexpr int64_t kClusterTokens = 16384;
 constexpr int64_t kMostTokens = int64_t{1} << 31;   // a sequence has fewer
 
-// Query rows that share a sequence's head, on average where their numbers are the device's.
+// Query rows that share a sequence's head, on average where their numbers are the device's.  One kernel does the whole call, so a batch that mixes
+// single tokens with a prompt's chunk is served by the one that suits neither: 63 tokens and a chunk of 200 or 512 rows, 4096 tokens each, 8 heads of 128
+// with 8 rows, 344 and 391 us, as two calls 153 and 196.
 int64_t rows_each(const nnb200_attention_i8_args& a)
 {
     const nnb200_cache_i8& c = a.cache;

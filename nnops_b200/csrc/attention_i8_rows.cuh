@@ -10,9 +10,9 @@
 // One pass over the tokens, with the running maximum; the sums are rescaled only when that has grown by more than 2^8 (f32 rows: 2^2), and the
 // lanes of a row compare their maxima only then.  What is subtracted is not m but m - 7 (f32 rows: m - 13), which the quotient takes out
 // again: the largest weights lie between 2^7 (2^13) and 2^15, the upper end of f16's range, so that half of its least step, which a weight far below the
-// largest may be off by, is 2^-32 (2^-38) of the largest instead of 2^-25.  8192 tokens, the first
-// with nothing for values and a score 14 higher than the others': outputs 1.2e-3 off with weights up to 1 (f16 in tiles 2.5e-3), now 3.3e-4 of
-// f16's own step, 8.6e-7 with f32 rows.
+// largest may be off by, is 2^-32 (2^-38) of the largest instead of 2^-25.  Of 8192 tokens the first with
+// nothing for values and a score 14 higher than the others': with the largest weights at 1 outputs were 1.2e-3 off (f32 rows; f16 in tiles 2.5e-3), now
+// 8.6e-7 (3.7e-4, f16's own steps).
 //
 // A warp takes 16 tokens at a time and is on its own: it copies their codes into its part of shared memory, a few groups ahead
 // (16 tokens never leave a page, and one head's share of a page is contiguous), turns bytes into f16
@@ -25,8 +25,9 @@
 //
 // Bound by the reading of the codes, 2 D bytes for a token and head, and close behind it by instructions: about 280 of a warp for 16
 // tokens of 64 dims and 8 rows, 440 of 128 dims, 50 to 75 more for each 8 rows more.  Measured on one B200: 64 sequences of 128 to 8192 tokens, 8 heads of
-// 128, 8 rows: 95.5 us, 5.7 TB/s (0.88 of the measured copy rate; 107 us with nothing left in L2); 64 sequences of 4096 tokens, 8 heads: heads of
-// 64 with 8, 16 and 32 rows 62, 87 and 132 us, heads of 128 with 8 rows 98 us; 16 sequences behind a window of 4096, 24 rows of 64: 37 us.
+// 128, 8 rows: 108 us, 5.1 TB/s (0.79 of the measured copy rate; 98 us where the same call comes again and finds a part in L2); the same call again,
+// 64 sequences of 4096 tokens, 8 heads: heads of 64 with 8, 16 and 32 rows 62, 86 and 130 us, heads of 128 with 8 rows 96 us, f32 rows 128; 16 sequences
+// behind a window of 4096, 24 rows of 64: 37 us.
 //
 // The work of all sequences, row tiles and heads is one line of 16-token groups, cut into equal pieces, one for each block, so
 // that lengths of any mix keep every SM busy to the end.  A row tile of a head that is cut leaves (m, l, sums) in the
@@ -34,7 +35,7 @@
 //
 // A few row tiles over contexts that cannot be long, all sequences with as many rows, go to a cluster of eight blocks each instead:
 // their sums meet in shared memory, without a workspace, a search for one's place or a second kernel.  One sequence of 4096 tokens, 8 heads of
-// 128: 9.1 us, with the line and its second kernel 14.
+// 128: 9.4 us, with the line and its second kernel 14.8.
 #pragma once
 
 #include "cache_i8.cuh"
@@ -89,7 +90,9 @@ struct RowsCall {
     float* sums;         // [blocks][2][piece]
 };
 
-// One sequence's part of the line.
+// One sequence's part of the line.  Its row tiles are all as long: from what its first row sees to its last token.  That is nothing to speak of for the
+// few rows that this kernel is for; f32 prompts, which have no other, take up to twice the groups that they see (8192 rows of 32 heads of 128: 9.97 ms), and
+// behind a window as many as without one (of 256: 10.4 ms).
 struct SequenceWork {
     SequenceRows s;
     int sink_groups, first_group, groups;   // groups of a row tile: the sinks', then those from first_group on; 1 at least
@@ -304,7 +307,8 @@ constexpr int rows_warps(int64_t dim, int columns, bool split)
     return rows_blocks(dim, columns, split) == 1 && rows_weight(dim, columns, split) <= 128 ? 12 : 8;
 }
 
-// Beyond these the sums no longer fit the registers.
+// At these the sums all but fit the registers (of a thread's 255, bytes that are spilled, on the line and in clusters: heads of 256 with 16 rows 308 and
+// 188, of 96 with 32 rows 200 and 12, of 128 with 24 rows 8 and 0, all others none); with eight rows more they do not.
 constexpr int rows_most_columns(int64_t dim, bool split) { return split ? (dim > 128 ? 1 : 2) : dim > 128 ? 2 : dim > 96 ? 3 : 4; }
 
 template <int D, int NT, bool SPLIT>
@@ -490,7 +494,7 @@ attention_i8_rows_kernel(const RowsCall call)
         const int rows = min(kTile, work.s.n * call.group - tile * kTile);
         const int first_pos = work.s.len - work.s.n;
 
-        // This warp's groups of the piece: off + warp, off + warp + 8, ...
+        // This warp's groups of the piece: off + warp, off + warp + kWarps, ...
         const int mine = count > warp ? (count - warp + kWarps - 1) / kWarps : 0;
         const auto group_of = [&](int i) {
             const int idx = off + warp + i * kWarps;

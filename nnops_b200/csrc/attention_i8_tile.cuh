@@ -15,7 +15,8 @@
 // while the second is computed.  One warp issues all MMAs, in the order that the halves take turns in: scores come over the weights whose
 // products it has issued before.  Another, the scout, looks up each block's pages and scales (one for each 16 tokens) ahead of everyone,
 // marks blocks that some row does not see all of, and asks for the queries that come next.  Softmax warps need more registers than
-// the rest: the groups of four trade them (152, 112 and 96 of a thread's; 128 at launch).
+// the rest: the groups of four trade them (152, 112 and 96 of a thread's; 128 at launch; 20 bytes are
+// spilled with heads of 96, 56 and 48 with bf16 and heads of 128 and 256).
 //
 // The sums are rescaled only when a row's maximum has grown by more than 2^8 since they were last.  Weights are 2^7 times what the formula has, so
 // that the largest is between 2^7 and 2^15 and f16 holds more of those far below it (attention_i8_rows.cuh).
@@ -24,8 +25,9 @@
 // kernel writes down which tiles there are.
 //
 // Bound by the chain from scores over weights to products, of which two are under way, on warps that issue in 46 % of the cycles; tensor cores, exponentials and
-// integer units are busy for 38 % of the time each.  Measured on one B200: 8192 rows of 32 heads of 128, causal: 650 us, 845 TFLOP/s (0.50 of the measured
-// bf16 rate); 8 chunks of 288 rows over 9216 tokens 398 us; 2048 rows 76 us; 8192 rows of 64: 545 us; 4096 of 256: 490 us.  Not faster: scores of 64
+// integer units are busy for 38 % of the time each.  Measured on one B200: 8192 rows of 32 heads of 128, causal: 686 us, 802 TFLOP/s (0.48 of the measured
+// bf16 rate); the same call again and again 652 us, 8 chunks of 288 rows over 9216 tokens 396 us, 2048 rows 79 us, 8192 rows of 64 540 us, of 96 600 us, 4096 of
+// 256 488 us.  Not faster: scores of 64
 // tokens at a time, also into tensor memory of their own (for heads of 64); one part instead of two; weights ahead of the maximum, made up for
 // afterwards; two threads to a row; what a row sees of a block applied to registers instead of to tensor memory; a part of the exponentials as polynomials
 // (one in eight 2 % slower, half 13 %); one issuing warp for each half, which would also need an order between the two.

@@ -689,7 +689,8 @@ def attention_i8_cache(q: torch.Tensor, cache: CacheI8, page_table: torch.Tensor
                        engine: str = "auto") -> torch.Tensor:
     """Attention of the rows ``q`` [rows, query heads, dim] (f32 / f16 / bf16), the last tokens of their sequences, over ``cache`` on the
     current CUDA stream.  Each group of query heads shares a head of the cache.  ``window``: a row sees that many tokens up to
-    its own and the first ``sinks``; 0: all up to its own.  ``causal`` false: all of its sequence.  ``scale``: 1 / sqrt(dim)."""
+    its own and the first ``sinks``; 0: all up to its own.  ``causal`` false: all of its sequence.  ``scale``: 1 / sqrt(dim).  Single tokens and chunks of
+    prompts are faster in a call each than mixed in one."""
     made = (_native or _front()).attention_i8_cache(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, lens, cu, causal, window,
                                                        sinks, scale, out, engine)
     if made is not None:
