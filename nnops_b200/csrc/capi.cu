@@ -1225,24 +1225,20 @@ bool rows_overlap(int64_t rows, int64_t stride_row, int64_t heads, int64_t strid
 // written before another block has read it.
 bool written_over(const void* in, int64_t in_stride, const void* out, int64_t out_stride, int64_t rows, int64_t cols, int64_t bytes)
 {
-    if (in == nullptr || out == nullptr || (in == out && (rows == 1 || in_stride == out_stride))) {
+    using Wide = __int128;   // any stride times any number of rows
+    if (in == nullptr || out == nullptr || cols == 0 || (in == out && (rows == 1 || in_stride == out_stride))) {
         return false;
     }
-    int64_t in_last, out_last;   // bytes from the first row to the last
-    if (__builtin_mul_overflow((rows - 1) * bytes, in_stride, &in_last) || __builtin_mul_overflow((rows - 1) * bytes, out_stride, &out_last)) {
-        return true;
-    }
-    const intptr_t a = reinterpret_cast<intptr_t>(in), b = reinterpret_cast<intptr_t>(out);
-    const int64_t row = cols * bytes;
-    const intptr_t a_low = in_last < 0 ? a + in_last : a, a_high = (in_last < 0 ? a : a + in_last) + row;
-    const intptr_t b_low = out_last < 0 ? b + out_last : b, b_high = (out_last < 0 ? b : b + out_last) + row;
-    if (a_high <= b_low || b_high <= a_low) {
+    const Wide a = reinterpret_cast<uintptr_t>(in), b = reinterpret_cast<uintptr_t>(out), row = static_cast<Wide>(cols) * bytes;
+    const Wide a_last = a + static_cast<Wide>(rows - 1) * in_stride * bytes, b_last = b + static_cast<Wide>(rows - 1) * out_stride * bytes;
+    const Wide a_low = a < a_last ? a : a_last, b_low = b < b_last ? b : b_last;
+    if ((a < a_last ? a_last : a) + row <= b_low || (b < b_last ? b_last : b) + row <= a_low) {
         return false;
     }
     if (rows == 1 || in_stride != out_stride) {
         return true;
     }
-    const int64_t pitch = out_stride * bytes, ahead = ((b - a) % pitch + pitch) % pitch;   // (an output's stride is at least cols)
+    const Wide pitch = static_cast<Wide>(out_stride) * bytes, ahead = ((b - a) % pitch + pitch) % pitch;   // (an output's stride is at least cols)
     return ahead < row || pitch - ahead < row;
 }
 

@@ -230,7 +230,8 @@ def test_a_norm_that_would_write_over_rows_not_yet_read(nnb200_lib):
         for over in (dict(residual_out=at, residual_out_stride=64), dict(residual_out=at, residual_out_stride=136), dict(residual_out=at + 2),
                      dict(residual_out=at + 126), dict(residual_out=at - 2), dict(residual_out=at + 256 * 3 + 126), dict(residual_out=at + 256 - 126),
                      dict(residual_out=at + 128, residual_out_stride=64), {"residual_out": at, f"{name}_stride": 0},
-                     {"residual_out": at - 256 * 3, f"{name}_stride": -128}, {"residual_out": BASE + 0x90000, f"{name}_stride": 1 << 62}):
+                     {"residual_out": at - 256 * 3, f"{name}_stride": -128}, dict(residual_out=BASE - 0x1000, residual_out_stride=1 << 61),
+                     {"residual_out": BASE + 0x90000, f"{name}_stride": 1 << 62}, {"residual_out": BASE + 0x90000, f"{name}_stride": (1 << 63) - 1}):
             assert call(C.byref(_norm(**(base | over))), None) == capi.INVALID_ARGUMENT, (name, over)
         assert call(C.byref(_norm(**(base | dict(rows=1, residual_out=at + 64)))), None) == capi.INVALID_ARGUMENT
         # Row upon row, between the rows, before and behind them: no mistake, but there is no device here.
@@ -246,6 +247,8 @@ def test_a_norm_of_no_columns_is_a_call(nnb200_lib):
     call = nnb200_lib.nnb200_rms_norm_i8
     assert call(C.byref(_norm(cols=0, scale=None)), None) == capi.INVALID_ARGUMENT
     if not torch.cuda.is_available():
+        # Rows of nothing lie nowhere.
+        assert call(C.byref(_norm(cols=0, rows=4, residual=BASE + 64, residual_out=BASE + 2, residual_out_stride=1, x_stride=3)), None) == capi.INTERNAL
         assert call(C.byref(_norm(cols=0, x=None, weight=None, out=None)), None) == capi.INTERNAL
     assert call(C.byref(_norm(rows=0, cols=0, scale=None)), None) == capi.OK
 
